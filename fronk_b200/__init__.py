@@ -22,6 +22,8 @@ RUN_RMSNORM = 1
 RUN_OVERLAP = 2
 RUN_PEER = 4
 RUN_X_BF16 = 8
+F32, BF16 = 0, 1      # element types of device buffers
+ROUTE_SHARED = 1
 PEER_HANDLE_BYTES = 64
 MAX_BLOCKS, ROUTED, SHARED, TOPK, ACTIVE, NEURONS, MAX_TOKENS = 20, 512, 512, 10, 11, 32, 16
 MAX_PREFILL_TOKENS = 512
@@ -114,6 +116,16 @@ _SIGS = {
     "frc_prefill_timing": (_int, [_vp, _int]),
     "frc_prefill_times": (_int, [_vp, _vp]),
     "frc_debug_phases": (_int, [_vp, _vp, _sz, _vp]),
+    "frc_matrix_check": (_int, [_u32, _u32, _u32]),
+    "frc_matrix_open": (_int, [_vp, _u32, _u32, _u32, _vp, _sz, _vp]),
+    "frc_matrix_close": (_int, [_vp]),
+    "frc_matvec_device": (_int, [_vp, _vp, _u32, _vp, _sz, _u32, _vp, _sz, _u32, _vp]),
+    "frc_routing_check": (_int, [_u32, _u32, _sz, _u32, _u32]),
+    "frc_balance_workspace": (_sz, [_u32, _u32]),
+    "frc_route_device": (_int, [_vp, _u32, _u32, _vp, _sz, _u32, _vp, _vp, _vp, _u32, _vp, _vp]),
+    "frc_balance_device": (_int, [_vp, _u32, _u32, _vp, _sz, _u32, _vp, _vp, _vp, _vp]),
+    "frc_route_backward_device": (_int, [_vp, _u32, _u32, _vp, _sz, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _u32,
+                                         _vp]),
 }
 EXPORTS = sorted(_SIGS) + ["fr_cuda", "fr_cuda_f32", "fr_cuda_avx2", "fr_cuda_select_device", "fr_cuda_close",
                           "fr_cuda_avx2_workers"]
@@ -179,6 +191,68 @@ class CostModel(ctypes.Structure):
     """frc_costmodel (the fields and meaning of the reference's fr_costmodel)."""
     _fields_ = [("burst_max", ctypes.c_uint), ("t0_ns", ctypes.c_double), ("bw_eff", ctypes.c_double),
                 ("ns", ctypes.c_double * 8), ("bytes", ctypes.c_uint64 * 8)]
+
+
+class Balance(ctypes.Structure):
+    """frc_balance: device pointers of the balance statistics' outputs and the call's workspace."""
+    _fields_ = [("loss", _vp), ("count", _vp), ("prob", _vp), ("workspace", _vp), ("workspace_bytes", _sz)]
+
+
+def balance_workspace(tokens, experts):
+    """Bytes of the workspace a balance call of these sizes needs (frc_balance_workspace)."""
+    n = library().frc_balance_workspace(tokens, experts)
+    if not n:
+        raise FrcError(INVALID, "balance_workspace", "%d tokens, %d experts" % (tokens, experts))
+    return n
+
+
+def matrix_check(type_, rows, n):
+    """Status code of frc_matrix_check."""
+    return library().frc_matrix_check(type_, rows, n)
+
+
+def routing_check(tokens, experts, stride, type_=F32, flags=0):
+    """Status code of frc_routing_check."""
+    return library().frc_routing_check(tokens, experts, stride, type_, flags)
+
+
+class Matrix:
+    """A dense 4-bit matrix in HBM (frc_matrix); made by Context.matrix."""
+
+    def __init__(self, ctx, type_, rows, n, data, nbytes=None):
+        self.lib, self.ctx, self.type, self.rows, self.n = ctx.lib, ctx, type_, rows, n
+        self.h = None
+        if nbytes is None:
+            data = np.ascontiguousarray(data, np.uint8)
+            src, nbytes = data.ctypes.data, data.nbytes
+        else:
+            src = data
+        h = ctypes.c_void_p()
+        ctx._check(self.lib.frc_matrix_open(ctx.h, type_, rows, n, src, nbytes, ctypes.byref(h)), "matrix_open")
+        self.h = h
+
+    def matvec_device(self, tokens, x_ptr, y_ptr, x_type=F32, y_type=F32, x_stride=None, y_stride=None, stream=None):
+        """y[t] = W x[t] on device buffers (frc_matvec_device); strides default to n and rows."""
+        rc = self.lib.frc_matvec_device(self.ctx.h, self.h, tokens, x_ptr, self.n if x_stride is None else x_stride,
+                                        x_type, y_ptr, self.rows if y_stride is None else y_stride, y_type, stream)
+        self.ctx._check(rc, "matvec_device")
+
+    def close(self):
+        if self.h:
+            self.lib.frc_matrix_close(self.h)
+            self.h = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 def costmodel_fit(ns, nbytes):
@@ -435,6 +509,38 @@ class Context:
         rc = self.lib.frc_run_device_fixed(self.h, layer, tokens, expert_ptr, gate_ptr, x_ptr, x_add_ptr,
                                            x_out_ptr, y_ptr, act, flags, stream)
         self._check(rc, "run_device_fixed")
+
+    def matrix(self, type_, rows, n, data, nbytes=None):
+        """A Matrix of 4-bit rows in the reference's layout.  data: a numpy uint8 array, or with nbytes the address
+        of host or device memory."""
+        return Matrix(self, type_, rows, n, data, nbytes)
+
+    def route_device(self, tokens, experts, logits_ptr, expert_ptr, gate_ptr, stride=None, type_=F32, valid_ptr=None,
+                     flags=0, balance=None, stream=None):
+        """Experts and gates of every token from its logits, on device buffers (frc_route_device); balance: a
+        Balance whose statistics the same pass makes.  stride defaults to the columns."""
+        stride = experts + (flags & ROUTE_SHARED) if stride is None else stride
+        rc = self.lib.frc_route_device(self.h, tokens, experts, logits_ptr, stride, type_, valid_ptr, expert_ptr,
+                                       gate_ptr, flags, None if balance is None else ctypes.byref(balance), stream)
+        self._check(rc, "route_device")
+
+    def balance_device(self, tokens, experts, logits_ptr, expert_ptr, balance, stride=None, type_=F32,
+                       valid_ptr=None, stream=None):
+        """Counts, mean probabilities and the balance loss of given expert ids (frc_balance_device)."""
+        rc = self.lib.frc_balance_device(self.h, tokens, experts, logits_ptr, experts if stride is None else stride,
+                                         type_, valid_ptr, expert_ptr, ctypes.byref(balance), stream)
+        self._check(rc, "balance_device")
+
+    def route_backward_device(self, tokens, experts, logits_ptr, expert_ptr, d_logits_ptr, d_gate_ptr=None,
+                              count_ptr=None, d_loss_ptr=None, stride=None, d_stride=None, type_=F32, valid_ptr=None,
+                              flags=0, stream=None):
+        """Gradient of the gates (d_gate_ptr) and of the balance loss (count_ptr, d_loss_ptr) with respect to the
+        logits (frc_route_backward_device)."""
+        cols = experts + (flags & ROUTE_SHARED)
+        rc = self.lib.frc_route_backward_device(self.h, tokens, experts, logits_ptr, cols if stride is None else stride,
+                                                type_, valid_ptr, expert_ptr, d_gate_ptr, count_ptr, d_loss_ptr,
+                                                d_logits_ptr, cols if d_stride is None else d_stride, flags, stream)
+        self._check(rc, "route_backward_device")
 
     def host_pass(self, first_layer, expert, gate, h, act=ACT_Q8, flags=0):
         """Decode pass from the host (frc_host_pass_flags).  expert: [layers][10] or

@@ -16,6 +16,7 @@
 #include <string.h>
 
 #include <mutex>
+#include <new>
 
 #include "../../include/fronk_b200.h"
 #include "frc_device.cuh"
@@ -27,6 +28,8 @@ using namespace frc;
 #include "frc_umma.cuh"
 #include "frc_prefill.cuh"
 #include "frc_avx2.cuh"
+#include "frc_matvec.cuh"
+#include "frc_route.cuh"
 #include "frc_units.h"
 
 // ===================================================== set-up kernels
@@ -1756,6 +1759,195 @@ int frc_plane_run(frc_plane* p, unsigned layer, unsigned tokens, const uint16_t*
 int frc_plane_late_status(const frc_plane* p, unsigned participant, int* status) {
   if (!p || !status || participant >= p->n) return FRC_INVALID;
   *status = p->late_status[participant];
+  return FRC_OK;
+}
+
+// ------------------------------------------------------ 4-bit matrices
+
+// Makes `device` current for a scope and puts the caller's device back.
+struct DeviceScope {
+  int before = -1, device;
+  bool ok;
+  explicit DeviceScope(int d) : device(d) {
+    ok = cudaGetDevice(&before) == cudaSuccess && (before == d || cudaSetDevice(d) == cudaSuccess);
+  }
+  ~DeviceScope() {
+    if (before >= 0 && before != device) cudaSetDevice(before);
+  }
+};
+
+static bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+static size_t type_size(unsigned type) { return type == FRC_BF16 ? 2 : 4; }
+
+struct frc_matrix {
+  int device = 0;
+  unsigned type = 0, rows = 0, n = 0;
+  size_t row_bytes = 0;
+  uint8_t* data = nullptr;
+};
+
+int frc_matrix_close(frc_matrix* m) {
+  if (!m) return FRC_INVALID;
+  DeviceScope dev(m->device);
+  cudaFree(m->data);  // waits for the device's work, calls that read the matrix among it
+  delete m;
+  return FRC_OK;
+}
+
+int frc_matrix_open(frc_context* c, unsigned type, unsigned rows, unsigned n, const void* bytes, size_t len,
+                    frc_matrix** out) {
+  if (!c || !bytes || !out) return fail(c, FRC_INVALID, "null argument");
+  const int check = frc_matrix_check(type, rows, n);
+  if (check) return fail(c, check, "matrix: type %u, %u rows of %u weights", type, rows, n);
+  const size_t rowb = frc_row_bytes(type, n), total = rowb * rows;
+  if (len != total) return fail(c, FRC_INVALID, "matrix: %zu bytes given, %zu expected", len, total);
+  DeviceScope dev(c->device);
+  if (!dev.ok) return fail(c, FRC_IO, "cudaSetDevice");
+  frc_matrix* m = new (std::nothrow) frc_matrix();
+  if (!m) return fail(c, FRC_IO, "out of memory");
+  m->device = c->device; m->type = type; m->rows = rows; m->n = n; m->row_bytes = rowb;
+  const size_t flag_at = (total + 15) / 16 * 16;
+  cudaError_t e = cudaMalloc(&m->data, flag_at + 16);
+  unsigned bad = 0;
+  unsigned* flag = reinterpret_cast<unsigned*>(m->data + flag_at);
+  if (e == cudaSuccess) e = cudaMemsetAsync(flag, 0, sizeof bad, c->stream);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(m->data, bytes, total, cudaMemcpyDefault, c->stream);
+  if (e == cudaSuccess) {
+    const size_t blocks = static_cast<size_t>(rows) * (n / (type == FRC_Q4_K ? 256 : 32));
+    matrix_check_kernel<<<static_cast<unsigned>((blocks + 255) / 256), 256, 0, c->stream>>>(m->data, type, blocks, flag);
+    e = cudaGetLastError();
+    ++c->launches;
+  }
+  if (e == cudaSuccess) e = cudaMemcpyAsync(&bad, flag, sizeof bad, cudaMemcpyDeviceToHost, c->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
+  if (e != cudaSuccess || bad) {
+    frc_matrix_close(m);
+    return bad ? fail(c, FRC_NUMERIC, "matrix: a scale is not finite") : fail(c, FRC_IO, "matrix: %s", cudaGetErrorString(e));
+  }
+  *out = m;
+  return FRC_OK;
+}
+
+int frc_matvec_device(frc_context* c, const frc_matrix* m, unsigned tokens, const void* x, size_t x_stride,
+                      unsigned x_type, void* y, size_t y_stride, unsigned y_type, void* stream) {
+  if (!c || !m || !x || !y) return fail(c, FRC_INVALID, "null argument");
+  if (m->device != c->device) return fail(c, FRC_INVALID, "the matrix is on device %d, the context on %d", m->device, c->device);
+  if (tokens < 1 || tokens > FRC_MAX_TOKENS) return fail(c, FRC_INVALID, "matvec: tokens must be 1..%d", FRC_MAX_TOKENS);
+  if (x_type > FRC_BF16 || y_type > FRC_BF16) return fail(c, FRC_INVALID, "matvec: unknown element type");
+  if (tokens > 1 && (x_stride < m->n || y_stride < m->rows))
+    return fail(c, FRC_INVALID, "matvec: strides below %u and %u", m->n, m->rows);
+  if (!aligned_to(x, type_size(x_type)) || !aligned_to(y, type_size(y_type)))
+    return fail(c, FRC_INVALID, "matvec: x or y is not aligned to its element type");
+  DeviceScope dev(c->device);
+  if (!dev.ok) return fail(c, FRC_IO, "cudaSetDevice");
+  MatvecParams a{};
+  a.w = m->data; a.x = x; a.y = y; a.x_stride = x_stride; a.y_stride = y_stride;
+  a.rows = m->rows; a.n = m->n; a.tokens = tokens; a.row_bytes = static_cast<unsigned>(m->row_bytes);
+  a.status = c->status;
+  if (m->type == FRC_Q4_K) launch_matvec<kQ4K>(a, x_type, y_type, static_cast<cudaStream_t>(stream));
+  else launch_matvec<kMXFP4>(a, x_type, y_type, static_cast<cudaStream_t>(stream));
+  CK(cudaGetLastError());
+  ++c->launches;
+  return FRC_OK;
+}
+
+// -------------------------------------------------------------- routing
+
+size_t frc_balance_workspace(unsigned tokens, unsigned experts) {
+  if (frc_routing_check(tokens, experts, experts, FRC_F32, 0)) return 0;
+  const size_t parts = route_parts(tokens);
+  return parts * (experts * (sizeof(float) + sizeof(unsigned)) + sizeof(unsigned));
+}
+
+static int check_balance(frc_context* c, const frc_balance* b, unsigned tokens, unsigned experts) {
+  if (!b->loss || !b->count || !b->prob || !b->workspace) return fail(c, FRC_INVALID, "balance: null output or workspace");
+  if (b->workspace_bytes < frc_balance_workspace(tokens, experts))
+    return fail(c, FRC_INVALID, "balance: workspace of %zu bytes, %zu needed", b->workspace_bytes,
+                frc_balance_workspace(tokens, experts));
+  if (!aligned_to(b->loss, 4) || !aligned_to(b->count, 4) || !aligned_to(b->prob, 4) || !aligned_to(b->workspace, 16))
+    return fail(c, FRC_INVALID, "balance: outputs need 4-byte, the workspace 16-byte alignment");
+  return FRC_OK;
+}
+
+static int route(frc_context* c, unsigned tokens, unsigned experts, const void* logits, size_t stride, unsigned type,
+                 const uint8_t* valid, const uint16_t* expert_in, uint16_t* expert, float* gate, unsigned flags,
+                 const frc_balance* b, cudaStream_t s) {
+  const int check = frc_routing_check(tokens, experts, stride, type, flags);
+  if (check) return fail(c, check, "routing: %u tokens, %u experts, stride %zu, type %u, flags %u", tokens, experts, stride, type, flags);
+  if (!aligned_to(logits, type_size(type)) || !aligned_to(expert_in ? expert_in : expert, 2) || !aligned_to(gate, 4))
+    return fail(c, FRC_INVALID, "routing: a pointer is not aligned to its element type");
+  if (b) {
+    const int rc = check_balance(c, b, tokens, experts);
+    if (rc) return rc;
+  }
+  DeviceScope dev(c->device);
+  if (!dev.ok) return fail(c, FRC_IO, "cudaSetDevice");
+  RouteParams a{};
+  a.logits = logits; a.stride = stride; a.valid = valid; a.expert_in = expert_in; a.expert = expert; a.gate = gate;
+  a.tokens = tokens; a.experts = experts; a.shared = flags & FRC_ROUTE_SHARED;
+  a.status = c->status;
+  const unsigned parts = route_parts(tokens);
+  if (b) {
+    a.psum = static_cast<float*>(b->workspace);
+    a.pcount = reinterpret_cast<unsigned*>(a.psum + static_cast<size_t>(parts) * experts);
+    a.pvalid = a.pcount + static_cast<size_t>(parts) * experts;
+  }
+  if (type == FRC_BF16) launch_route<__nv_bfloat16>(a, expert_in == nullptr, b != nullptr, s);
+  else launch_route<float>(a, expert_in == nullptr, b != nullptr, s);
+  CK(cudaGetLastError());
+  ++c->launches;
+  if (b) {
+    const RouteFinish f{a.psum, a.pcount, a.pvalid, parts, experts, b->loss, b->count, b->prob};
+    route_finish_kernel<<<1, kMaxExperts, 0, s>>>(f);
+    CK(cudaGetLastError());
+    ++c->launches;
+  }
+  return FRC_OK;
+}
+
+int frc_route_device(frc_context* c, unsigned tokens, unsigned experts, const void* logits, size_t stride,
+                     unsigned type, const uint8_t* valid, uint16_t* expert, float* gate, unsigned flags,
+                     const frc_balance* balance, void* stream) {
+  if (!c || !logits || !expert || !gate) return fail(c, FRC_INVALID, "null argument");
+  return route(c, tokens, experts, logits, stride, type, valid, nullptr, expert, gate, flags, balance,
+               static_cast<cudaStream_t>(stream));
+}
+
+int frc_balance_device(frc_context* c, unsigned tokens, unsigned experts, const void* logits, size_t stride,
+                       unsigned type, const uint8_t* valid, const uint16_t* expert, const frc_balance* balance,
+                       void* stream) {
+  if (!c || !logits || !expert || !balance) return fail(c, FRC_INVALID, "null argument");
+  return route(c, tokens, experts, logits, stride, type, valid, expert, nullptr, nullptr, 0, balance,
+               static_cast<cudaStream_t>(stream));
+}
+
+int frc_route_backward_device(frc_context* c, unsigned tokens, unsigned experts, const void* logits, size_t stride,
+                              unsigned type, const uint8_t* valid, const uint16_t* expert, const float* d_gate,
+                              const uint32_t* count, const float* d_loss, void* d_logits, size_t d_stride,
+                              unsigned flags, void* stream) {
+  if (!c || !logits || !d_logits) return fail(c, FRC_INVALID, "null argument");
+  if (!d_gate && !count) return fail(c, FRC_INVALID, "route_backward: neither a gate nor a loss gradient");
+  if (d_gate && !expert) return fail(c, FRC_INVALID, "route_backward: the gate gradient needs the expert ids");
+  if (!count != !d_loss) return fail(c, FRC_INVALID, "route_backward: count and d_loss come together");
+  int check = frc_routing_check(tokens, experts, stride, type, flags);
+  if (!check) check = frc_routing_check(tokens, experts, d_stride, type, flags);
+  if (check) return fail(c, check, "routing: %u tokens, %u experts, strides %zu and %zu, type %u, flags %u", tokens, experts, stride, d_stride, type, flags);
+  if (d_logits == logits && d_stride != stride) return fail(c, FRC_INVALID, "route_backward: in place needs one stride");
+  if (!aligned_to(logits, type_size(type)) || !aligned_to(d_logits, type_size(type)) || !aligned_to(expert, 2) ||
+      !aligned_to(d_gate, 4) || !aligned_to(count, 4) || !aligned_to(d_loss, 4))
+    return fail(c, FRC_INVALID, "routing: a pointer is not aligned to its element type");
+  DeviceScope dev(c->device);
+  if (!dev.ok) return fail(c, FRC_IO, "cudaSetDevice");
+  RouteBackwardParams a{};
+  a.logits = logits; a.stride = stride; a.d_stride = d_stride; a.valid = valid; a.expert = expert; a.d_gate = d_gate;
+  a.count = count; a.d_loss = d_loss; a.d_logits = d_logits; a.tokens = tokens; a.experts = experts;
+  a.shared = flags & FRC_ROUTE_SHARED; a.status = c->status;
+  const unsigned grid = (tokens + kRouteWarps - 1) / kRouteWarps;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (type == FRC_BF16) route_backward_kernel<__nv_bfloat16><<<grid, 32 * kRouteWarps, 0, s>>>(a);
+  else route_backward_kernel<float><<<grid, 32 * kRouteWarps, 0, s>>>(a);
+  CK(cudaGetLastError());
+  ++c->launches;
   return FRC_OK;
 }
 

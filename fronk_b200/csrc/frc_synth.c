@@ -49,6 +49,20 @@ uint64_t frc_slice_offset(const frc_geometry *g, unsigned layer, unsigned expert
     return (uint64_t)layer * frc_layer_bytes(g) + (uint64_t)expert * frc_slice_bytes(g);
 }
 
+int frc_matrix_check(unsigned type, unsigned rows, unsigned n) {
+    if (type == FRC_Q8_0) return FRC_UNSUPPORTED;
+    if (type != FRC_Q4_K && type != FRC_MXFP4) return FRC_INVALID;
+    if (!rows || rows > FRC_MATRIX_MAX_ROWS || n > FRC_MATRIX_MAX_N || !frc_row_bytes(type, n)) return FRC_INVALID;
+    return FRC_OK;
+}
+
+int frc_routing_check(unsigned tokens, unsigned experts, size_t stride, unsigned type, unsigned flags) {
+    if (!tokens || tokens > FRC_ROUTE_MAX_TOKENS || experts < FRC_TOPK || experts > FRC_ROUTED_EXPERTS) return FRC_INVALID;
+    if ((type != FRC_F32 && type != FRC_BF16) || (flags & ~(unsigned)FRC_ROUTE_SHARED)) return FRC_INVALID;
+    if (stride < (size_t)experts + (flags & FRC_ROUTE_SHARED)) return FRC_INVALID;
+    return FRC_OK;
+}
+
 /* ------------------------------------------------------------- random */
 
 /* splitmix64 finalizer over a Weyl sequence, indexed directly. */

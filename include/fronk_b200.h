@@ -249,6 +249,96 @@ int frc_run_device(frc_context *c, unsigned layer, unsigned tokens, const uint16
 int frc_run_device_fixed(frc_context *c, unsigned layer, unsigned tokens, const uint16_t *expert,
                          const float *gate, const float *x, const float *x_add, float *x_out,
                          float *y, int act, unsigned flags, void *stream);
+/* ---- Dense 4-bit matrices: the products beside the experts ----
+ * y[t] = W x[t] for a burst of 1..FRC_MAX_TOKENS tokens, W in the same row
+ * formats as the experts' rows (a router's rows, a projection, a vocabulary
+ * head).  Sums are fp32.  No reference counterpart (its dense products belong
+ * to the external engine). */
+enum { FRC_F32 = 0, FRC_BF16 = 1 };  /* element types of device buffers */
+enum { FRC_MATRIX_MAX_ROWS = 1 << 24, FRC_MATRIX_MAX_N = 1 << 16 };
+typedef struct frc_matrix frc_matrix;
+/* FRC_OK when a matrix of `rows` rows of n weights can be opened: type
+ * FRC_Q4_K (n a multiple of 256) or FRC_MXFP4 (a multiple of 32), n up to
+ * FRC_MATRIX_MAX_N, any row count up to FRC_MATRIX_MAX_ROWS.  FRC_UNSUPPORTED
+ * for FRC_Q8_0, else FRC_INVALID.  Host only. */
+int frc_matrix_check(unsigned type, unsigned rows, unsigned n);
+/* Copies rows x frc_row_bytes(type, n) bytes (the reference's row layout, row
+ * after row; host or device memory, ready when the call is made) into HBM and
+ * checks every scale: FRC_NUMERIC when one is not finite (MXFP4 exponent 255
+ * too).  Synchronous.  The matrix belongs to the context's device, works with
+ * any context of that device and may outlive the one that opened it. */
+int frc_matrix_open(frc_context *c, unsigned type, unsigned rows, unsigned n, const void *bytes, size_t len,
+                    frc_matrix **out);
+/* Frees the matrix after the device's work in flight; not while a stream
+ * capture holds or a captured graph still replays a call that reads it. */
+int frc_matrix_close(frc_matrix *m);
+/* y[t][r] = sum_j W[r][j] x[t][j], asynchronous on `stream`, allocates
+ * nothing, can be captured.  x: [tokens][n] (x_type, x_stride elements
+ * between tokens), y: [tokens][rows] (y_type, y_stride); strides are not read
+ * for one token.  x and y must not overlap.  A result that is not finite
+ * (or whose x is not) sets FRC_NUMERIC in the context's device status
+ * (frc_status).  Concurrent calls on several streams are independent. */
+int frc_matvec_device(frc_context *c, const frc_matrix *m, unsigned tokens, const void *x, size_t x_stride,
+                      unsigned x_type, void *y, size_t y_stride, unsigned y_type, void *stream);
+
+/* ---- Routing: from expert logits to what frc_run_device reads ----
+ * Device buffers, asynchronous on `stream`, no allocation, capturable; the
+ * results are bitwise repeatable.  logits: [tokens][experts] of `type`
+ * (FRC_F32 or FRC_BF16), `stride` elements between rows; with
+ * FRC_ROUTE_SHARED column `experts` holds the shared expert's gate logit.
+ * experts: 10..512; a logit of -inf masks its expert out.
+ * valid: [tokens] bytes or NULL (all); a row with 0 is padding: its logits
+ * are not looked at.  A NaN or +inf logit of a valid row sets FRC_NUMERIC in
+ * the device status, and the row counts as padding.  No reference counterpart
+ * (its router belongs to the external engine). */
+enum { FRC_ROUTE_SHARED = 1 };
+enum { FRC_ROUTE_MAX_TOKENS = 1 << 24 };
+/* FRC_OK when a routing call with these sizes is accepted.  Host only. */
+int frc_routing_check(unsigned tokens, unsigned experts, size_t stride, unsigned type, unsigned flags);
+/* Balance statistics over the N valid rows, all on the device:
+ *   count[e]: rows that chose e (masked experts never count); count[experts] = N
+ *   prob[e]:  mean of softmax(logits)[e]
+ *   loss:     experts * sum_e count[e] / (10 N) * prob[e]   (1 when even; 0 for N = 0)
+ * workspace: frc_balance_workspace(tokens, experts) bytes of device memory,
+ * 16-byte aligned, any contents; calls that may overlap (other streams,
+ * captured graphs that may run at one time) need one each. */
+typedef struct {
+    float *loss;      /* [1] */
+    uint32_t *count;  /* [experts + 1] */
+    float *prob;      /* [experts] */
+    void *workspace;
+    size_t workspace_bytes;
+} frc_balance;
+size_t frc_balance_workspace(unsigned tokens, unsigned experts);  /* 0 for sizes that are refused; host only */
+/* expert[t][10]: the ten largest logits, descending, ties by the lower index
+ * (masked experts fill up when fewer than ten are left); gate[t][0..9] =
+ * softmax over the chosen (0 for a masked one), gate[t][10] = sigmoid of the
+ * shared logit with FRC_ROUTE_SHARED, else 0.  A padding row gets experts
+ * 0..9 and gates 0, so a layer call adds nothing for it.  balance: NULL, or
+ * the statistics of this routing from the same pass. */
+int frc_route_device(frc_context *c, unsigned tokens, unsigned experts, const void *logits, size_t stride,
+                     unsigned type, const uint8_t *valid, uint16_t *expert, float *gate, unsigned flags,
+                     const frc_balance *balance, void *stream);
+/* The statistics for expert ids [tokens][10] that something else chose.  An
+ * id outside 0..experts-1 of a valid row is left out and sets FRC_INVALID in
+ * the device status; an id named twice in a row counts twice. */
+int frc_balance_device(frc_context *c, unsigned tokens, unsigned experts, const void *logits, size_t stride,
+                       unsigned type, const uint8_t *valid, const uint16_t *expert, const frc_balance *balance,
+                       void *stream);
+/* d_logits[t][experts (+ 1)] (`type`, d_stride) of both outputs; padding rows
+ * get zeros, elements behind a row's columns are left alone.
+ *   gates (d_gate [tokens][11] not NULL; expert as chosen):
+ *     g_i (d_i - sum_j g_j d_j) at the chosen, s (1 - s) d_10 at the shared column
+ *   loss (count as frc_balance wrote it and the scalar d_loss, not NULL):
+ *     d_loss * experts / (10 N^2) * p_e (count_e - sum_j p_j count_j);
+ *     the counts are constants, as usual
+ * The two are added.  d_logits may be logits itself (same stride), else they
+ * must not overlap. */
+int frc_route_backward_device(frc_context *c, unsigned tokens, unsigned experts, const void *logits, size_t stride,
+                              unsigned type, const uint8_t *valid, const uint16_t *expert, const float *d_gate,
+                              const uint32_t *count, const float *d_loss, void *d_logits, size_t d_stride,
+                              unsigned flags, void *stream);
+
 /* ---- In-box reduce over NVLink peer memory (replaces the per-layer
  * all-reduce of the slice partials; the reference's fanout/plane gather,
  * src/plane.c:110-121, inside one box).  One process per GPU:

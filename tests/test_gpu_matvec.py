@@ -1,0 +1,265 @@
+"""Products of 4-bit matrices (frc_matrix_open, frc_matvec_device) against float64.
+
+Tolerance.  With A = sum_j a_j |x_j| (a_j: the size of weight j's terms, Q4_K: |d sc q| + |dmin mi|), an fp32 sum
+of n terms that is formed 16 terms at a time and truncated at each step is off by at most 2 n/16 steps of 2^-23 A,
+plus two roundings for every 256 weights' scales and 16 for joining the parts: (n/8 + n/128 + 16) 2^-23 A.  The
+vector may be carried with 22 significant bits (2^-23 A, inside the 16), and not below 2^-34 of the largest value in
+its span of 256 weights: + 2^-34 sum_j a_j max|x|.  A bf16 result adds half a step, 2^-8 of the value."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import fronk_b200 as fb
+from tests import quant
+
+pytestmark = pytest.mark.gpu
+
+
+def bound(a, x, n):
+    spans = -(-n // 256) * 256
+    xp = np.zeros((x.shape[0], spans))
+    xp[:, :n] = np.abs(x)
+    top = np.repeat(xp.reshape(x.shape[0], -1, 256).max(-1), 256, axis=1)[:, :n]
+    return (n / 8 + n / 128 + 16) * 2.0 ** -23 * (np.abs(x) @ a.T) + 2.0 ** -34 * (top @ a.T)
+
+
+def to_device(x, dtype):
+    import torch
+    t = torch.from_numpy(np.ascontiguousarray(x, np.float32)).cuda()
+    return t.to(torch.bfloat16 if dtype == fb.BF16 else torch.float32)
+
+
+def host(t):
+    return t.float().cpu().numpy().astype(np.float64)
+
+
+def check(y, x, w, a, n, y_type):
+    ref = x @ w.T
+    tol = bound(a, x, n) + (2.0 ** -8 * np.abs(ref) if y_type == fb.BF16 else 0)
+    err = np.abs(y - ref)
+    assert np.all(err <= tol), (err / tol).max()
+
+
+@pytest.fixture(scope="module")
+def ctx(gpu):
+    with fb.Context(0, 512) as c:
+        yield c
+
+
+def run(ctx, type_, raw, n, xd, x_type, y_type, x_stride=None, y_stride=None):
+    import torch
+    rows, tokens = raw.shape[0], xd.shape[0]
+    y = torch.full((tokens, rows), float("nan"), dtype=torch.bfloat16 if y_type == fb.BF16 else torch.float32,
+                   device="cuda")
+    with ctx.matrix(type_, rows, n, raw) as m:
+        m.matvec_device(tokens, xd.data_ptr(), y.data_ptr(), x_type, y_type, x_stride, y_stride,
+                        torch.cuda.current_stream().cuda_stream)
+        assert ctx.status(torch.cuda.current_stream().cuda_stream) == fb.OK
+    return y
+
+
+SHAPES = [(fb.Q4_K, 1, 256), (fb.Q4_K, 15, 512), (fb.Q4_K, 17, 2304), (fb.Q4_K, 513, 2048), (fb.Q4_K, 130, 8192),
+          (fb.Q4_K, 5000, 256), (fb.MXFP4, 1, 32), (fb.MXFP4, 16, 64), (fb.MXFP4, 33, 288), (fb.MXFP4, 513, 2048),
+          (fb.MXFP4, 75, 4192), (fb.MXFP4, 3, 16384), (fb.MXFP4, 2051, 672)]
+
+
+@pytest.mark.parametrize("type_,rows,n", SHAPES)
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 5, 8, 9, 16])
+def test_shapes(ctx, type_, rows, n, tokens):
+    rng = np.random.default_rng(rows * 1000 + n + tokens)
+    raw = quant.random_rows(type_, rows, n, rng)
+    w, a = quant.weights(type_, raw, n)
+    x = rng.standard_normal((tokens, n))
+    for x_type, y_type in [(fb.F32, fb.F32), (fb.BF16, fb.BF16), (fb.F32, fb.BF16), (fb.BF16, fb.F32)]:
+        xd = to_device(x, x_type)
+        y = run(ctx, type_, raw, n, xd, x_type, y_type)
+        check(host(y), host(xd), w, a, n, y_type)
+
+
+@pytest.mark.parametrize("type_,rows", [(fb.Q4_K, 70001), (fb.MXFP4, 65537)])
+def test_many_rows(ctx, type_, rows):
+    """More row tiles than the GPU holds at a time."""
+    rng = np.random.default_rng(rows)
+    n = 512
+    raw = np.tile(quant.random_rows(type_, 257, n, rng), (rows // 257 + 1, 1))[:rows]
+    w, a = quant.weights(type_, raw[:257], n)
+    for tokens in (1, 7, 16):
+        xd = to_device(rng.standard_normal((tokens, n)), fb.F32)
+        y = host(run(ctx, type_, raw, n, xd, fb.F32, fb.F32))
+        check(y[:, :257], host(xd), w, a, n, fb.F32)
+        for r in range(257, rows, 257):
+            k = min(257, rows - r)
+            assert np.array_equal(y[:, r:r + k], y[:, :k]), r
+
+
+@pytest.mark.parametrize("type_", [fb.Q4_K, fb.MXFP4])
+@pytest.mark.parametrize("x_type,y_type", [(fb.F32, fb.F32), (fb.BF16, fb.BF16)])
+def test_strides_and_alignment(ctx, type_, x_type, y_type):
+    """Odd row strides, x and y that start on an odd element; what lies between the rows of y stays."""
+    import torch
+    rng = np.random.default_rng(11)
+    rows, n, tokens = 45, 768, 5
+    raw = quant.random_rows(type_, rows, n, rng)
+    w, a = quant.weights(type_, raw, n)
+    dt = torch.bfloat16 if x_type == fb.BF16 else torch.float32
+    xb = torch.full((1 + tokens * (n + 3),), float("nan"), dtype=dt, device="cuda")
+    xv = xb[1:].view(tokens, n + 3)
+    xv[:, :n] = to_device(rng.standard_normal((tokens, n)), x_type)
+    yb = torch.full((1 + tokens * (rows + 2),), -7.0, dtype=torch.bfloat16 if y_type == fb.BF16 else torch.float32,
+                    device="cuda")
+    yv = yb[1:].view(tokens, rows + 2)
+    s = torch.cuda.current_stream().cuda_stream
+    with ctx.matrix(type_, rows, n, raw) as m:
+        m.matvec_device(tokens, xv.data_ptr(), yv.data_ptr(), x_type, y_type, n + 3, rows + 2, s)
+        assert ctx.status(s) == fb.OK
+    check(host(yv[:, :rows]), host(xv[:, :n]), w, a, n, y_type)
+    assert bool((yv[:, rows:] == -7).all()) and float(yb[0]) == -7
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 16])
+def test_range_of_values(ctx, tokens):
+    """Spans of very different size in one vector, single large and tiny values, rows of zeros."""
+    rng = np.random.default_rng(3)
+    for type_, n in [(fb.Q4_K, 1536), (fb.MXFP4, 1440)]:
+        raw = quant.random_rows(type_, 40, n, rng)
+        w, a = quant.weights(type_, raw, n)
+        x = rng.standard_normal((tokens, n)).astype(np.float32)
+        x[:, :256] *= 1e-18
+        x[:, 256:512] *= 1e12
+        x[:, 512:768] = 0
+        x[0, 800] = 3e4
+        x[0, 900] = 1e-39  # subnormal
+        if tokens > 1:
+            x[1] = 0
+            x[2] *= 1e-30
+        xd = to_device(x, fb.F32)
+        y = host(run(ctx, type_, raw, n, xd, fb.F32, fb.F32))
+        xr = host(xd)
+        ref, tol = xr @ w.T, bound(a, xr, n) + 2.0 ** -126  # results below the normal range may be flushed
+        assert np.all(np.abs(y - ref) <= tol), (np.abs(y - ref) / tol).max()
+
+
+def test_scales_at_the_border(ctx):
+    """Q4_K super scales that are subnormal, zero or large; MXFP4 exponents far apart in one row, 0 and 200."""
+    rng = np.random.default_rng(4)
+    n = 768
+    raw = quant.random_rows(fb.Q4_K, 48, n, rng)
+    b = raw.reshape(48, 3, 144)
+    b[:8, :, :4] = np.array([2 ** -24, 2 ** -20], np.float16).view(np.uint8)
+    b[8:16, :, :4] = 0
+    b[16:24, :, :4] = np.array([60000, -60000], np.float16).view(np.uint8)
+    b[24:32, :, 4:16] = 255  # all scales and minima 63
+    b[32:40, :, 4:16] = 0
+    w, a = quant.weights(fb.Q4_K, raw, n)
+    xd = to_device(rng.standard_normal((2, n)), fb.F32)
+    check(host(run(ctx, fb.Q4_K, raw, n, xd, fb.F32, fb.F32)), host(xd), w, a, n, fb.F32)
+
+    raw = quant.random_rows(fb.MXFP4, 48, n, rng)
+    b = raw.reshape(48, 24, 17)
+    b[:8, :, 0] = rng.integers(60, 180, (8, 24))
+    b[8:16, :, 0] = 0
+    b[16:24, :, 0] = 200
+    b[24:32, ::2, 0] = 1
+    b[32:40, :, 1:] = 0x88  # minus zero
+    w, a = quant.weights(fb.MXFP4, raw, n)
+    xd = to_device(rng.standard_normal((2, n)), fb.F32)
+    y, x = host(run(ctx, fb.MXFP4, raw, n, xd, fb.F32, fb.F32)), host(xd)
+    tol = bound(a, x, n) + 2.0 ** -126
+    assert np.all(np.abs(y - x @ w.T) <= tol)
+
+
+def test_numeric_status(ctx):
+    import torch
+    rng = np.random.default_rng(5)
+    s = torch.cuda.current_stream().cuda_stream
+    for type_ in (fb.Q4_K, fb.MXFP4):
+        n, rows = 512, 20
+        raw = quant.random_rows(type_, rows, n, rng)
+        for value in (float("nan"), float("inf"), -float("inf")):
+            x = torch.randn(3, n, device="cuda")
+            x[1, 77] = value
+            y = torch.zeros(3, rows, device="cuda")
+            with ctx.matrix(type_, rows, n, raw) as m:
+                m.matvec_device(3, x.data_ptr(), y.data_ptr(), stream=s)
+                assert ctx.status(s) == fb.NUMERIC
+                good = torch.zeros(2, rows, device="cuda")
+                m.matvec_device(2, x[::2].contiguous().data_ptr(), good.data_ptr(), stream=s)
+                assert ctx.status(s) == fb.OK
+            assert bool(torch.isfinite(y[::2]).all()) and not bool(torch.isfinite(y[1]).all())
+        big = torch.full((1, n), 3e38, device="cuda")
+        y = torch.zeros(1, rows, device="cuda")
+        raw = quant.random_rows(fb.MXFP4, rows, n, rng, exponents=(140, 141))
+        with ctx.matrix(fb.MXFP4, rows, n, raw) as m:
+            m.matvec_device(1, big.data_ptr(), y.data_ptr(), stream=s)
+            assert ctx.status(s) == fb.NUMERIC
+
+
+def test_refusals(ctx):
+    import torch
+    rng = np.random.default_rng(6)
+    raw = quant.random_rows(fb.Q4_K, 4, 256, rng)
+
+    def refused(code, *args):
+        with pytest.raises(fb.FrcError) as e:
+            ctx.matrix(*args)
+        assert e.value.code == code
+
+    refused(fb.INVALID, fb.Q4_K, 5, 256, raw)
+    refused(fb.INVALID, fb.Q4_K, 4, 128, raw)
+    refused(fb.UNSUPPORTED, fb.Q8_0, 4, 256, raw)
+    for at, v in [(1, 0x7c), (3, 0xfc), (1, 0x7e)]:
+        broken = raw.copy()
+        broken[3, at] = v
+        refused(fb.NUMERIC, fb.Q4_K, 4, 256, broken)
+    mx = quant.random_rows(fb.MXFP4, 4, 96, rng)
+    mx[2, 34] = 255
+    refused(fb.NUMERIC, fb.MXFP4, 4, 96, mx)
+    x = torch.zeros(17, 256, device="cuda")
+    y = torch.zeros(17, 4, device="cuda")
+    before = ctx.launches
+    with ctx.matrix(fb.Q4_K, 4, 256, raw) as m:
+        opened = ctx.launches
+        for kw in [dict(tokens=0), dict(tokens=17), dict(x_type=2), dict(y_type=2), dict(tokens=2, x_stride=255),
+                   dict(tokens=2, y_stride=3), dict(x_ptr=None), dict(y_ptr=None), dict(x_ptr=x.data_ptr() + 2),
+                   dict(y_ptr=y.data_ptr() + 1, y_type=fb.BF16)]:
+            a = dict(tokens=1, x_ptr=x.data_ptr(), y_ptr=y.data_ptr())
+            a.update(kw)
+            with pytest.raises(fb.FrcError) as e:
+                m.matvec_device(**a)
+            assert e.value.code == fb.INVALID
+        assert ctx.launches == opened > before
+
+
+def test_device_rows_graph_and_streams(ctx):
+    """Rows given in device memory; a captured call that is replayed on new values; two streams at once; the same
+    call twice gives the same bits."""
+    import torch
+    rng = np.random.default_rng(7)
+    rows, n = 300, 1024
+    raw = quant.random_rows(fb.MXFP4, rows, n, rng)
+    w, a = quant.weights(fb.MXFP4, raw, n)
+    dev = torch.from_numpy(raw).cuda()
+    torch.cuda.synchronize()
+    m = ctx.matrix(fb.MXFP4, rows, n, dev.data_ptr(), dev.numel())
+    del dev
+    x = torch.zeros(2, n, device="cuda")
+    y = torch.zeros(2, rows, device="cuda")
+    side = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        m.matvec_device(2, x.data_ptr(), y.data_ptr(), stream=side.cuda_stream)
+    for k in range(3):
+        x.copy_(torch.from_numpy(rng.standard_normal((2, n)).astype(np.float32)))
+        g.replay()
+        torch.cuda.synchronize()
+        check(host(y), host(x), w, a, n, fb.F32)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ys = [torch.zeros(2, rows, device="cuda") for _ in range(8)]
+    torch.cuda.synchronize()
+    for k in range(8):
+        m.matvec_device(2, x.data_ptr(), ys[k].data_ptr(), stream=streams[k % 2].cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, y) for v in ys)
+    assert ctx.status() == fb.OK
+    m.close()
