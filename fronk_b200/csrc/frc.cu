@@ -1782,7 +1782,7 @@ static size_t type_size(unsigned type) { return type == FRC_BF16 ? 2 : 4; }
 struct frc_matrix {
   int device = 0;
   unsigned type = 0, rows = 0, n = 0;
-  size_t row_bytes = 0;
+  MvLayout layout{};
   uint8_t* data = nullptr;
 };
 
@@ -1805,21 +1805,27 @@ int frc_matrix_open(frc_context* c, unsigned type, unsigned rows, unsigned n, co
   if (!dev.ok) return fail(c, FRC_IO, "cudaSetDevice");
   frc_matrix* m = new (std::nothrow) frc_matrix();
   if (!m) return fail(c, FRC_IO, "out of memory");
-  m->device = c->device; m->type = type; m->rows = rows; m->n = n; m->row_bytes = rowb;
-  const size_t flag_at = (total + 15) / 16 * 16;
-  cudaError_t e = cudaMalloc(&m->data, flag_at + 16);
+  m->device = c->device; m->type = type; m->rows = rows; m->n = n;
+  m->layout = mv_layout(type, rows, n);
+  // the rows as given (freed again) behind a word for the scale check
+  uint8_t* raw = nullptr;
   unsigned bad = 0;
-  unsigned* flag = reinterpret_cast<unsigned*>(m->data + flag_at);
+  cudaError_t e = cudaMalloc(&m->data, m->layout.total);
+  if (e == cudaSuccess) e = cudaMalloc(&raw, 16 + total);
+  unsigned* flag = reinterpret_cast<unsigned*>(raw);
   if (e == cudaSuccess) e = cudaMemsetAsync(flag, 0, sizeof bad, c->stream);
-  if (e == cudaSuccess) e = cudaMemcpyAsync(m->data, bytes, total, cudaMemcpyDefault, c->stream);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(raw + 16, bytes, total, cudaMemcpyDefault, c->stream);
   if (e == cudaSuccess) {
-    const size_t blocks = static_cast<size_t>(rows) * (n / (type == FRC_Q4_K ? 256 : 32));
-    matrix_check_kernel<<<static_cast<unsigned>((blocks + 255) / 256), 256, 0, c->stream>>>(m->data, type, blocks, flag);
+    if (type == FRC_Q4_K)
+      matrix_layout_kernel<kQ4K><<<m->layout.tiles, 256, 0, c->stream>>>(raw + 16, m->data, m->layout, rows, n, static_cast<unsigned>(rowb), flag);
+    else
+      matrix_layout_kernel<kMXFP4><<<m->layout.tiles, 256, 0, c->stream>>>(raw + 16, m->data, m->layout, rows, n, static_cast<unsigned>(rowb), flag);
     e = cudaGetLastError();
     ++c->launches;
   }
   if (e == cudaSuccess) e = cudaMemcpyAsync(&bad, flag, sizeof bad, cudaMemcpyDeviceToHost, c->stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
+  cudaFree(raw);
   if (e != cudaSuccess || bad) {
     frc_matrix_close(m);
     return bad ? fail(c, FRC_NUMERIC, "matrix: a scale is not finite") : fail(c, FRC_IO, "matrix: %s", cudaGetErrorString(e));
@@ -1842,11 +1848,13 @@ int frc_matvec_device(frc_context* c, const frc_matrix* m, unsigned tokens, cons
   if (!dev.ok) return fail(c, FRC_IO, "cudaSetDevice");
   MatvecParams a{};
   a.w = m->data; a.x = x; a.y = y; a.x_stride = x_stride; a.y_stride = y_stride;
-  a.rows = m->rows; a.n = m->n; a.tokens = tokens; a.row_bytes = static_cast<unsigned>(m->row_bytes);
+  a.rows = m->rows; a.n = m->n; a.tokens = tokens;
+  a.x_vec = aligned_to(x, 16) && (tokens == 1 || x_stride * type_size(x_type) % 16 == 0);
+  a.y_bf16 = y_type == FRC_BF16;
   a.status = c->status;
-  if (m->type == FRC_Q4_K) launch_matvec<kQ4K>(a, x_type, y_type, static_cast<cudaStream_t>(stream));
-  else launch_matvec<kMXFP4>(a, x_type, y_type, static_cast<cudaStream_t>(stream));
-  CK(cudaGetLastError());
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  CK(m->type == FRC_Q4_K ? launch_matvec<kQ4K>(a, m->layout, x_type, static_cast<unsigned>(c->sms), s)
+                         : launch_matvec<kMXFP4>(a, m->layout, x_type, static_cast<unsigned>(c->sms), s));
   ++c->launches;
   return FRC_OK;
 }

@@ -3,6 +3,23 @@
 // y[t][r] = sum_j W[r][j] x[t][j], W in the row formats of the expert slices:
 // Q4_K (w = d sc_g q - dmin mi_g, a 6-bit scale and minimum per 32 weights
 // under fp16 super scales per 256) or MXFP4 (w = 2^(e-127) E2M1 per 32).
+//
+// The weights' bytes bound it, so the work per weight has to stay under the
+// ~1.5 integer and ~3 other lane operations that one weight may cost at the
+// HBM rate (43 weights a clock and SM).  Both formats are exact in fp16, so a
+// warp multiplies 16 rows x 256 columns ("a span of a tile") on the tensor
+// cores (m16n8k16, fp32 accumulators) with the vectors as the eight columns:
+//   Q4_K: nibble pairs masked out of a word are fp16 subnormals q 2^-24; one
+//     half2 product by sc makes q sc 2^-24 (10 bits, exact), so a whole span
+//     accumulates without touching the scales, and the minima are one more
+//     product, of mi with the sums of x over each 32.
+//   MXFP4: the hardware's E2M1 -> fp16 conversion, and per 32 weights one fma
+//     with 2^(e - base), base the row's largest exponent.
+// x is scaled by a power of two per span (largest value in [2^13, 2^14)) and
+// held in fp16: a bf16 value fits (P = 1), an fp32 value is the sum of two
+// (P = 2; 22 of its 24 bits, or 2^-34 of the span's largest value where that
+// is more: half a step of an fp16 hi, then of an fp16 lo part).  The two parts
+// are columns of their own.
 #pragma once
 #include <cuda_bf16.h>
 
@@ -11,92 +28,548 @@
 
 namespace frc {
 
+constexpr unsigned kMvSpan = 256;          // weights of a row in one step
+constexpr unsigned kMvTile = 16;           // rows of one step
+constexpr unsigned kMvColPad = 64;         // bytes: columns start in alternate halves of the banks
+
+// Device layout: tile after tile (16 rows, the last one filled up with zero
+// rows), in it span after span of [scales][pieces], a piece being 64 weights
+// of the 16 rows: lane (g = lane / 4, q = lane % 4) owns 16 bytes {row g
+// group 0, row g + 8 group 0, row g group 1, row g + 8 group 1}, a word of
+// eight weights 32 group + 8 q + 0..7 each, so that a load is the fragment.
+// The last span stops at the last piece that holds weights.
+//   Q4_K scales: the 16 header bytes of each row (d, dmin, packed 6 bits).
+//   MXFP4 scales: 8 exponents a row, relative to the row's largest (127 is
+//   that one, 0 stands for nothing); the largest are 16 bytes a tile at `base`.
+struct MvLayout {
+  unsigned tiles, spans, pieces_last, span_bytes, scale_bytes;
+  size_t tile_bytes, base_at, total;
+};
+inline MvLayout mv_layout(unsigned type, unsigned rows, unsigned n) {
+  MvLayout l;
+  l.tiles = (rows + kMvTile - 1) / kMvTile;
+  l.spans = (n + kMvSpan - 1) / kMvSpan;
+  l.pieces_last = (n - (l.spans - 1) * kMvSpan + 63) / 64;
+  l.scale_bytes = type == FRC_Q4_K ? 256 : 128;
+  l.span_bytes = l.scale_bytes + 2048;
+  l.tile_bytes = static_cast<size_t>(l.spans - 1) * l.span_bytes + l.scale_bytes + 512 * l.pieces_last;
+  l.base_at = l.tile_bytes * l.tiles;
+  l.total = l.base_at + static_cast<size_t>(l.tiles) * kMvTile;
+  return l;
+}
+
+// Reference rows -> the layout above, one CTA a tile; scales that are not
+// finite (Q4_K super scales, MXFP4 exponent 255) raise the numeric bit.
+template <unsigned TYPE>
+__global__ void __launch_bounds__(256) matrix_layout_kernel(const uint8_t* __restrict__ src, uint8_t* dst, MvLayout l,
+                                                            unsigned rows, unsigned n, unsigned row_bytes,
+                                                            unsigned* flag) {
+  __shared__ unsigned s_base[kMvTile];
+  const unsigned tile = blockIdx.x, tid = threadIdx.x;
+  const uint8_t* in = src + static_cast<size_t>(tile) * kMvTile * row_bytes;
+  uint8_t* out = dst + tile * l.tile_bytes;
+  const unsigned left = rows - tile * kMvTile < kMvTile ? rows - tile * kMvTile : kMvTile;
+  bool bad = false;
+  if (TYPE == kMXFP4) {
+    if (tid < kMvTile) s_base[tid] = 0;
+    __syncthreads();
+    for (unsigned i = tid; i < left * (n / 32); i += 256) {
+      const unsigned r = i / (n / 32), b = i % (n / 32), e = in[static_cast<size_t>(r) * row_bytes + 17 * b];
+      bad |= e == 255;
+      atomicMax(&s_base[r], e);
+    }
+    __syncthreads();
+    if (tid < kMvTile) dst[l.base_at + static_cast<size_t>(tile) * kMvTile + tid] = static_cast<uint8_t>(s_base[tid]);
+  }
+  for (unsigned s = 0; s < l.spans; ++s) {
+    uint8_t* o = out + static_cast<size_t>(s) * l.span_bytes;
+    if (TYPE == kQ4K) {
+      if (tid < 64) {  // a 4-byte word of a row's header
+        const unsigned r = tid / 4, w = tid % 4;
+        const uint8_t* b = in + static_cast<size_t>(r) * row_bytes + 144 * s + 4 * w;
+        const unsigned v = r < left ? b[0] | b[1] << 8 | b[2] << 16 | static_cast<unsigned>(b[3]) << 24 : 0u;
+        if (w == 0) bad |= (v & 0x7c00u) == 0x7c00u || (v & 0x7c000000u) == 0x7c000000u;
+        reinterpret_cast<unsigned*>(o)[tid] = v;
+      }
+    } else if (tid < 128) {
+      const unsigned r = tid / 8, b = 8 * s + tid % 8;
+      unsigned e = 0;
+      if (r < left && b < n / 32) {
+        const unsigned v = in[static_cast<size_t>(r) * row_bytes + 17 * b], base = s_base[r];
+        e = base - v < 127u ? v + 127u - base : 0u;
+      }
+      o[tid] = static_cast<uint8_t>(e);
+    }
+    const unsigned pieces = s + 1 < l.spans ? 4 : l.pieces_last;
+    for (unsigned i = tid; i < pieces * 128; i += 256) {
+      const unsigned piece = i / 128, lane = i / 4 % 32, part = i % 4;
+      const unsigned r = lane / 4 + 8 * (part & 1), grp = 2 * piece + part / 2, k0 = 8 * (lane % 4);
+      unsigned v = 0;
+      if (r < left && kMvSpan * s + 32 * grp < n) {
+        const uint8_t* b = in + static_cast<size_t>(r) * row_bytes;
+        if (TYPE == kQ4K) {
+          const uint8_t* q = b + 144 * s + 16 + 32 * (grp / 2) + k0;
+#pragma unroll
+          for (unsigned j = 0; j < 8; ++j)  // pair j / 2: its two weights in the word's halves
+            v |= (q[j] >> (4 * (grp & 1)) & 15u) << (4 * (j / 2) + 16 * (j & 1));
+        } else {
+          const uint8_t* q = b + 17 * (8 * s + grp) + 1 + (k0 & 8);
+#pragma unroll
+          for (unsigned j = 0; j < 8; ++j) v |= (q[j] >> (k0 < 16 ? 0 : 4) & 15u) << (4 * j);
+        }
+      }
+      reinterpret_cast<unsigned*>(o + l.scale_bytes)[i] = v;
+    }
+  }
+  if (bad) atomicOr(flag, kStNumeric);
+}
+
 struct MatvecParams {
-  const uint8_t* w;  // rows x row_bytes
+  const uint8_t* w;
   const void* x;
   void* y;
   size_t x_stride, y_stride;  // elements between tokens
-  unsigned rows, n, tokens, row_bytes;
+  size_t tile_bytes, base_at;
+  unsigned rows, n, tokens, tiles, spans, pieces_last;
+  unsigned chunk;             // spans of x in shared memory at a time
+  unsigned split;             // warps that share a tile's spans
+  unsigned x_vec, y_bf16;     // x rows are 16-byte aligned; y is bf16
   unsigned* status;
 };
 
-// Weight j of one row in the reference byte layout, exact in fp32.
+// m16n8k16, fp16 inputs, fp32 accumulators.
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// Eight E2M1 values -> fp16 pairs.
+__device__ __forceinline__ void e2m1_f16(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+__device__ __forceinline__ uint4 ldg_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+// A lane's share of one span of a tile.
 template <unsigned TYPE>
-__device__ __forceinline__ float matvec_weight(const uint8_t* row, unsigned j) {
-  if (TYPE == kQ4K) {
-    const uint8_t* b = row + j / 256 * 144;
-    const unsigned g = j % 256 / 32, l = j % 32;
-    const unsigned sc = g < 4 ? b[4 + g] & 63u : (b[8 + g] & 15u) | (b[g] >> 6) << 4;
-    const unsigned mi = g < 4 ? b[8 + g] & 63u : static_cast<unsigned>(b[8 + g] >> 4) | (b[4 + g] >> 6) << 4;
-    const unsigned q = b[16 + g / 2 * 32 + l] >> (4 * (g & 1)) & 15u;
-    const float d = h2f(b[0] | b[1] << 8), m = h2f(b[2] | b[3] << 8);
-    return __fmaf_rn(__fmul_rn(d, static_cast<float>(sc)), static_cast<float>(q), -__fmul_rn(m, static_cast<float>(mi)));
-  }
-  const uint8_t* b = row + j / 32 * 17;
-  const unsigned l = j % 32, c = b[1 + l % 16] >> (l < 16 ? 0 : 4) & 15u;
-  const float mag = byte_f((c & 4u) ? kE2M1Hi : kE2M1Lo, c & 3u);
-  return (c & 8u ? -mag : mag) * pow2_m128(b[0]);
-}
+struct MvFrag {
+  uint4 w[4];
+  uint4 s[TYPE == kQ4K ? 2 : 1];  // Q4_K: headers of rows g and g + 8; MXFP4: their exponents, 8 bytes each
 
-// Scales that are not finite (Q4_K super scales, MXFP4 exponent 255) raise
-// the numeric bit; one thread a block of weights.
-__global__ void matrix_check_kernel(const uint8_t* w, unsigned type, size_t blocks, unsigned* status) {
-  const size_t i = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x;
-  if (i >= blocks) return;
-  bool bad;
-  if (type == kQ4K) {
-    const uint8_t* b = w + i * 144;
-    bad = (b[1] & 0x7cu) == 0x7cu || (b[3] & 0x7cu) == 0x7cu;
-  } else {
-    bad = w[i * 17] == 255u;
+  __device__ __forceinline__ void load(const MatvecParams& a, unsigned tile, unsigned span, unsigned lane) {
+    constexpr unsigned scale = TYPE == kQ4K ? 256 : 128;
+    const uint8_t* p = a.w + tile * a.tile_bytes + static_cast<size_t>(span) * (scale + 2048);
+    if (TYPE == kQ4K) {
+      s[0] = ldg_stream(p + 16 * (lane / 4));
+      s[TYPE == kQ4K ? 1 : 0] = ldg_stream(p + 128 + 16 * (lane / 4));
+    } else {
+      const uint2 e0 = __ldg(reinterpret_cast<const uint2*>(p) + lane / 4);
+      const uint2 e1 = __ldg(reinterpret_cast<const uint2*>(p) + 8 + lane / 4);
+      s[0] = make_uint4(e0.x, e0.y, e1.x, e1.y);
+    }
+    const unsigned pieces = TYPE == kQ4K || span + 1 < a.spans ? 4 : a.pieces_last;
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j)
+      w[j] = j < pieces ? ldg_stream(p + scale + 512 * j + 16 * lane) : make_uint4(0, 0, 0, 0);
   }
-  if (bad) atomicOr(status, kStNumeric);
-}
+};
 
-template <typename X>
-__device__ __forceinline__ float matvec_load(const X* p);
-template <>
-__device__ __forceinline__ float matvec_load<float>(const float* p) { return *p; }
-template <>
-__device__ __forceinline__ float matvec_load<__nv_bfloat16>(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void matvec_store(float* p, float v) { *p = v; }
-__device__ __forceinline__ void matvec_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+// The vectors of one K chunk in shared memory: columns of fp16 parts, per
+// token and span the power of two, and for Q4_K the sums over each 32 as
+// eight hi and eight lo parts (x 2^-5: they fit fp16).
+struct MvShared {
+  uint8_t* col;     // [tokens * P][chunk * 512 + pad]
+  float* scale;     // [tokens][chunk]
+  uint8_t* sums;    // [tokens][chunk][32]
+  float* part;      // [warps][values][32], when warps share a tile
+};
+inline __host__ __device__ size_t mv_col_bytes(unsigned chunk) { return static_cast<size_t>(chunk) * 512 + kMvColPad; }
 
-// One warp a row, a lane every 32nd weight, fp32 sums.
-template <unsigned TYPE, typename X, typename Y>
-__global__ void __launch_bounds__(256) matvec_kernel(const MatvecParams a) {
-  const unsigned row = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x & 31;
-  if (row >= a.rows) return;
-  const uint8_t* w = a.w + static_cast<size_t>(row) * a.row_bytes;
-  const X* x = static_cast<const X*>(a.x);
-  float acc[kMaxTokens] = {};
-  for (unsigned j = lane; j < a.n; j += 32) {
-    const float v = matvec_weight<TYPE>(w, j);
+template <unsigned TYPE, unsigned P>
+__device__ __forceinline__ void mv_prepare(const MatvecParams& a, const MvShared& sh, unsigned first, unsigned count) {
+  const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = blockDim.x / 32;
+  for (unsigned u = warp; u < a.tokens * count; u += warps) {
+    const unsigned t = u / count, s = u % count, k = (first + s) * kMvSpan + 8 * lane;
+    float v[8];
+    if (k >= a.n) {
 #pragma unroll
-    for (unsigned t = 0; t < kMaxTokens; ++t)
-      if (t < a.tokens) acc[t] = fmaf(v, matvec_load(x + t * a.x_stride + j), acc[t]);
-  }
+      for (unsigned j = 0; j < 8; ++j) v[j] = 0.0f;
+    } else if (P == 2) {
+      const float* x = static_cast<const float*>(a.x) + t * a.x_stride + k;
+      if (a.x_vec) {
+        const float4 p = reinterpret_cast<const float4*>(x)[0], q = reinterpret_cast<const float4*>(x)[1];
+        v[0] = p.x; v[1] = p.y; v[2] = p.z; v[3] = p.w; v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
+      } else {
 #pragma unroll
-  for (unsigned t = 0; t < kMaxTokens; ++t) {
-    if (t >= a.tokens) break;
-    float s = acc[t];
+        for (unsigned j = 0; j < 8; ++j) v[j] = x[j];
+      }
+    } else {
+      const uint16_t* x = static_cast<const uint16_t*>(a.x) + t * a.x_stride + k;
+      if (a.x_vec) {
+        const uint4 p = *reinterpret_cast<const uint4*>(x);
+        const uint32_t w[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
-    for (unsigned o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) {
-      Y* y = static_cast<Y*>(a.y) + t * a.y_stride + row;
-      matvec_store(y, s);
-      if (!isfinite(matvec_load(y))) atomicOr(a.status, kStNumeric);
+        for (unsigned j = 0; j < 4; ++j) {
+          v[2 * j] = __uint_as_float(w[j] << 16);
+          v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        }
+      } else {
+#pragma unroll
+        for (unsigned j = 0; j < 8; ++j) v[j] = __uint_as_float(static_cast<uint32_t>(x[j]) << 16);
+      }
+    }
+    unsigned top = 0;
+#pragma unroll
+    for (unsigned j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+    top = __reduce_max_sync(0xffffffffu, top);
+    // x = v 2^ex; a span that is not finite has the scale NaN and so its results
+    int ex = static_cast<int>(top >> 23) - 127 - 13;
+    if (ex < -126) ex = -126;
+    const bool finite = top < 0x7f800000u;
+    const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+    float sum = 0.0f;
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j) {
+      // odd pairs of a Q4_K word carry 16 q
+      const float f = TYPE == kQ4K && (j & 1) ? 0.0625f : 1.0f;
+      float p = finite ? v[2 * j] * inv : 0.0f, q = finite ? v[2 * j + 1] * inv : 0.0f;
+      sum += p + q;
+      p *= f;
+      q *= f;
+      const __half2 h = __floats2half2_rn(p, q);
+      hi[j] = *reinterpret_cast<const uint32_t*>(&h);
+      const float2 b = __half22float2(h);
+      const __half2 l = __floats2half2_rn(p - b.x, q - b.y);
+      lo[j] = *reinterpret_cast<const uint32_t*>(&l);
+    }
+    uint8_t* c = sh.col + (t * P) * mv_col_bytes(a.chunk) + 512 * s + 16 * lane;
+    *reinterpret_cast<uint4*>(c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if (P == 2) *reinterpret_cast<uint4*>(c + mv_col_bytes(a.chunk)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    if (lane == 0) sh.scale[t * a.chunk + s] = finite ? __uint_as_float(static_cast<uint32_t>(127 + ex) << 23) : NAN;
+    if (TYPE == kQ4K) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sum *= 0.03125f;
+      if (lane % 4 == 0) {
+        const __half h = __float2half_rn(sum), l = __float2half_rn(sum - __half2float(h));
+        __half* o = reinterpret_cast<__half*>(sh.sums + (t * a.chunk + s) * 32) + lane / 4;
+        o[0] = h;
+        o[8] = l;
+      }
     }
   }
 }
 
+// One span of a tile times the columns; acc: [row g | row g + 8] of the
+// lane's token(s) in each group of eight columns.
+template <unsigned TYPE, unsigned P, unsigned NT>
+__device__ __forceinline__ void mv_span(const MatvecParams& a, const MvShared& sh, const MvFrag<TYPE>& f, unsigned s,
+                                        unsigned lane, float (&acc)[NT * (P == 2 ? 2 : 4)]) {
+  const unsigned g = lane / 4, q = lane % 4, cols = a.tokens * P;
+  const uint8_t* xc[NT];
+#pragma unroll
+  for (unsigned t = 0; t < NT; ++t) {
+    const unsigned c = 8 * t + g < cols ? 8 * t + g : 0;  // columns past the tokens are not looked at
+    xc[t] = sh.col + c * mv_col_bytes(a.chunk) + 512 * s + 16 * q;
+  }
+  float sum[NT][4];
+#pragma unroll
+  for (unsigned t = 0; t < NT; ++t) sum[t][0] = sum[t][1] = sum[t][2] = sum[t][3] = 0.0f;
+  if constexpr (TYPE == kQ4K) {
+    uint32_t sc[2][2], mi[2][2];
+    float d[2], dm[2];
+#pragma unroll
+    for (unsigned h = 0; h < 2; ++h) {
+      const uint4 b = f.s[h];
+      d[h] = h2f(b.x & 0xffffu) * 16777216.0f;   // against q sc 2^-24
+      dm[h] = h2f(b.x >> 16) * 536870912.0f;     // against mi 2^-24 and sums 2^-5
+      sc[h][0] = b.y & 0x3f3f3f3fu;
+      mi[h][0] = b.z & 0x3f3f3f3fu;
+      sc[h][1] = (b.w & 0x0f0f0f0fu) | (b.y >> 2 & 0x30303030u);
+      mi[h][1] = (b.w >> 4 & 0x0f0f0f0fu) | (b.z >> 2 & 0x30303030u);
+    }
+    float m[NT][4];
+    // minima of groups 2 q and 2 q + 1 as fp16 subnormals mi 2^-24, against the sums' hi and lo parts
+    const uint32_t sel = 2 * q | (2 * q + 1) << 4;
+    const uint32_t m0 = prmt(prmt(mi[0][0], mi[0][1], sel), 0, 0x4140), m1 = prmt(prmt(mi[1][0], mi[1][1], sel), 0, 0x4140);
+#pragma unroll
+    for (unsigned t = 0; t < NT; ++t) {
+      const unsigned c = 8 * t + g, tok = c / P;
+      uint32_t b0 = 0, b1 = 0;
+      if (c < cols && (P == 1 || c % 2 == 0)) {
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(sh.sums + (tok * a.chunk + s) * 32) + q;
+        b0 = p[0];
+        b1 = p[4];
+      }
+      m[t][0] = m[t][1] = m[t][2] = m[t][3] = 0.0f;
+      mma_f16(m[t], m0, m1, m0, m1, b0, b1);
+    }
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j) {
+      const uint32_t w[4] = {f.w[j].x, f.w[j].y, f.w[j].z, f.w[j].w};
+#pragma unroll
+      for (unsigned e = 0; e < 2; ++e) {
+        const unsigned grp = 2 * j + e;
+        uint32_t av[2][4];
+#pragma unroll
+        for (unsigned h = 0; h < 2; ++h) {
+          const uint32_t v = w[2 * e + h], u = v >> 8;
+          // 1024 + sc in both halves, less 1024
+          const uint32_t k = hsub2(prmt(sc[h][grp / 4], 0x64646464u, 0x4040u | (grp % 4) * 0x0101u), 0x64006400u);
+          av[h][0] = hmul2(v & 0x000f000fu, k);
+          av[h][1] = hmul2(v & 0x00f000f0u, k);
+          av[h][2] = hmul2(u & 0x000f000fu, k);
+          av[h][3] = hmul2(u & 0x00f000f0u, k);
+        }
+#pragma unroll
+        for (unsigned t = 0; t < NT; ++t) {
+          const uint4 b = *reinterpret_cast<const uint4*>(xc[t] + 64 * grp);
+          mma_f16(sum[t], av[0][0], av[1][0], av[0][1], av[1][1], b.x, b.y);
+          mma_f16(sum[t], av[0][2], av[1][2], av[0][3], av[1][3], b.z, b.w);
+        }
+      }
+    }
+#pragma unroll
+    for (unsigned t = 0; t < NT; ++t) {
+#pragma unroll
+      for (unsigned h = 0; h < 2; ++h) {
+        if (P == 2) {
+          const unsigned tok = 4 * t + q < a.tokens ? 4 * t + q : 0;
+          const float v = d[h] * (sum[t][2 * h] + sum[t][2 * h + 1]) - dm[h] * m[t][2 * h];
+          acc[2 * t + h] = fmaf(v, sh.scale[tok * a.chunk + s], acc[2 * t + h]);
+        } else {
+#pragma unroll
+          for (unsigned c = 0; c < 2; ++c) {
+            const unsigned tok = 8 * t + 2 * q + c < a.tokens ? 8 * t + 2 * q + c : 0;
+            const float v = d[h] * sum[t][2 * h + c] - dm[h] * m[t][2 * h + c];
+            acc[4 * t + 2 * h + c] = fmaf(v, sh.scale[tok * a.chunk + s], acc[4 * t + 2 * h + c]);
+          }
+        }
+      }
+    }
+  } else {
+    const uint32_t ex[2][2] = {{f.s[0].x, f.s[0].y}, {f.s[0].z, f.s[0].w}};
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j) {
+      const uint32_t w[4] = {f.w[j].x, f.w[j].y, f.w[j].z, f.w[j].w};
+#pragma unroll
+      for (unsigned e = 0; e < 2; ++e) {
+        const unsigned grp = 2 * j + e;
+        uint32_t av[2][4];
+        float k[2];
+#pragma unroll
+        for (unsigned h = 0; h < 2; ++h) {
+          e2m1_f16(w[2 * e + h], av[h]);
+          k[h] = __uint_as_float((ex[h][grp / 4] >> (8 * (grp % 4)) & 255u) << 23);
+        }
+#pragma unroll
+        for (unsigned t = 0; t < NT; ++t) {
+          const uint4 b = *reinterpret_cast<const uint4*>(xc[t] + 64 * grp);
+          float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          mma_f16(c, av[0][0], av[1][0], av[0][1], av[1][1], b.x, b.y);
+          mma_f16(c, av[0][2], av[1][2], av[0][3], av[1][3], b.z, b.w);
+#pragma unroll
+          for (unsigned i = 0; i < 4; ++i) sum[t][i] = fmaf(c[i], k[i / 2], sum[t][i]);
+        }
+      }
+    }
+#pragma unroll
+    for (unsigned t = 0; t < NT; ++t) {
+#pragma unroll
+      for (unsigned h = 0; h < 2; ++h) {
+        if (P == 2) {
+          const unsigned tok = 4 * t + q < a.tokens ? 4 * t + q : 0;
+          acc[2 * t + h] = fmaf(sum[t][2 * h] + sum[t][2 * h + 1], sh.scale[tok * a.chunk + s], acc[2 * t + h]);
+        } else {
+#pragma unroll
+          for (unsigned c = 0; c < 2; ++c) {
+            const unsigned tok = 8 * t + 2 * q + c < a.tokens ? 8 * t + 2 * q + c : 0;
+            acc[4 * t + 2 * h + c] = fmaf(sum[t][2 * h + c], sh.scale[tok * a.chunk + s], acc[4 * t + 2 * h + c]);
+          }
+        }
+      }
+    }
+  }
+}
+
+// CTAs of W warps; `split` of them share the spans of a tile.  Tiles are
+// dealt round robin; x is prepared once a CTA, or once a tile and chunk where
+// it does not fit shared memory as a whole.
+template <unsigned TYPE, unsigned P, unsigned NT, unsigned W>
+__global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 1) matvec_kernel(const MatvecParams a) {
+  constexpr unsigned V = NT * (P == 2 ? 2 : 4);
+  extern __shared__ __align__(128) uint8_t smem[];
+  const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, q = lane % 4;
+  MvShared sh;
+  sh.col = smem;
+  sh.sums = smem + a.tokens * P * mv_col_bytes(a.chunk);
+  sh.scale = reinterpret_cast<float*>(sh.sums + (TYPE == kQ4K ? a.tokens * a.chunk * 32 : 0));
+  sh.part = sh.scale + a.tokens * a.chunk;
+  const unsigned split = a.split, per_cta = W / split, sub = warp / split, ks = warp % split;
+  bool prepared = false, bad = false;
+  for (unsigned base = blockIdx.x * per_cta; base < a.tiles; base += gridDim.x * per_cta) {
+    const unsigned tile = base + sub;
+    float acc[V];
+#pragma unroll
+    for (unsigned i = 0; i < V; ++i) acc[i] = 0.0f;
+    for (unsigned first = 0; first < a.spans; first += a.chunk) {
+      const unsigned count = min(a.chunk, a.spans - first);
+      MvFrag<TYPE> cur, next;
+      const bool any = tile < a.tiles && ks < count;
+      if (any) cur.load(a, tile, first + ks, lane);
+      if (!prepared || a.chunk < a.spans) {
+        __syncthreads();  // every warp has left the chunk before
+        mv_prepare<TYPE, P>(a, sh, first, count);
+        __syncthreads();
+        prepared = true;
+      }
+      if (any) {
+        for (unsigned s = ks; s < count; s += split) {
+          if (s + split < count) next.load(a, tile, first + s + split, lane);
+          mv_span<TYPE, P, NT>(a, sh, cur, s, lane, acc);
+          cur = next;
+        }
+      }
+    }
+    if (split > 1) {
+      float* p = sh.part + (warp * V) * 32 + lane;
+#pragma unroll
+      for (unsigned i = 0; i < V; ++i) p[32 * i] = acc[i];
+      __syncthreads();
+      if (ks == 0) {
+        for (unsigned w = 1; w < split; ++w)
+#pragma unroll
+          for (unsigned i = 0; i < V; ++i) acc[i] += p[32 * (w * V + i)];
+      }
+      __syncthreads();
+    }
+    if (ks == 0 && tile < a.tiles) {
+#pragma unroll
+      for (unsigned h = 0; h < 2; ++h) {
+        const unsigned row = tile * kMvTile + g + 8 * h;
+        if (row >= a.rows) continue;
+        float f = 1.0f;
+        if (TYPE == kMXFP4) {
+          const unsigned e = a.w[a.base_at + row];
+          f = __uint_as_float(e ? e << 23 : 0x00400000u);
+        }
+#pragma unroll
+        for (unsigned i = 0; i < V / 2; ++i) {
+          const unsigned tok = P == 2 ? 4 * i + q : 8 * (i / 2) + 2 * q + i % 2;
+          if (tok >= a.tokens) continue;
+          float v = acc[P == 2 ? 2 * i + h : 4 * (i / 2) + 2 * h + i % 2];
+          if (TYPE == kMXFP4) v *= f;
+          if (a.y_bf16) {
+            const __nv_bfloat16 o = __float2bfloat16_rn(v);
+            v = __bfloat162float(o);
+            static_cast<__nv_bfloat16*>(a.y)[tok * a.y_stride + row] = o;
+          } else {
+            static_cast<float*>(a.y)[tok * a.y_stride + row] = v;
+          }
+          bad |= !isfinite(v);
+        }
+      }
+    }
+  }
+  if (bad) atomicOr(a.status, kStNumeric);
+}
+
+// ------------------------------------------------------------ host side
+
+struct MvPlan {
+  unsigned warps, chunk, split, grid, smem;
+};
+
+constexpr unsigned kMvSmemSm = 228 * 1024, kMvSmemCta = 227 * 1024;
+
+// Shared memory of a CTA; the parts only where warps share tiles.
+inline size_t mv_smem(unsigned type, unsigned P, unsigned tokens, unsigned values, unsigned warps, unsigned chunk, bool part) {
+  return tokens * P * mv_col_bytes(chunk) + static_cast<size_t>(tokens) * chunk * ((type == FRC_Q4_K ? 32 : 0) + 4) +
+         (part ? static_cast<size_t>(warps) * values * 128 : 0);
+}
+
+// Two CTAs of eight warps an SM where the vectors fit twice, else one of 16;
+// K in chunks where they do not fit once.  Warps share a tile (up to eight)
+// until the tiles fill the GPU evenly: the last round of tiles should not
+// leave more than a twentieth of the CTAs idle.
+inline MvPlan mv_plan(unsigned type, unsigned P, unsigned nt, unsigned tokens, const MvLayout& l, unsigned sms) {
+  const unsigned values = nt * (P == 2 ? 2 : 4);
+  MvPlan p{};
+  p.chunk = l.spans;
+  p.warps = 8;
+  if (mv_smem(type, P, tokens, values, 8, p.chunk, true) > (kMvSmemSm - 2048) / 2) {
+    p.warps = 16;
+    while (mv_smem(type, P, tokens, values, 16, p.chunk, true) > kMvSmemCta) p.chunk = (p.chunk + 1) / 2;
+  }
+  const unsigned resident = sms * (p.warps == 8 ? 2 : 1);
+  double best = 0;
+  for (unsigned split = 1; split <= 8 && (split == 1 || split / 2 < p.chunk); split *= 2) {
+    const unsigned per = p.warps / split, ctas = (l.tiles + per - 1) / per, rounds = (ctas + resident - 1) / resident;
+    const double use = static_cast<double>(l.tiles) / (static_cast<double>(rounds) * resident * per);
+    if (use > best * 1.02) {
+      best = use;
+      p.split = split;
+      p.grid = ctas < resident ? ctas : resident;
+    }
+    if (use > 0.95) break;
+  }
+  p.smem = static_cast<unsigned>(mv_smem(type, P, tokens, values, p.warps, p.chunk, p.split > 1));
+  return p;
+}
+
+template <unsigned TYPE, unsigned P, unsigned NT, unsigned W>
+inline cudaError_t mv_launch(const MatvecParams& a, const MvPlan& p, cudaStream_t s) {
+  if (p.smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(matvec_kernel<TYPE, P, NT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(p.smem));
+    if (e != cudaSuccess) return e;
+  }
+  matvec_kernel<TYPE, P, NT, W><<<p.grid, 32 * W, p.smem, s>>>(a);
+  return cudaGetLastError();
+}
+template <unsigned TYPE, unsigned P, unsigned NT>
+inline cudaError_t mv_launch_w(const MatvecParams& a, const MvPlan& p, cudaStream_t s) {
+  return p.warps == 8 ? mv_launch<TYPE, P, NT, 8>(a, p, s) : mv_launch<TYPE, P, NT, 16>(a, p, s);
+}
+
 template <unsigned TYPE>
-inline void launch_matvec(const MatvecParams& a, unsigned xt, unsigned yt, cudaStream_t s) {
-  const unsigned grid = (a.rows + 7) / 8;
-  if (xt == FRC_F32 && yt == FRC_F32) matvec_kernel<TYPE, float, float><<<grid, 256, 0, s>>>(a);
-  else if (xt == FRC_F32) matvec_kernel<TYPE, float, __nv_bfloat16><<<grid, 256, 0, s>>>(a);
-  else if (yt == FRC_F32) matvec_kernel<TYPE, __nv_bfloat16, float><<<grid, 256, 0, s>>>(a);
-  else matvec_kernel<TYPE, __nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, s>>>(a);
+inline cudaError_t launch_matvec(MatvecParams& a, const MvLayout& l, unsigned x_type, unsigned sms, cudaStream_t s) {
+  const unsigned P = x_type == FRC_F32 ? 2 : 1, cols = a.tokens * P, nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
+  const MvPlan p = mv_plan(TYPE, P, nt, a.tokens, l, sms);
+  a.tile_bytes = l.tile_bytes; a.base_at = l.base_at; a.tiles = l.tiles; a.spans = l.spans; a.pieces_last = l.pieces_last;
+  a.chunk = p.chunk; a.split = p.split;
+  if (P == 2) {
+    if (nt == 1) return mv_launch_w<TYPE, 2, 1>(a, p, s);
+    if (nt == 2) return mv_launch_w<TYPE, 2, 2>(a, p, s);
+    return mv_launch_w<TYPE, 2, 4>(a, p, s);
+  }
+  if (nt == 1) return mv_launch_w<TYPE, 1, 1>(a, p, s);
+  return mv_launch_w<TYPE, 1, 2>(a, p, s);
 }
 
 }  // namespace frc
