@@ -1900,16 +1900,10 @@ static int route(frc_context* c, unsigned tokens, unsigned experts, const void* 
     a.pcount = reinterpret_cast<unsigned*>(a.psum + static_cast<size_t>(parts) * experts);
     a.pvalid = a.pcount + static_cast<size_t>(parts) * experts;
   }
-  if (type == FRC_BF16) launch_route<__nv_bfloat16>(a, expert_in == nullptr, b != nullptr, s);
-  else launch_route<float>(a, expert_in == nullptr, b != nullptr, s);
-  CK(cudaGetLastError());
-  ++c->launches;
-  if (b) {
-    const RouteFinish f{a.psum, a.pcount, a.pvalid, parts, experts, b->loss, b->count, b->prob};
-    route_finish_kernel<<<1, kMaxExperts, 0, s>>>(f);
-    CK(cudaGetLastError());
-    ++c->launches;
-  }
+  RouteFinish f{};
+  if (b) f = RouteFinish{a.psum, a.pcount, a.pvalid, parts, experts, b->loss, b->count, b->prob};
+  CK(launch_route(a, f, type, expert_in == nullptr, b != nullptr, static_cast<unsigned>(c->sms), s));
+  c->launches += b && tokens > kRouteOneCluster ? 2 : 1;
   return FRC_OK;
 }
 
@@ -1950,11 +1944,7 @@ int frc_route_backward_device(frc_context* c, unsigned tokens, unsigned experts,
   a.logits = logits; a.stride = stride; a.d_stride = d_stride; a.valid = valid; a.expert = expert; a.d_gate = d_gate;
   a.count = count; a.d_loss = d_loss; a.d_logits = d_logits; a.tokens = tokens; a.experts = experts;
   a.shared = flags & FRC_ROUTE_SHARED; a.status = c->status;
-  const unsigned grid = (tokens + kRouteWarps - 1) / kRouteWarps;
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (type == FRC_BF16) route_backward_kernel<__nv_bfloat16><<<grid, 32 * kRouteWarps, 0, s>>>(a);
-  else route_backward_kernel<float><<<grid, 32 * kRouteWarps, 0, s>>>(a);
-  CK(cudaGetLastError());
+  CK(launch_backward(a, type, static_cast<unsigned>(c->sms), static_cast<cudaStream_t>(stream)));
   ++c->launches;
   return FRC_OK;
 }

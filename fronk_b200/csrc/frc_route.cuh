@@ -11,14 +11,17 @@
 #pragma once
 #include <cuda_bf16.h>
 
+#include "../../include/fronk_b200.h"
 #include "frc_device.cuh"
 
 namespace frc {
 
 constexpr unsigned kTopK = 10, kGates = 11, kMaxExperts = 512;
 constexpr unsigned kRouteSlots = kMaxExperts / 32;  // logits a lane holds
-constexpr unsigned kRouteWarps = 4;                 // warps a CTA
-constexpr unsigned kRouteCtas = 296;                // CTAs that make statistics, at most
+constexpr unsigned kRouteWarps = 24;                // warps a CTA, at most
+constexpr unsigned kRouteSums = 8;                  // arrays of sums a CTA folds its warps into
+constexpr unsigned kRouteCtas = 160;                // CTAs that make statistics, at most
+constexpr unsigned kRouteCluster = 8;               // CTAs that finish them
 
 struct RouteParams {
   const void* logits;
@@ -64,8 +67,6 @@ template <>
 __device__ __forceinline__ float logit<float>(const float* p) { return *p; }
 template <>
 __device__ __forceinline__ float logit<__nv_bfloat16>(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void store_grad(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_grad(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 // Unsigned keys in the order of floats (no NaN); 0 lies below every float.
 __device__ __forceinline__ unsigned order_key(float v) {
@@ -80,22 +81,213 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (unsigned o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// Maxima that are NaN when a value is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float d;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
+  return d;
+}
 __device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (unsigned o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+  float d;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
+  return d;
 }
 __device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + expf(-v)); }
-// exp(v - m) with v <= m, both finite or v = -inf.
-__device__ __forceinline__ float exp_below(float v, float m) { return exp2f((v - m) * 1.4426950408889634f); }
+// exp(v - m) with v <= m, m finite; v may be -inf.
+__device__ __forceinline__ float exp_below(float v, float m) {
+  float d;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"((v - m) * 1.4426950408889634f));
+  return d;
+}
 
-// One warp a row; SELECT: choose experts and gates, STATS: sum p and counts
-// of the chosen (or given) experts over the CTA's rows.
-template <typename L, bool SELECT, bool STATS>
-__global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteParams a) {
-  __shared__ float s_psum[STATS ? kRouteWarps : 1][STATS ? kMaxExperts : 1];
+// A row's E logits over a warp, kRouteSlots a lane: V neighbours a load (V = 1
+// where rows are not 16-byte aligned), slot i of a lane being column
+// col<V>(i, lane); columns past E are -inf.
+template <unsigned V>
+__device__ __forceinline__ unsigned col(unsigned i, unsigned lane) {
+  return i / V * (32 * V) + V * lane + i % V;
+}
+template <typename L, unsigned V>
+struct RowLoad {
+  static constexpr unsigned kWords = V == 1 ? kRouteSlots : kRouteSlots * sizeof(L) / 4;
+  uint32_t w[kWords];  // fp32 bits, or pairs of bf16, or (V = 1) a value each
+
+  __device__ __forceinline__ void load(const L* row, unsigned E, unsigned lane) {
+    if constexpr (V == 1) {
+#pragma unroll
+      for (unsigned i = 0; i < kRouteSlots; ++i) w[i] = __float_as_uint(lane + 32 * i < E ? logit(row + lane + 32 * i) : -INFINITY);
+    } else {
+#pragma unroll
+      for (unsigned j = 0; j < kRouteSlots / V; ++j) {
+        const unsigned c = col<V>(j * V, lane);
+        uint4 v;
+        if (c + V <= E) {
+          v = *reinterpret_cast<const uint4*>(row + c);
+        } else if constexpr (sizeof(L) == 4) {
+          uint32_t e[4];
+#pragma unroll
+          for (unsigned k = 0; k < 4; ++k) e[k] = __float_as_uint(c + k < E ? logit(row + c + k) : -INFINITY);
+          v = make_uint4(e[0], e[1], e[2], e[3]);
+        } else {
+          uint32_t e[4];
+#pragma unroll
+          for (unsigned k = 0; k < 4; ++k) {
+            const float x = c + 2 * k < E ? logit(row + c + 2 * k) : -INFINITY, y = c + 2 * k + 1 < E ? logit(row + c + 2 * k + 1) : -INFINITY;
+            e[k] = __float_as_uint(x) >> 16 | (__float_as_uint(y) & 0xffff0000u);
+          }
+          v = make_uint4(e[0], e[1], e[2], e[3]);
+        }
+        w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
+      }
+    }
+  }
+  __device__ __forceinline__ float value(unsigned i) const {
+    if constexpr (V == 1 || sizeof(L) == 4) return __uint_as_float(w[i]);
+    else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+};
+
+// The ten largest of a row in order, ties by the lower column: lane r < 10
+// gets the r-th one's column and value.
+//
+// The tenth largest of the lanes' maxima bounds the tenth largest logit from
+// below, so only the logits at or above it (a dozen as a rule) are collected
+// and ranked against one another.  Where ties make them more than 32, ten
+// searches over the whole row choose one by one.
+template <unsigned V>
+__device__ __forceinline__ void choose(const float (&v)[kRouteSlots], unsigned E, unsigned lane, float top, float2* cand,
+                                       unsigned* id, float* val) {
+  float rest = top, bound = 0.0f;
+#pragma unroll
+  for (unsigned r = 0; r < kTopK; ++r) {
+    bound = warp_max(rest);
+    rest = rest == bound ? -INFINITY : rest;
+  }
+  unsigned total = 0;
+#pragma unroll
+  for (unsigned i = 0; i < kRouteSlots; ++i) {
+    const unsigned c = col<V>(i, lane);
+    const bool in = v[i] >= bound && c < E;
+    const unsigned m = __ballot_sync(0xffffffffu, in);
+    if (in) {
+      const unsigned at = total + __popc(m & ((1u << lane) - 1u));
+      if (at < 32) cand[at] = make_float2(v[i], __uint_as_float(c));
+    }
+    total += __popc(m);
+  }
+  __syncwarp();
+  if (total <= 32) {
+    const float2 mine = lane < total ? cand[lane] : make_float2(-INFINITY, 0.0f);
+    const unsigned c = __float_as_uint(mine.y);
+    unsigned rank = 0;
+    for (unsigned k = 0; k < total; ++k) {
+      const float2 o = cand[k];
+      rank += o.x > mine.x || (o.x == mine.x && __float_as_uint(o.y) < c);
+    }
+    __syncwarp();
+    if (lane < total) cand[rank] = mine;  // ranks are distinct
+    __syncwarp();
+    const float2 r = cand[lane < total ? lane : 0];
+    *id = __float_as_uint(r.y);
+    *val = r.x;
+  } else {
+    unsigned left = 0;
+#pragma unroll
+    for (unsigned i = 0; i < kRouteSlots; ++i) left |= (col<V>(i, lane) < E ? 1u : 0u) << i;
+    for (unsigned r = 0; r < kTopK; ++r) {
+      unsigned best = 0, at = 0;
+#pragma unroll
+      for (unsigned i = 0; i < kRouteSlots; ++i) {
+        const unsigned k = left >> i & 1u ? order_key(v[i] + 0.0f) : 0u;  // -0 becomes +0: equal logits are ties
+        if (k > best) { best = k; at = i; }
+      }
+      const unsigned high = __reduce_max_sync(0xffffffffu, best);
+      const unsigned win = __reduce_min_sync(0xffffffffu, best == high ? col<V>(at, lane) : 0xffffffffu);
+      if (best == high && col<V>(at, lane) == win) left &= ~(1u << at);
+      if (lane == r) { *id = win; *val = key_value(high); }
+    }
+  }
+  __syncwarp();
+}
+
+// Sums of the CTAs' parts: the loss from prob and count of E experts, the
+// experts dealt over the CTAs of a cluster.  part(k, e, p, c) adds part k of
+// expert e in order; every thread of every CTA of the cluster calls this.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Address of the same shared variable in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_map(const void* p, uint32_t rank) {
+  uint32_t d;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_u32(p)), "r"(rank));
+  return d;
+}
+__device__ __forceinline__ unsigned ld_cluster(uint32_t a) {
+  unsigned v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ double ld_cluster_f64(uint32_t a) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// Writes prob and count of one expert and returns its term of the loss.
+__device__ __forceinline__ double finish_expert(const RouteFinish& f, unsigned e, double p, unsigned c, unsigned n) {
+  p /= n ? n : 1u;
+  f.prob[e] = static_cast<float>(p);
+  f.count[e] = c;
+  return p * c;
+}
+// Sums the CTA's terms (blockDim.x threads), then the cluster's in rank order.
+__device__ __forceinline__ void finish_loss(const RouteFinish& f, double term, unsigned n, double* s_term, double* s_loss) {
+  const unsigned warp = threadIdx.x / 32, warps = blockDim.x / 32;
+#pragma unroll
+  for (unsigned o = 16; o; o >>= 1) term += __shfl_xor_sync(0xffffffffu, term, o);
+  if ((threadIdx.x & 31) == 0) s_term[warp] = term;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double l = 0.0;
+    for (unsigned w = 0; w < warps; ++w) l += s_term[w];
+    *s_loss = l;
+  }
+  cluster_sync();
+  if (cluster_rank() == 0 && threadIdx.x == 0) {
+    double l = 0.0;
+    for (unsigned r = 0; r < kRouteCluster; ++r) l += ld_cluster_f64(cluster_map(s_loss, r));
+    const double m = n ? n : 1u;
+    *f.loss = static_cast<float>(l * f.experts / (kTopK * m));
+    f.count[f.experts] = n;
+  }
+  cluster_sync();  // no CTA leaves while another reads its shared memory
+}
+
+// Statistics: none, as parts for route_finish_kernel, or finished by the one
+// cluster that runs (few rows).
+enum : int { kStatsNone = 0, kStatsParts = 1, kStatsCluster = 2 };
+
+// One warp a row; SELECT: choose experts and gates; STATS: sums of p and
+// counts of the chosen (or given) experts over the CTA's rows.  The next
+// row's logits are on their way while one is worked on.
+template <typename L, unsigned V, bool SELECT, int STATS>
+__global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteParams a, const RouteFinish f) {
+  __shared__ float s_psum[STATS ? kRouteSums : 1][STATS ? kMaxExperts : 1];
   __shared__ unsigned s_count[STATS ? kMaxExperts : 1], s_valid;
-  const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31, E = a.experts;
+  __shared__ float2 s_cand[SELECT ? kRouteWarps : 1][32];
+  __shared__ double s_term[STATS == kStatsCluster ? kRouteWarps : 1], s_loss;
+  const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = blockDim.x / 32, E = a.experts;
+  const L* logits = static_cast<const L*>(a.logits);
   float psum[STATS ? kRouteSlots : 1] = {};
   unsigned nvalid = 0;
   if (STATS) {
@@ -103,50 +295,48 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RoutePara
     if (threadIdx.x == 0) s_valid = 0;
     __syncthreads();
   }
-  for (unsigned t = blockIdx.x * kRouteWarps + warp; t < a.tokens; t += gridDim.x * kRouteWarps) {
-    const L* row = static_cast<const L*>(a.logits) + t * a.stride;
-    const bool valid = !a.valid || a.valid[t];
+  const unsigned step = gridDim.x * warps;
+  unsigned t = blockIdx.x * warps + warp;
+  RowLoad<L, V> next;
+  bool next_valid = false;
+  if (t < a.tokens) {
+    next_valid = !a.valid || a.valid[t];
+    next.load(logits + t * a.stride, E, lane);
+  }
+  for (; t < a.tokens; t += step) {
+    const L* row = logits + t * a.stride;
+    const bool valid = next_valid;
     float v[kRouteSlots];
-    bool bad = false;
 #pragma unroll
-    for (unsigned i = 0; i < kRouteSlots; ++i) {
-      const unsigned e = lane + 32 * i;
-      v[i] = e < E && valid ? logit(row + e) + 0.0f : -INFINITY;  // -0 becomes +0: equal logits are ties
-      bad |= !(v[i] < INFINITY);
-    }
-    bad = __any_sync(0xffffffffu, bad);
-    if (bad && lane == 0) atomicOr(a.status, kStNumeric);
-    const bool use = valid && !bad;
+    for (unsigned i = 0; i < kRouteSlots; ++i) v[i] = next.value(i);
     unsigned id = lane;
     float val = -INFINITY;
+    if (STATS && !SELECT && lane < kTopK) id = a.expert_in[static_cast<size_t>(t) * kTopK + lane];
+    if (t + step < a.tokens) {
+      next_valid = !a.valid || a.valid[t + step];
+      next.load(row + step * a.stride, E, lane);
+    }
+    float top = v[0];
+#pragma unroll
+    for (unsigned i = 1; i < kRouteSlots; ++i) top = max_nan(top, v[i]);
+    const float m = warp_max_nan(top);
+    const bool bad = valid && !(m < INFINITY);
+    if (bad && lane == 0) atomicOr(a.status, kStNumeric);
+    const bool use = valid && !bad;
     if (SELECT) {
+      float g = 0.0f;
       if (use) {
-        unsigned left = 0;
-#pragma unroll
-        for (unsigned i = 0; i < kRouteSlots; ++i) left |= (lane + 32 * i < E ? 1u : 0u) << i;
-        for (unsigned r = 0; r < kTopK; ++r) {
-          unsigned best = 0, slot = 0;
-#pragma unroll
-          for (unsigned i = 0; i < kRouteSlots; ++i) {
-            const unsigned k = left >> i & 1u ? order_key(v[i]) : 0u;
-            if (k > best) { best = k; slot = i; }
+        choose<V>(v, E, lane, top, s_cand[warp], &id, &val);
+        const float e = lane < kTopK && m > -INFINITY ? expf(val - m) : 0.0f;
+        const float sum = warp_sum(e);
+        g = sum > 0.0f ? e / sum : 0.0f;
+        if (lane == kTopK && a.shared) {
+          const float s = logit(row + E);
+          g = sigmoid(s);
+          if (s != s) {
+            g = 0.0f;
+            atomicOr(a.status, kStNumeric);
           }
-          const unsigned top = __reduce_max_sync(0xffffffffu, best);
-          const unsigned win = __reduce_min_sync(0xffffffffu, best == top ? lane + 32 * slot : 0xffffffffu);
-          if ((win & 31) == lane) left &= ~(1u << (win >> 5));
-          if (lane == r) { id = win; val = key_value(top); }
-        }
-      }
-      const float m = __shfl_sync(0xffffffffu, val, 0);
-      const float e = lane < kTopK && m > -INFINITY ? expf(val - m) : 0.0f;
-      const float sum = warp_sum(e);
-      float g = sum > 0.0f ? e / sum : 0.0f;
-      if (lane == kTopK && a.shared && use) {
-        const float s = logit(row + E);
-        g = sigmoid(s);
-        if (s != s) {
-          g = 0.0f;
-          atomicOr(a.status, kStNumeric);
         }
       }
       if (lane < kTopK) a.expert[static_cast<size_t>(t) * kTopK + lane] = static_cast<uint16_t>(id);
@@ -155,16 +345,11 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RoutePara
     if (STATS && use) {
       if (lane < kTopK) {
         if (!SELECT) {
-          id = a.expert_in[static_cast<size_t>(t) * kTopK + lane];
           if (id < E) val = logit(row + id);
           else atomicOr(a.status, kStInvalid);
         }
         if (val > -INFINITY) atomicAdd(&s_count[id], 1u);
       }
-      float m = -INFINITY;
-#pragma unroll
-      for (unsigned i = 0; i < kRouteSlots; ++i) m = fmaxf(m, v[i]);
-      m = warp_max(m);
       ++nvalid;
       if (m > -INFINITY) {
         float z = 0.0f;
@@ -180,150 +365,297 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RoutePara
     }
   }
   if (STATS) {
-#pragma unroll
-    for (unsigned i = 0; i < kRouteSlots; ++i) s_psum[warp][lane + 32 * i] = psum[i];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (lane == 0) atomicAdd(&s_valid, nvalid);
-    __syncthreads();
-    for (unsigned e = threadIdx.x; e < E; e += blockDim.x) {
-      float s = 0.0f;
+    for (unsigned w = 0; w < warps; w += kRouteSums) {  // in a fixed order
+      if (warp >= w && warp < w + kRouteSums)
 #pragma unroll
-      for (unsigned w = 0; w < kRouteWarps; ++w) s += s_psum[w][e];
-      a.psum[static_cast<size_t>(blockIdx.x) * E + e] = s;
-      a.pcount[static_cast<size_t>(blockIdx.x) * E + e] = s_count[e];
+        for (unsigned i = 0; i < kRouteSlots; ++i) {
+          float* p = &s_psum[warp - w][col<V>(i, lane)];
+          *p = (w ? *p : 0.0f) + psum[i];
+        }
+      __syncthreads();
     }
-    if (threadIdx.x == 0) a.pvalid[blockIdx.x] = s_valid;
+    const unsigned sums = warps < kRouteSums ? warps : kRouteSums;
+    if (STATS == kStatsParts) {
+      for (unsigned e = threadIdx.x; e < E; e += blockDim.x) {
+        float s = 0.0f;
+        for (unsigned w = 0; w < sums; ++w) s += s_psum[w][e];
+        a.psum[static_cast<size_t>(blockIdx.x) * E + e] = s;
+        a.pcount[static_cast<size_t>(blockIdx.x) * E + e] = s_count[e];
+      }
+      if (threadIdx.x == 0) a.pvalid[blockIdx.x] = s_valid;
+    } else {
+      for (unsigned e = threadIdx.x; e < E; e += blockDim.x) {
+        float s = 0.0f;
+        for (unsigned w = 0; w < sums; ++w) s += s_psum[w][e];
+        s_psum[0][e] = s;
+      }
+      cluster_sync();
+      const unsigned own = (E + kRouteCluster - 1) / kRouteCluster, e = cluster_rank() * own + threadIdx.x;
+      unsigned n = 0;
+      double term = 0.0;
+      for (unsigned r = 0; r < kRouteCluster; ++r) n += ld_cluster(cluster_map(&s_valid, r));
+      if (threadIdx.x < own && e < E) {
+        double p = 0.0;
+        unsigned c = 0;
+        for (unsigned r = 0; r < kRouteCluster; ++r) {
+          p += __uint_as_float(ld_cluster(cluster_map(&s_psum[0][e], r)));
+          c += ld_cluster(cluster_map(&s_count[e], r));
+        }
+        term = finish_expert(f, e, p, c, n);
+      }
+      finish_loss(f, term, n, s_term, &s_loss);
+    }
   }
 }
 
-// Sums the CTAs' parts in order (one thread an expert, in double) and forms
-// the loss.
-__global__ void __launch_bounds__(kMaxExperts) route_finish_kernel(const RouteFinish a) {
-  __shared__ double s_part[kMaxExperts / 32];
-  __shared__ unsigned s_n;
-  const unsigned e = threadIdx.x, lane = e & 31;
-  if (e < 32) {
-    unsigned n = 0;
-    for (unsigned k = lane; k < a.parts; k += 32) n += a.pvalid[k];
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (e == 0) s_n = n;
-  }
+// Sums the CTAs' parts in order, in double, and forms the loss: one cluster,
+// eight threads an expert that take every eighth part.
+constexpr unsigned kFinishThreads = kMaxExperts / kRouteCluster * 8;
+__global__ void __cluster_dims__(kRouteCluster, 1, 1) __launch_bounds__(kFinishThreads)
+    route_finish_kernel(const RouteFinish f) {
+  __shared__ double s_p[8][kMaxExperts / kRouteCluster], s_term[kFinishThreads / 32], s_loss;
+  __shared__ unsigned s_c[8][kMaxExperts / kRouteCluster];
+  const unsigned own = kMaxExperts / kRouteCluster, i = threadIdx.x % own, k0 = threadIdx.x / own;
+  const unsigned e = cluster_rank() * own + i;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   double p = 0.0;
   unsigned c = 0;
-  if (e < a.experts)
-    for (unsigned k = 0; k < a.parts; ++k) {
-      p += a.psum[static_cast<size_t>(k) * a.experts + e];
-      c += a.pcount[static_cast<size_t>(k) * a.experts + e];
+  if (e < f.experts) {
+#pragma unroll 8
+    for (unsigned k = k0; k < f.parts; k += 8) {
+      p += f.psum[static_cast<size_t>(k) * f.experts + e];
+      c += f.pcount[static_cast<size_t>(k) * f.experts + e];
     }
-  __syncthreads();
-  const double n = s_n ? s_n : 1u;
-  p /= n;
-  if (e < a.experts) {
-    a.prob[e] = static_cast<float>(p);
-    a.count[e] = c;
   }
-  if (e == 0) a.count[a.experts] = s_n;
-  double l = p * c;
-#pragma unroll
-  for (unsigned o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  if (lane == 0) s_part[e / 32] = l;
+  unsigned n = 0;
+  for (unsigned k = threadIdx.x & 31; k < f.parts; k += 32) n += f.pvalid[k];
+  n = __reduce_add_sync(0xffffffffu, n);
+  s_p[k0][i] = p;
+  s_c[k0][i] = c;
   __syncthreads();
-  if (e == 0) {
-    l = 0.0;
-    for (unsigned w = 0; w < kMaxExperts / 32; ++w) l += s_part[w];
-    *a.loss = static_cast<float>(l * a.experts / (kTopK * n));
+  double term = 0.0;
+  if (k0 == 0 && e < f.experts) {
+    for (unsigned k = 1; k < 8; ++k) {
+      p += s_p[k][i];
+      c += s_c[k][i];
+    }
+    term = finish_expert(f, e, p, c, n);
+  }
+  finish_loss(f, term, n, s_term, &s_loss);
+}
+
+__device__ __forceinline__ void store_grad(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_grad(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+template <typename L, unsigned V>
+__device__ __forceinline__ void store_row(L* row, unsigned E, unsigned lane, const float (&d)[kRouteSlots]) {
+  if constexpr (V == 1) {
+#pragma unroll
+    for (unsigned i = 0; i < kRouteSlots; ++i)
+      if (lane + 32 * i < E) store_grad(row + lane + 32 * i, d[i]);
+  } else {
+#pragma unroll
+    for (unsigned j = 0; j < kRouteSlots / V; ++j) {
+      const unsigned c = col<V>(j * V, lane);
+      if (c + V <= E) {
+        if constexpr (sizeof(L) == 4) {
+          *reinterpret_cast<float4*>(row + c) = make_float4(d[4 * j], d[4 * j + 1], d[4 * j + 2], d[4 * j + 3]);
+        } else {
+          uint32_t w[4];
+#pragma unroll
+          for (unsigned k = 0; k < 4; ++k) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(d[8 * j + 2 * k], d[8 * j + 2 * k + 1]);
+            w[k] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          *reinterpret_cast<uint4*>(row + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      } else {
+#pragma unroll
+        for (unsigned k = 0; k < V; ++k)
+          if (c + k < E) store_grad(row + c + k, d[j * V + k]);
+      }
+    }
   }
 }
 
-// One warp a row: d_logits = routing term + balance term.
-template <typename L>
-__global__ void __launch_bounds__(32 * kRouteWarps) route_backward_kernel(const RouteBackwardParams a) {
-  const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31, E = a.experts;
-  const float n = a.count ? static_cast<float>(a.count[E]) : 0.0f;
-  const float scale = n > 0.0f ? *a.d_loss * static_cast<float>(E) / (static_cast<float>(kTopK) * n * n) : 0.0f;
-  for (unsigned t = blockIdx.x * kRouteWarps + warp; t < a.tokens; t += gridDim.x * kRouteWarps) {
-    const L* row = static_cast<const L*>(a.logits) + t * a.stride;
+// One warp a row: the balance term of every logit is stored first, then lanes
+// 0-9 store the chosen ones' sum with the routing term.  BALANCE off: only
+// the chosen logits are read.
+template <typename L, unsigned V, bool BALANCE>
+__global__ void __launch_bounds__(256, 3) route_backward_kernel(const RouteBackwardParams a) {
+  __shared__ float s_count[BALANCE ? kMaxExperts : 1];
+  const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = blockDim.x / 32, E = a.experts;
+  const L* logits = static_cast<const L*>(a.logits);
+  float scale = 0.0f;
+  if (BALANCE) {
+    for (unsigned e = threadIdx.x; e < kMaxExperts; e += blockDim.x) s_count[e] = e < E ? static_cast<float>(a.count[e]) : 0.0f;
+    const float n = static_cast<float>(a.count[E]);
+    scale = n > 0.0f ? *a.d_loss * static_cast<float>(E) / (static_cast<float>(kTopK) * n * n) : 0.0f;
+    __syncthreads();
+  }
+  const unsigned step = gridDim.x * warps;
+  unsigned t = blockIdx.x * warps + warp;
+  RowLoad<L, V> next;
+  if (BALANCE && t < a.tokens) next.load(logits + t * a.stride, E, lane);
+  for (; t < a.tokens; t += step) {
+    const L* row = logits + t * a.stride;
     L* out = static_cast<L*>(a.d_logits) + t * a.d_stride;
     const bool valid = !a.valid || a.valid[t];
-    float d[kRouteSlots] = {};
+    float d[kRouteSlots];
+    // the chosen experts of lanes 0-9, the shared logit in lane 10
+    unsigned id = E + 1;
+    float val = -INFINITY, dg = 0.0f;
+    if (a.d_gate && valid) {
+      if (lane < kTopK) id = a.expert[static_cast<size_t>(t) * kTopK + lane];
+      if (lane < kGates) dg = a.d_gate[static_cast<size_t>(t) * kGates + lane];
+      if (lane == kTopK && a.shared) val = logit(row + E);
+    }
+#pragma unroll
+    for (unsigned i = 0; i < kRouteSlots; ++i) d[i] = BALANCE ? next.value(i) : 0.0f;
+    if (BALANCE && t + step < a.tokens) next.load(row + step * a.stride, E, lane);
+    if (lane < kTopK && a.d_gate && valid) {
+      if (id < E) val = logit(row + id);
+      else atomicOr(a.status, kStInvalid);
+      if (!(val < INFINITY)) atomicOr(a.status, kStNumeric);
+    }
     float m = -INFINITY, zi = 0.0f, dot = 0.0f;
-    if (valid && a.count) {
-      bool bad = false;
+    if (BALANCE) {
+      m = d[0];
 #pragma unroll
-      for (unsigned i = 0; i < kRouteSlots; ++i) {
-        const unsigned e = lane + 32 * i;
-        d[i] = e < E ? logit(row + e) : -INFINITY;
-        bad |= !(d[i] < INFINITY);
-        m = fmaxf(m, d[i]);
-      }
-      if (bad) atomicOr(a.status, kStNumeric);
-      m = warp_max(m);
-      float z = 0.0f;
+      for (unsigned i = 1; i < kRouteSlots; ++i) m = max_nan(m, d[i]);
+      m = warp_max_nan(m);
+      if (valid && !(m < INFINITY) && lane == 0) atomicOr(a.status, kStNumeric);
+      if (valid && m > -INFINITY) {
+        float z = 0.0f;
 #pragma unroll
-      for (unsigned i = 0; i < kRouteSlots; ++i) {
-        const unsigned e = lane + 32 * i;
-        d[i] = m > -INFINITY ? exp_below(d[i], m) : 0.0f;
-        z += d[i];
-        if (e < E) dot = fmaf(d[i], static_cast<float>(a.count[e]), dot);
-      }
-      z = warp_sum(z);
-      zi = z > 0.0f ? 1.0f / z : 0.0f;
-      dot = warp_sum(dot) * zi;
+        for (unsigned i = 0; i < kRouteSlots; ++i) {
+          d[i] = exp_below(d[i], m);
+          z += d[i];
+          dot = fmaf(d[i], s_count[col<V>(i, lane)], dot);
+        }
+        zi = 1.0f / warp_sum(z);
+        dot = warp_sum(dot) * zi;
+        const float k = scale * zi;
 #pragma unroll
-      for (unsigned i = 0; i < kRouteSlots; ++i) {
-        const unsigned e = lane + 32 * i;
-        if (e < E) d[i] = scale * (d[i] * zi) * (static_cast<float>(a.count[e]) - dot);
+        for (unsigned i = 0; i < kRouteSlots; ++i) d[i] = (k * d[i]) * (s_count[col<V>(i, lane)] - dot);
+      } else {
+#pragma unroll
+        for (unsigned i = 0; i < kRouteSlots; ++i) d[i] = 0.0f;
       }
     }
-    float d_shared = 0.0f;
-    if (valid && a.d_gate) {
-      unsigned id = 0;
-      float val = -INFINITY, dg = 0.0f;
-      if (lane < kTopK) {
-        id = a.expert[static_cast<size_t>(t) * kTopK + lane];
-        dg = a.d_gate[static_cast<size_t>(t) * kGates + lane];
-        if (id < E) val = logit(row + id);
-        else atomicOr(a.status, kStInvalid);
-        if (!(val < INFINITY)) atomicOr(a.status, kStNumeric);
-      }
-      const float mk = warp_max(val);
+    __syncwarp();  // d_logits may be logits: every lane has read the row
+    store_row<L, V>(out, E, lane, d);
+    if (a.d_gate) {
+      const float chosen = lane < kTopK ? val : -INFINITY, mk = warp_max(chosen);
       float g = lane < kTopK && mk > -INFINITY ? expf(val - mk) : 0.0f;
       const float s = warp_sum(g);
       g = s > 0.0f ? g / s : 0.0f;
       const float gd = warp_sum(g * dg);
-      const float term = g * (dg - gd);
-      for (unsigned r = 0; r < kTopK; ++r) {  // the same index twice adds twice
-        const unsigned er = __shfl_sync(0xffffffffu, id, r);
-        const float tr = __shfl_sync(0xffffffffu, term, r);
-#pragma unroll
-        for (unsigned i = 0; i < kRouteSlots; ++i) d[i] += lane + 32 * i == er && er < E ? tr : 0.0f;
+      const float own = g * (dg - gd);
+      float term = own;
+      const unsigned same = __match_any_sync(0xffffffffu, id) & 0x3ffu;
+      const bool twice = lane < kTopK && same != 1u << lane;
+      if (__any_sync(0xffffffffu, twice)) {  // the same index twice adds twice
+        if (twice) term = 0.0f;
+        for (unsigned r = 0; r < kTopK; ++r) {
+          const float o = __shfl_sync(0xffffffffu, own, r);
+          if (twice && (same >> r & 1u)) term += o;
+        }
       }
-      if (a.shared) {
-        const float sg = sigmoid(logit(row + E));
-        d_shared = sg * (1.0f - sg) * a.d_gate[static_cast<size_t>(t) * kGates + kTopK];
-      }
+      if (BALANCE && lane < kTopK && zi > 0.0f && id < E) term += (scale * zi * exp_below(val, m)) * (s_count[id] - dot);
+      __syncwarp();  // behind the row's stores
+      if (valid && lane < kTopK && id < E) store_grad(out + id, term);
     }
-    __syncwarp();  // d_logits may be logits: every lane has read the row
-#pragma unroll
-    for (unsigned i = 0; i < kRouteSlots; ++i) {
-      const unsigned e = lane + 32 * i;
-      if (e < E) store_grad(out + e, d[i]);
+    if (a.shared && lane == kTopK) {
+      const float sg = a.d_gate && valid ? sigmoid(val) : 0.0f;
+      store_grad(out + E, sg * (1.0f - sg) * dg);
     }
-    if (a.shared && lane == 0) store_grad(out + E, d_shared);
   }
 }
+
+// ------------------------------------------------------------ host side
+
+// Up to this many rows one cluster makes the statistics in one launch.
+constexpr unsigned kRouteOneCluster = 1024;
 
 // CTAs that make statistics of `tokens` rows: one part of the sums each.
 inline unsigned route_parts(unsigned tokens) {
   const unsigned n = (tokens + kRouteWarps - 1) / kRouteWarps;
   return n < kRouteCtas ? n : kRouteCtas;
 }
+inline bool rows_aligned(const void* p, size_t stride, size_t size) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0;
+}
 
-template <typename L>
-inline void launch_route(const RouteParams& a, bool select, bool stats, cudaStream_t s) {
-  const unsigned full = (a.tokens + kRouteWarps - 1) / kRouteWarps, threads = 32 * kRouteWarps;
-  if (!stats) route_kernel<L, true, false><<<full, threads, 0, s>>>(a);
-  else if (select) route_kernel<L, true, true><<<route_parts(a.tokens), threads, 0, s>>>(a);
-  else route_kernel<L, false, true><<<route_parts(a.tokens), threads, 0, s>>>(a);
+// route_finish_kernel may start while route_kernel ends (it waits for it).
+inline cudaError_t launch_finish(const RouteFinish& f, cudaStream_t s) {
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(kRouteCluster);
+  cfg.blockDim = dim3(kFinishThreads);
+  cfg.stream = s;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, route_finish_kernel, f);
+}
+
+template <typename L, unsigned V, bool SELECT>
+inline cudaError_t launch_stats(const RouteParams& a, const RouteFinish& f, unsigned sms, cudaStream_t s) {
+  if (a.tokens <= kRouteOneCluster) {
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = kRouteCluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(kRouteCluster);
+    cfg.blockDim = dim3(32 * kRouteWarps);
+    cfg.stream = s;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, route_kernel<L, V, SELECT, kStatsCluster>, a, f);
+  }
+  route_kernel<L, V, SELECT, kStatsParts><<<f.parts, 32 * kRouteWarps, 0, s>>>(a, f);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? launch_finish(f, s) : e;
+}
+
+template <typename L, unsigned V>
+inline cudaError_t launch_route(const RouteParams& a, const RouteFinish& f, bool select, bool stats, unsigned sms,
+                                cudaStream_t s) {
+  if (stats) return select ? launch_stats<L, V, true>(a, f, sms, s) : launch_stats<L, V, false>(a, f, sms, s);
+  // few rows: four warps a CTA spread them over the SMs
+  const unsigned warps = a.tokens <= 8 * sms ? 4 : kRouteWarps, ctas = (a.tokens + warps - 1) / warps;
+  route_kernel<L, V, true, kStatsNone><<<warps == 4 || ctas < sms ? ctas : sms, 32 * warps, 0, s>>>(a, f);
+  return cudaGetLastError();
+}
+inline cudaError_t launch_route(const RouteParams& a, const RouteFinish& f, unsigned type, bool select, bool stats,
+                                unsigned sms, cudaStream_t s) {
+  const size_t size = type == FRC_BF16 ? 2 : 4;
+  // neighbours a lane only where they leave no lane without logits: the
+  // bound on the tenth largest needs the lanes' maxima
+  const bool vec = rows_aligned(a.logits, a.stride, size) && a.experts * size >= 512;
+  if (type == FRC_BF16)
+    return vec ? launch_route<__nv_bfloat16, 8>(a, f, select, stats, sms, s)
+               : launch_route<__nv_bfloat16, 1>(a, f, select, stats, sms, s);
+  return vec ? launch_route<float, 4>(a, f, select, stats, sms, s) : launch_route<float, 1>(a, f, select, stats, sms, s);
+}
+
+template <typename L, unsigned V>
+inline cudaError_t launch_backward(const RouteBackwardParams& a, unsigned sms, cudaStream_t s) {
+  const unsigned warps = a.tokens <= 8 * sms ? 4 : 8, ctas = (a.tokens + warps - 1) / warps, grid = ctas < 3 * sms ? ctas : 3 * sms;
+  if (a.count) route_backward_kernel<L, V, true><<<grid, 32 * warps, 0, s>>>(a);
+  else route_backward_kernel<L, V, false><<<grid, 32 * warps, 0, s>>>(a);
+  return cudaGetLastError();
+}
+inline cudaError_t launch_backward(const RouteBackwardParams& a, unsigned type, unsigned sms, cudaStream_t s) {
+  const size_t size = type == FRC_BF16 ? 2 : 4;
+  const bool vec = rows_aligned(a.logits, a.stride, size) && rows_aligned(a.d_logits, a.d_stride, size);
+  if (type == FRC_BF16)
+    return vec ? launch_backward<__nv_bfloat16, 8>(a, sms, s) : launch_backward<__nv_bfloat16, 1>(a, sms, s);
+  return vec ? launch_backward<float, 4>(a, sms, s) : launch_backward<float, 1>(a, sms, s);
 }
 
 }  // namespace frc
