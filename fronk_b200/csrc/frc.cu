@@ -1863,7 +1863,7 @@ int frc_matvec_device(frc_context* c, const frc_matrix* m, unsigned tokens, cons
 
 size_t frc_balance_workspace(unsigned tokens, unsigned experts) {
   if (frc_routing_check(tokens, experts, experts, FRC_F32, 0)) return 0;
-  const size_t parts = route_parts(tokens);
+  const size_t parts = route_parts(tokens, kRouteCtas);
   return parts * (experts * (sizeof(float) + sizeof(unsigned)) + sizeof(unsigned));
 }
 
@@ -1894,7 +1894,7 @@ static int route(frc_context* c, unsigned tokens, unsigned experts, const void* 
   a.logits = logits; a.stride = stride; a.valid = valid; a.expert_in = expert_in; a.expert = expert; a.gate = gate;
   a.tokens = tokens; a.experts = experts; a.shared = flags & FRC_ROUTE_SHARED;
   a.status = c->status;
-  const unsigned parts = route_parts(tokens);
+  const unsigned sms = static_cast<unsigned>(c->sms), parts = route_parts(tokens, sms < kRouteCtas ? sms : kRouteCtas);
   if (b) {
     a.psum = static_cast<float*>(b->workspace);
     a.pcount = reinterpret_cast<unsigned*>(a.psum + static_cast<size_t>(parts) * experts);
@@ -1902,7 +1902,7 @@ static int route(frc_context* c, unsigned tokens, unsigned experts, const void* 
   }
   RouteFinish f{};
   if (b) f = RouteFinish{a.psum, a.pcount, a.pvalid, parts, experts, b->loss, b->count, b->prob};
-  CK(launch_route(a, f, type, expert_in == nullptr, b != nullptr, static_cast<unsigned>(c->sms), s));
+  CK(launch_route(a, f, type, expert_in == nullptr, b != nullptr, sms, s));
   c->launches += b && tokens > kRouteOneCluster ? 2 : 1;
   return FRC_OK;
 }

@@ -20,7 +20,7 @@ constexpr unsigned kTopK = 10, kGates = 11, kMaxExperts = 512;
 constexpr unsigned kRouteSlots = kMaxExperts / 32;  // logits a lane holds
 constexpr unsigned kRouteWarps = 24;                // warps a CTA, at most
 constexpr unsigned kRouteSums = 8;                  // arrays of sums a CTA folds its warps into
-constexpr unsigned kRouteCtas = 160;                // CTAs that make statistics, at most
+constexpr unsigned kRouteCtas = 160;                // CTAs that make statistics (one an SM), at most
 constexpr unsigned kRouteCluster = 8;               // CTAs that finish them
 
 struct RouteParams {
@@ -580,9 +580,9 @@ __global__ void __launch_bounds__(256, 3) route_backward_kernel(const RouteBackw
 constexpr unsigned kRouteOneCluster = 1024;
 
 // CTAs that make statistics of `tokens` rows: one part of the sums each.
-inline unsigned route_parts(unsigned tokens) {
+inline unsigned route_parts(unsigned tokens, unsigned sms) {
   const unsigned n = (tokens + kRouteWarps - 1) / kRouteWarps;
-  return n < kRouteCtas ? n : kRouteCtas;
+  return n < sms ? n : sms;
 }
 inline bool rows_aligned(const void* p, size_t stride, size_t size) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0;
