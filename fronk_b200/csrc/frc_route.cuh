@@ -105,6 +105,32 @@ __device__ __forceinline__ float exp_below(float v, float m) {
   return d;
 }
 
+// Two fp32 operations an instruction: a row's arithmetic is 16 values a lane.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 pack2(float a, float b) {
+  F2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d.v) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void unpack2(F2 d, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d.v)); }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+
 // A row's E logits over a warp, kRouteSlots a lane: V neighbours a load (V = 1
 // where rows are not 16-byte aligned), slot i of a lane being column
 // col<V>(i, lane); columns past E are -inf.
@@ -152,15 +178,35 @@ struct RowLoad {
   }
 };
 
+// e = exp(v - m) of a lane's slots, in pairs; returns their sum.
+__device__ __forceinline__ float exp_row(const float (&v)[kRouteSlots], float m, F2 (&e)[kRouteSlots / 2]) {
+  const F2 shift = pack2(-m, -m), log2e = pack2(1.4426950408889634f, 1.4426950408889634f);
+  F2 z = pack2(0.0f, 0.0f);
+#pragma unroll
+  for (unsigned i = 0; i < kRouteSlots / 2; ++i) {
+    float x, y;
+    unpack2(mul2(add2(pack2(v[2 * i], v[2 * i + 1]), shift), log2e), x, y);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(y));
+    e[i] = pack2(x, y);
+    z = add2(z, e[i]);
+  }
+  float x, y;
+  unpack2(z, x, y);
+  return x + y;
+}
+
 // The ten largest of a row in order, ties by the lower column: lane r < 10
 // gets the r-th one's column and value.
 //
 // The tenth largest of the lanes' maxima bounds the tenth largest logit from
 // below, so only the logits at or above it (a dozen as a rule) are collected
-// and ranked against one another.  Where ties make them more than 32, ten
-// searches over the whole row choose one by one.
+// (each lane behind the lanes before it) and ranked against one another by
+// {order of the value, lower column first} as one integer.  Where they are
+// more than 32 (ties) or the bound is -inf (few logits left), ten searches
+// over the whole row choose one by one.
 template <unsigned V>
-__device__ __forceinline__ void choose(const float (&v)[kRouteSlots], unsigned E, unsigned lane, float top, float2* cand,
+__device__ __forceinline__ void choose(const float (&v)[kRouteSlots], unsigned E, unsigned lane, float top, uint64_t* cand,
                                        unsigned* id, float* val) {
   float rest = top, bound = 0.0f;
 #pragma unroll
@@ -168,34 +214,49 @@ __device__ __forceinline__ void choose(const float (&v)[kRouteSlots], unsigned E
     bound = warp_max(rest);
     rest = rest == bound ? -INFINITY : rest;
   }
-  unsigned total = 0;
+  unsigned total = 64;
+  if (bound > -INFINITY) {
+    unsigned n = 0;
 #pragma unroll
-  for (unsigned i = 0; i < kRouteSlots; ++i) {
-    const unsigned c = col<V>(i, lane);
-    const bool in = v[i] >= bound && c < E;
-    const unsigned m = __ballot_sync(0xffffffffu, in);
-    if (in) {
-      const unsigned at = total + __popc(m & ((1u << lane) - 1u));
-      if (at < 32) cand[at] = make_float2(v[i], __uint_as_float(c));
+    for (unsigned i = 0; i < kRouteSlots; ++i) n += v[i] >= bound ? 1u : 0u;
+    unsigned end = n;
+#pragma unroll
+    for (unsigned o = 1; o < 32; o <<= 1) {
+      const unsigned u = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end += u;
     }
-    total += __popc(m);
+    total = __shfl_sync(0xffffffffu, end, 31);
+    if (total <= 32) {
+      uint64_t* p = cand + (end - n);
+#pragma unroll
+      for (unsigned i = 0; i < kRouteSlots; ++i)
+        if (v[i] >= bound) *p++ = static_cast<uint64_t>(__float_as_uint(v[i])) << 32 | col<V>(i, lane);
+      __syncwarp();
+      uint64_t key = 0;
+      if (lane < total) {
+        const uint64_t c = cand[lane];
+        key = static_cast<uint64_t>(order_key(__uint_as_float(static_cast<unsigned>(c >> 32)) + 0.0f)) << 32 | (~static_cast<unsigned>(c));
+      }
+      __syncwarp();
+      cand[lane] = key;
+      __syncwarp();
+      unsigned rank = 0;
+      for (unsigned k = 0; k < total; k += 4) {
+        const ulonglong2 a = reinterpret_cast<const ulonglong2*>(cand)[k / 2], b = reinterpret_cast<const ulonglong2*>(cand)[k / 2 + 1];
+        rank += a.x > key ? 1u : 0u;
+        rank += a.y > key ? 1u : 0u;
+        rank += b.x > key ? 1u : 0u;
+        rank += b.y > key ? 1u : 0u;
+      }
+      __syncwarp();
+      if (lane < total) cand[rank] = key;  // ranks are distinct
+      __syncwarp();
+      const uint64_t r = cand[lane < total ? lane : 0];
+      *id = ~static_cast<unsigned>(r);
+      *val = key_value(static_cast<unsigned>(r >> 32));
+    }
   }
-  __syncwarp();
-  if (total <= 32) {
-    const float2 mine = lane < total ? cand[lane] : make_float2(-INFINITY, 0.0f);
-    const unsigned c = __float_as_uint(mine.y);
-    unsigned rank = 0;
-    for (unsigned k = 0; k < total; ++k) {
-      const float2 o = cand[k];
-      rank += o.x > mine.x || (o.x == mine.x && __float_as_uint(o.y) < c);
-    }
-    __syncwarp();
-    if (lane < total) cand[rank] = mine;  // ranks are distinct
-    __syncwarp();
-    const float2 r = cand[lane < total ? lane : 0];
-    *id = __float_as_uint(r.y);
-    *val = r.x;
-  } else {
+  if (total > 32) {
     unsigned left = 0;
 #pragma unroll
     for (unsigned i = 0; i < kRouteSlots; ++i) left |= (col<V>(i, lane) < E ? 1u : 0u) << i;
@@ -284,13 +345,15 @@ template <typename L, unsigned V, bool SELECT, int STATS>
 __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteParams a, const RouteFinish f) {
   __shared__ float s_psum[STATS ? kRouteSums : 1][STATS ? kMaxExperts : 1];
   __shared__ unsigned s_count[STATS ? kMaxExperts : 1], s_valid;
-  __shared__ float2 s_cand[SELECT ? kRouteWarps : 1][32];
+  __shared__ __align__(16) uint64_t s_cand[SELECT ? kRouteWarps : 1][32];
   __shared__ double s_term[STATS == kStatsCluster ? kRouteWarps : 1], s_loss;
   const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = blockDim.x / 32, E = a.experts;
   const L* logits = static_cast<const L*>(a.logits);
-  float psum[STATS ? kRouteSlots : 1] = {};
+  F2 psum[STATS ? kRouteSlots / 2 : 1];
   unsigned nvalid = 0;
   if (STATS) {
+#pragma unroll
+    for (unsigned i = 0; i < kRouteSlots / 2; ++i) psum[i] = pack2(0.0f, 0.0f);
     for (unsigned e = threadIdx.x; e < E; e += blockDim.x) s_count[e] = 0;
     if (threadIdx.x == 0) s_valid = 0;
     __syncthreads();
@@ -352,15 +415,11 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteP
       }
       ++nvalid;
       if (m > -INFINITY) {
-        float z = 0.0f;
+        F2 e[kRouteSlots / 2];
+        const float zi = __frcp_rn(warp_sum(exp_row(v, m, e)));
+        const F2 z2 = pack2(zi, zi);
 #pragma unroll
-        for (unsigned i = 0; i < kRouteSlots; ++i) {
-          v[i] = exp_below(v[i], m);
-          z += v[i];
-        }
-        z = 1.0f / warp_sum(z);
-#pragma unroll
-        for (unsigned i = 0; i < kRouteSlots; ++i) psum[i] = fmaf(v[i], z, psum[i]);
+        for (unsigned i = 0; i < kRouteSlots / 2; ++i) psum[i] = fma2(e[i], z2, psum[i]);
       }
     }
   }
@@ -371,8 +430,10 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteP
       if (warp >= w && warp < w + kRouteSums)
 #pragma unroll
         for (unsigned i = 0; i < kRouteSlots; ++i) {
+          float x, y;
+          unpack2(psum[i / 2], x, y);
           float* p = &s_psum[warp - w][col<V>(i, lane)];
-          *p = (w ? *p : 0.0f) + psum[i];
+          *p = (w ? *p : 0.0f) + (i & 1 ? y : x);
         }
       __syncthreads();
     }
@@ -484,15 +545,19 @@ __device__ __forceinline__ void store_row(L* row, unsigned E, unsigned lane, con
 // the chosen logits are read.
 template <typename L, unsigned V, bool BALANCE>
 __global__ void __launch_bounds__(256, 3) route_backward_kernel(const RouteBackwardParams a) {
-  __shared__ float s_count[BALANCE ? kMaxExperts : 1];
   const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = blockDim.x / 32, E = a.experts;
   const L* logits = static_cast<const L*>(a.logits);
+  // the balance term as p_e (k_e - sum p k), k = scale count
   float scale = 0.0f;
+  F2 k2[BALANCE ? kRouteSlots / 2 : 1];
   if (BALANCE) {
-    for (unsigned e = threadIdx.x; e < kMaxExperts; e += blockDim.x) s_count[e] = e < E ? static_cast<float>(a.count[e]) : 0.0f;
     const float n = static_cast<float>(a.count[E]);
     scale = n > 0.0f ? *a.d_loss * static_cast<float>(E) / (static_cast<float>(kTopK) * n * n) : 0.0f;
-    __syncthreads();
+#pragma unroll
+    for (unsigned i = 0; i < kRouteSlots / 2; ++i) {
+      const unsigned c = col<V>(2 * i, lane), d = col<V>(2 * i + 1, lane);
+      k2[i] = pack2(c < E ? scale * static_cast<float>(a.count[c]) : 0.0f, d < E ? scale * static_cast<float>(a.count[d]) : 0.0f);
+    }
   }
   const unsigned step = gridDim.x * warps;
   unsigned t = blockIdx.x * warps + warp;
@@ -527,18 +592,18 @@ __global__ void __launch_bounds__(256, 3) route_backward_kernel(const RouteBackw
       m = warp_max_nan(m);
       if (valid && !(m < INFINITY) && lane == 0) atomicOr(a.status, kStNumeric);
       if (valid && m > -INFINITY) {
-        float z = 0.0f;
+        F2 e[kRouteSlots / 2], s2 = pack2(0.0f, 0.0f);
+        const float z = exp_row(d, m, e);
 #pragma unroll
-        for (unsigned i = 0; i < kRouteSlots; ++i) {
-          d[i] = exp_below(d[i], m);
-          z += d[i];
-          dot = fmaf(d[i], s_count[col<V>(i, lane)], dot);
-        }
-        zi = 1.0f / warp_sum(z);
+        for (unsigned i = 0; i < kRouteSlots / 2; ++i) s2 = fma2(e[i], k2[i], s2);
+        unpack2(s2, dot, zi);
+        dot += zi;
+        zi = __frcp_rn(warp_sum(z));
         dot = warp_sum(dot) * zi;
-        const float k = scale * zi;
+        // (e / z) (k - dot) = e (k / z - dot / z)
+        const F2 z2 = pack2(zi, zi), c2 = pack2(-dot * zi, -dot * zi);
 #pragma unroll
-        for (unsigned i = 0; i < kRouteSlots; ++i) d[i] = (k * d[i]) * (s_count[col<V>(i, lane)] - dot);
+        for (unsigned i = 0; i < kRouteSlots / 2; ++i) unpack2(mul2(e[i], fma2(k2[i], z2, c2)), d[2 * i], d[2 * i + 1]);
       } else {
 #pragma unroll
         for (unsigned i = 0; i < kRouteSlots; ++i) d[i] = 0.0f;
@@ -563,7 +628,7 @@ __global__ void __launch_bounds__(256, 3) route_backward_kernel(const RouteBackw
           if (twice && (same >> r & 1u)) term += o;
         }
       }
-      if (BALANCE && lane < kTopK && zi > 0.0f && id < E) term += (scale * zi * exp_below(val, m)) * (s_count[id] - dot);
+      if (BALANCE && lane < kTopK && zi > 0.0f && id < E) term += exp_below(val, m) * fmaf(scale * static_cast<float>(a.count[id]), zi, -dot * zi);
       __syncwarp();  // behind the row's stores
       if (valid && lane < kTopK && id < E) store_grad(out + id, term);
     }
