@@ -1864,7 +1864,7 @@ int frc_matvec_device(frc_context* c, const frc_matrix* m, unsigned tokens, cons
 size_t frc_balance_workspace(unsigned tokens, unsigned experts) {
   if (frc_routing_check(tokens, experts, experts, FRC_F32, 0)) return 0;
   const size_t parts = route_parts(tokens, kRouteCtas);
-  return parts * (experts * (sizeof(float) + sizeof(unsigned)) + sizeof(unsigned));
+  return parts * (experts * sizeof(float2) + sizeof(unsigned));
 }
 
 static int check_balance(frc_context* c, const frc_balance* b, unsigned tokens, unsigned experts) {
@@ -1896,12 +1896,11 @@ static int route(frc_context* c, unsigned tokens, unsigned experts, const void* 
   a.status = c->status;
   const unsigned sms = static_cast<unsigned>(c->sms), parts = route_parts(tokens, sms < kRouteCtas ? sms : kRouteCtas);
   if (b) {
-    a.psum = static_cast<float*>(b->workspace);
-    a.pcount = reinterpret_cast<unsigned*>(a.psum + static_cast<size_t>(parts) * experts);
-    a.pvalid = a.pcount + static_cast<size_t>(parts) * experts;
+    a.part = static_cast<float2*>(b->workspace);
+    a.pvalid = reinterpret_cast<unsigned*>(a.part + static_cast<size_t>(parts) * experts);
   }
   RouteFinish f{};
-  if (b) f = RouteFinish{a.psum, a.pcount, a.pvalid, parts, experts, b->loss, b->count, b->prob};
+  if (b) f = RouteFinish{a.part, a.pvalid, parts, experts, b->loss, b->count, b->prob};
   CK(launch_route(a, f, type, expert_in == nullptr, b != nullptr, sms, s));
   c->launches += b && tokens > kRouteOneCluster ? 2 : 1;
   return FRC_OK;

@@ -31,16 +31,14 @@ struct RouteParams {
   uint16_t* expert;
   float* gate;
   unsigned tokens, experts, shared;
-  // statistics: [CTA][E] sums of p, [CTA][E] counts, [CTA] valid rows
-  float* psum;
-  unsigned* pcount;
+  // statistics: [CTA][E] {sum of p, count}, [CTA] valid rows
+  float2* part;
   unsigned* pvalid;
   unsigned* status;
 };
 
 struct RouteFinish {
-  const float* psum;
-  const unsigned* pcount;
+  const float2* part;
   const unsigned* pvalid;
   unsigned parts, experts;
   float* loss;
@@ -103,6 +101,18 @@ __device__ __forceinline__ float exp_below(float v, float m) {
   float d;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"((v - m) * 1.4426950408889634f));
   return d;
+}
+
+// The largest of a lane's slots (NaN when one is), as a tree.
+__device__ __forceinline__ float row_max(const float (&v)[kRouteSlots]) {
+  float m[kRouteSlots / 2];
+#pragma unroll
+  for (unsigned i = 0; i < kRouteSlots / 2; ++i) m[i] = max_nan(v[2 * i], v[2 * i + 1]);
+#pragma unroll
+  for (unsigned k = kRouteSlots / 4; k; k /= 2)
+#pragma unroll
+    for (unsigned i = 0; i < k; ++i) m[i] = max_nan(m[i], m[i + k]);
+  return m[0];
 }
 
 // Two fp32 operations an instruction: a row's arithmetic is 16 values a lane.
@@ -181,7 +191,7 @@ struct RowLoad {
 // e = exp(v - m) of a lane's slots, in pairs; returns their sum.
 __device__ __forceinline__ float exp_row(const float (&v)[kRouteSlots], float m, F2 (&e)[kRouteSlots / 2]) {
   const F2 shift = pack2(-m, -m), log2e = pack2(1.4426950408889634f, 1.4426950408889634f);
-  F2 z = pack2(0.0f, 0.0f);
+  F2 z = pack2(0.0f, 0.0f), z1 = z;
 #pragma unroll
   for (unsigned i = 0; i < kRouteSlots / 2; ++i) {
     float x, y;
@@ -189,10 +199,11 @@ __device__ __forceinline__ float exp_row(const float (&v)[kRouteSlots], float m,
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(y));
     e[i] = pack2(x, y);
-    z = add2(z, e[i]);
+    if (i & 1) z1 = add2(z1, e[i]);
+    else z = add2(z, e[i]);
   }
   float x, y;
-  unpack2(z, x, y);
+  unpack2(add2(z, z1), x, y);
   return x + y;
 }
 
@@ -362,10 +373,13 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteP
   unsigned t = blockIdx.x * warps + warp;
   RowLoad<L, V> next;
   bool next_valid = false;
-  if (t < a.tokens) {
-    next_valid = !a.valid || a.valid[t];
-    next.load(logits + t * a.stride, E, lane);
-  }
+  unsigned next_id = 0;
+  const auto fetch = [&](unsigned r) {
+    next_valid = !a.valid || a.valid[r];
+    if (STATS && !SELECT && lane < kTopK) next_id = a.expert_in[static_cast<size_t>(r) * kTopK + lane];
+    next.load(logits + r * a.stride, E, lane);
+  };
+  if (t < a.tokens) fetch(t);
   for (; t < a.tokens; t += step) {
     const L* row = logits + t * a.stride;
     const bool valid = next_valid;
@@ -374,15 +388,12 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteP
     for (unsigned i = 0; i < kRouteSlots; ++i) v[i] = next.value(i);
     unsigned id = lane;
     float val = -INFINITY;
-    if (STATS && !SELECT && lane < kTopK) id = a.expert_in[static_cast<size_t>(t) * kTopK + lane];
-    if (t + step < a.tokens) {
-      next_valid = !a.valid || a.valid[t + step];
-      next.load(row + step * a.stride, E, lane);
+    if (STATS && !SELECT && lane < kTopK) {
+      id = next_id;
+      if (id < E && valid) val = logit(row + id);
     }
-    float top = v[0];
-#pragma unroll
-    for (unsigned i = 1; i < kRouteSlots; ++i) top = max_nan(top, v[i]);
-    const float m = warp_max_nan(top);
+    if (t + step < a.tokens) fetch(t + step);
+    const float top = row_max(v), m = warp_max_nan(top);
     const bool bad = valid && !(m < INFINITY);
     if (bad && lane == 0) atomicOr(a.status, kStNumeric);
     const bool use = valid && !bad;
@@ -407,10 +418,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteP
     }
     if (STATS && use) {
       if (lane < kTopK) {
-        if (!SELECT) {
-          if (id < E) val = logit(row + id);
-          else atomicOr(a.status, kStInvalid);
-        }
+        if (!SELECT && id >= E) atomicOr(a.status, kStInvalid);
         if (val > -INFINITY) atomicAdd(&s_count[id], 1u);
       }
       ++nvalid;
@@ -442,8 +450,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteP
       for (unsigned e = threadIdx.x; e < E; e += blockDim.x) {
         float s = 0.0f;
         for (unsigned w = 0; w < sums; ++w) s += s_psum[w][e];
-        a.psum[static_cast<size_t>(blockIdx.x) * E + e] = s;
-        a.pcount[static_cast<size_t>(blockIdx.x) * E + e] = s_count[e];
+        a.part[static_cast<size_t>(blockIdx.x) * E + e] = make_float2(s, __uint_as_float(s_count[e]));
       }
       if (threadIdx.x == 0) a.pvalid[blockIdx.x] = s_valid;
     } else {
@@ -472,22 +479,28 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteP
 }
 
 // Sums the CTAs' parts in order, in double, and forms the loss: one cluster,
-// eight threads an expert that take every eighth part.
-constexpr unsigned kFinishThreads = kMaxExperts / kRouteCluster * 8;
+// 16 threads an expert that take every 16th part, all of them in flight.
+constexpr unsigned kFinishSplit = 16, kFinishThreads = kMaxExperts / kRouteCluster * kFinishSplit;
 __global__ void __cluster_dims__(kRouteCluster, 1, 1) __launch_bounds__(kFinishThreads)
     route_finish_kernel(const RouteFinish f) {
-  __shared__ double s_p[8][kMaxExperts / kRouteCluster], s_term[kFinishThreads / 32], s_loss;
-  __shared__ unsigned s_c[8][kMaxExperts / kRouteCluster];
+  __shared__ double s_p[kFinishSplit][kMaxExperts / kRouteCluster], s_term[kFinishThreads / 32], s_loss;
+  __shared__ unsigned s_c[kFinishSplit][kMaxExperts / kRouteCluster];
   const unsigned own = kMaxExperts / kRouteCluster, i = threadIdx.x % own, k0 = threadIdx.x / own;
   const unsigned e = cluster_rank() * own + i;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   double p = 0.0;
   unsigned c = 0;
   if (e < f.experts) {
-#pragma unroll 8
-    for (unsigned k = k0; k < f.parts; k += 8) {
-      p += f.psum[static_cast<size_t>(k) * f.experts + e];
-      c += f.pcount[static_cast<size_t>(k) * f.experts + e];
+    float2 v[kRouteCtas / kFinishSplit];
+#pragma unroll
+    for (unsigned j = 0; j < kRouteCtas / kFinishSplit; ++j) {
+      const unsigned k = k0 + kFinishSplit * j;
+      v[j] = k < f.parts ? f.part[static_cast<size_t>(k) * f.experts + e] : make_float2(0.0f, 0.0f);
+    }
+#pragma unroll
+    for (unsigned j = 0; j < kRouteCtas / kFinishSplit; ++j) {
+      p += v[j].x;
+      c += __float_as_uint(v[j].y);
     }
   }
   unsigned n = 0;
@@ -498,7 +511,7 @@ __global__ void __cluster_dims__(kRouteCluster, 1, 1) __launch_bounds__(kFinishT
   __syncthreads();
   double term = 0.0;
   if (k0 == 0 && e < f.experts) {
-    for (unsigned k = 1; k < 8; ++k) {
+    for (unsigned k = 1; k < kFinishSplit; ++k) {
       p += s_p[k][i];
       c += s_c[k][i];
     }
@@ -562,34 +575,38 @@ __global__ void __launch_bounds__(256, 3) route_backward_kernel(const RouteBackw
   const unsigned step = gridDim.x * warps;
   unsigned t = blockIdx.x * warps + warp;
   RowLoad<L, V> next;
-  if (BALANCE && t < a.tokens) next.load(logits + t * a.stride, E, lane);
+  bool next_valid = false;
+  unsigned next_id = E + 1;
+  float next_dg = 0.0f;
+  const auto fetch = [&](unsigned r) {
+    next_valid = !a.valid || a.valid[r];
+    if (a.d_gate) {
+      if (lane < kTopK) next_id = a.expert[static_cast<size_t>(r) * kTopK + lane];
+      if (lane < kGates) next_dg = a.d_gate[static_cast<size_t>(r) * kGates + lane];
+    }
+    if (BALANCE) next.load(logits + r * a.stride, E, lane);
+  };
+  if (t < a.tokens) fetch(t);
   for (; t < a.tokens; t += step) {
     const L* row = logits + t * a.stride;
     L* out = static_cast<L*>(a.d_logits) + t * a.d_stride;
-    const bool valid = !a.valid || a.valid[t];
+    const bool valid = next_valid;
     float d[kRouteSlots];
     // the chosen experts of lanes 0-9, the shared logit in lane 10
-    unsigned id = E + 1;
-    float val = -INFINITY, dg = 0.0f;
-    if (a.d_gate && valid) {
-      if (lane < kTopK) id = a.expert[static_cast<size_t>(t) * kTopK + lane];
-      if (lane < kGates) dg = a.d_gate[static_cast<size_t>(t) * kGates + lane];
-      if (lane == kTopK && a.shared) val = logit(row + E);
-    }
+    const unsigned id = next_id;
+    const float dg = next_dg;
+    float val = -INFINITY;
+    if (a.d_gate && valid && (lane < kTopK ? id < E : lane == kTopK && a.shared)) val = logit(row + (lane < kTopK ? id : E));
 #pragma unroll
     for (unsigned i = 0; i < kRouteSlots; ++i) d[i] = BALANCE ? next.value(i) : 0.0f;
-    if (BALANCE && t + step < a.tokens) next.load(row + step * a.stride, E, lane);
+    if (t + step < a.tokens) fetch(t + step);
     if (lane < kTopK && a.d_gate && valid) {
-      if (id < E) val = logit(row + id);
-      else atomicOr(a.status, kStInvalid);
+      if (id >= E) atomicOr(a.status, kStInvalid);
       if (!(val < INFINITY)) atomicOr(a.status, kStNumeric);
     }
     float m = -INFINITY, zi = 0.0f, dot = 0.0f;
     if (BALANCE) {
-      m = d[0];
-#pragma unroll
-      for (unsigned i = 1; i < kRouteSlots; ++i) m = max_nan(m, d[i]);
-      m = warp_max_nan(m);
+      m = warp_max_nan(row_max(d));
       if (valid && !(m < INFINITY) && lane == 0) atomicOr(a.status, kStNumeric);
       if (valid && m > -INFINITY) {
         F2 e[kRouteSlots / 2], s2 = pack2(0.0f, 0.0f);
