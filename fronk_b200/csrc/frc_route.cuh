@@ -95,6 +95,11 @@ __device__ __forceinline__ float warp_max(float v) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
   return d;
 }
+__device__ __forceinline__ float rcp(float v) {  // within one step; v is a sum of exponentials, at least 1
+  float d;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(v));
+  return d;
+}
 __device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + expf(-v)); }
 // exp(v - m) with v <= m, m finite; v may be -inf.
 __device__ __forceinline__ float exp_below(float v, float m) {
@@ -148,7 +153,8 @@ template <unsigned V>
 __device__ __forceinline__ unsigned col(unsigned i, unsigned lane) {
   return i / V * (32 * V) + V * lane + i % V;
 }
-template <typename L, unsigned V>
+// FULL: E is kMaxExperts (the framework's expert count), no slot is past it.
+template <typename L, unsigned V, bool FULL>
 struct RowLoad {
   static constexpr unsigned kWords = V == 1 ? kRouteSlots : kRouteSlots * sizeof(L) / 4;
   uint32_t w[kWords];  // fp32 bits, or pairs of bf16, or (V = 1) a value each
@@ -156,13 +162,16 @@ struct RowLoad {
   __device__ __forceinline__ void load(const L* row, unsigned E, unsigned lane) {
     if constexpr (V == 1) {
 #pragma unroll
-      for (unsigned i = 0; i < kRouteSlots; ++i) w[i] = __float_as_uint(lane + 32 * i < E ? logit(row + lane + 32 * i) : -INFINITY);
+      for (unsigned i = 0; i < kRouteSlots; ++i) {
+        if (FULL || 32 * i + 32 <= E) w[i] = __float_as_uint(logit(row + lane + 32 * i));
+        else w[i] = __float_as_uint(lane + 32 * i < E ? logit(row + lane + 32 * i) : -INFINITY);
+      }
     } else {
 #pragma unroll
       for (unsigned j = 0; j < kRouteSlots / V; ++j) {
         const unsigned c = col<V>(j * V, lane);
         uint4 v;
-        if (c + V <= E) {
+        if (FULL || c + V <= E) {
           v = *reinterpret_cast<const uint4*>(row + c);
         } else if constexpr (sizeof(L) == 4) {
           uint32_t e[4];
@@ -352,7 +361,7 @@ enum : int { kStatsNone = 0, kStatsParts = 1, kStatsCluster = 2 };
 // One warp a row; SELECT: choose experts and gates; STATS: sums of p and
 // counts of the chosen (or given) experts over the CTA's rows.  The next
 // row's logits are on their way while one is worked on.
-template <typename L, unsigned V, bool SELECT, int STATS>
+template <typename L, unsigned V, bool FULL, bool SELECT, int STATS>
 __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteParams a, const RouteFinish f) {
   __shared__ float s_psum[STATS ? kRouteSums : 1][STATS ? kMaxExperts : 1];
   __shared__ unsigned s_count[STATS ? kMaxExperts : 1], s_valid;
@@ -371,7 +380,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteP
   }
   const unsigned step = gridDim.x * warps;
   unsigned t = blockIdx.x * warps + warp;
-  RowLoad<L, V> next;
+  RowLoad<L, V, FULL> next;
   bool next_valid = false;
   unsigned next_id = 0;
   const auto fetch = [&](unsigned r) {
@@ -424,7 +433,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteP
       ++nvalid;
       if (m > -INFINITY) {
         F2 e[kRouteSlots / 2];
-        const float zi = __frcp_rn(warp_sum(exp_row(v, m, e)));
+        const float zi = rcp(warp_sum(exp_row(v, m, e)));
         const F2 z2 = pack2(zi, zi);
 #pragma unroll
         for (unsigned i = 0; i < kRouteSlots / 2; ++i) psum[i] = fma2(e[i], z2, psum[i]);
@@ -522,17 +531,17 @@ __global__ void __cluster_dims__(kRouteCluster, 1, 1) __launch_bounds__(kFinishT
 
 __device__ __forceinline__ void store_grad(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_grad(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-template <typename L, unsigned V>
+template <typename L, unsigned V, bool FULL>
 __device__ __forceinline__ void store_row(L* row, unsigned E, unsigned lane, const float (&d)[kRouteSlots]) {
   if constexpr (V == 1) {
 #pragma unroll
     for (unsigned i = 0; i < kRouteSlots; ++i)
-      if (lane + 32 * i < E) store_grad(row + lane + 32 * i, d[i]);
+      if (FULL || 32 * i + 32 <= E || lane + 32 * i < E) store_grad(row + lane + 32 * i, d[i]);
   } else {
 #pragma unroll
     for (unsigned j = 0; j < kRouteSlots / V; ++j) {
       const unsigned c = col<V>(j * V, lane);
-      if (c + V <= E) {
+      if (FULL || c + V <= E) {
         if constexpr (sizeof(L) == 4) {
           *reinterpret_cast<float4*>(row + c) = make_float4(d[4 * j], d[4 * j + 1], d[4 * j + 2], d[4 * j + 3]);
         } else {
@@ -556,25 +565,13 @@ __device__ __forceinline__ void store_row(L* row, unsigned E, unsigned lane, con
 // One warp a row: the balance term of every logit is stored first, then lanes
 // 0-9 store the chosen ones' sum with the routing term.  BALANCE off: only
 // the chosen logits are read.
-template <typename L, unsigned V, bool BALANCE>
+template <typename L, unsigned V, bool FULL, bool BALANCE>
 __global__ void __launch_bounds__(256, 3) route_backward_kernel(const RouteBackwardParams a) {
   const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = blockDim.x / 32, E = a.experts;
   const L* logits = static_cast<const L*>(a.logits);
-  // the balance term as p_e (k_e - sum p k), k = scale count
-  float scale = 0.0f;
-  F2 k2[BALANCE ? kRouteSlots / 2 : 1];
-  if (BALANCE) {
-    const float n = static_cast<float>(a.count[E]);
-    scale = n > 0.0f ? *a.d_loss * static_cast<float>(E) / (static_cast<float>(kTopK) * n * n) : 0.0f;
-#pragma unroll
-    for (unsigned i = 0; i < kRouteSlots / 2; ++i) {
-      const unsigned c = col<V>(2 * i, lane), d = col<V>(2 * i + 1, lane);
-      k2[i] = pack2(c < E ? scale * static_cast<float>(a.count[c]) : 0.0f, d < E ? scale * static_cast<float>(a.count[d]) : 0.0f);
-    }
-  }
   const unsigned step = gridDim.x * warps;
   unsigned t = blockIdx.x * warps + warp;
-  RowLoad<L, V> next;
+  RowLoad<L, V, FULL> next;
   bool next_valid = false;
   unsigned next_id = E + 1;
   float next_dg = 0.0f;
@@ -587,6 +584,18 @@ __global__ void __launch_bounds__(256, 3) route_backward_kernel(const RouteBackw
     if (BALANCE) next.load(logits + r * a.stride, E, lane);
   };
   if (t < a.tokens) fetch(t);
+  // the balance term as p_e (k_e - sum p k), k = scale count
+  float scale = 0.0f;
+  F2 k2[BALANCE ? kRouteSlots / 2 : 1];
+  if (BALANCE) {
+    const float n = static_cast<float>(a.count[E]);
+    scale = n > 0.0f ? *a.d_loss * static_cast<float>(E) / (static_cast<float>(kTopK) * n * n) : 0.0f;
+#pragma unroll
+    for (unsigned i = 0; i < kRouteSlots / 2; ++i) {
+      const unsigned c = col<V>(2 * i, lane), d = col<V>(2 * i + 1, lane);
+      k2[i] = pack2(c < E ? scale * static_cast<float>(a.count[c]) : 0.0f, d < E ? scale * static_cast<float>(a.count[d]) : 0.0f);
+    }
+  }
   for (; t < a.tokens; t += step) {
     const L* row = logits + t * a.stride;
     L* out = static_cast<L*>(a.d_logits) + t * a.d_stride;
@@ -615,7 +624,7 @@ __global__ void __launch_bounds__(256, 3) route_backward_kernel(const RouteBackw
         for (unsigned i = 0; i < kRouteSlots / 2; ++i) s2 = fma2(e[i], k2[i], s2);
         unpack2(s2, dot, zi);
         dot += zi;
-        zi = __frcp_rn(warp_sum(z));
+        zi = rcp(warp_sum(z));
         dot = warp_sum(dot) * zi;
         // (e / z) (k - dot) = e (k / z - dot / z)
         const F2 z2 = pack2(zi, zi), c2 = pack2(-dot * zi, -dot * zi);
@@ -627,12 +636,12 @@ __global__ void __launch_bounds__(256, 3) route_backward_kernel(const RouteBackw
       }
     }
     __syncwarp();  // d_logits may be logits: every lane has read the row
-    store_row<L, V>(out, E, lane, d);
+    store_row<L, V, FULL>(out, E, lane, d);
     if (a.d_gate) {
       const float chosen = lane < kTopK ? val : -INFINITY, mk = warp_max(chosen);
-      float g = lane < kTopK && mk > -INFINITY ? expf(val - mk) : 0.0f;
+      float g = mk > -INFINITY ? exp2f((chosen - mk) * 1.4426950408889634f) : 0.0f;  // subnormal gates count
       const float s = warp_sum(g);
-      g = s > 0.0f ? g / s : 0.0f;
+      g = s > 0.0f ? g * rcp(s) : 0.0f;
       const float gd = warp_sum(g * dg);
       const float own = g * (dg - gd);
       float term = own;
@@ -684,7 +693,7 @@ inline cudaError_t launch_finish(const RouteFinish& f, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, route_finish_kernel, f);
 }
 
-template <typename L, unsigned V, bool SELECT>
+template <typename L, unsigned V, bool FULL, bool SELECT>
 inline cudaError_t launch_stats(const RouteParams& a, const RouteFinish& f, unsigned sms, cudaStream_t s) {
   if (a.tokens <= kRouteOneCluster) {
     cudaLaunchAttribute at{};
@@ -697,20 +706,20 @@ inline cudaError_t launch_stats(const RouteParams& a, const RouteFinish& f, unsi
     cfg.stream = s;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, route_kernel<L, V, SELECT, kStatsCluster>, a, f);
+    return cudaLaunchKernelEx(&cfg, route_kernel<L, V, FULL, SELECT, kStatsCluster>, a, f);
   }
-  route_kernel<L, V, SELECT, kStatsParts><<<f.parts, 32 * kRouteWarps, 0, s>>>(a, f);
+  route_kernel<L, V, FULL, SELECT, kStatsParts><<<f.parts, 32 * kRouteWarps, 0, s>>>(a, f);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? launch_finish(f, s) : e;
 }
 
-template <typename L, unsigned V>
+template <typename L, unsigned V, bool FULL>
 inline cudaError_t launch_route(const RouteParams& a, const RouteFinish& f, bool select, bool stats, unsigned sms,
                                 cudaStream_t s) {
-  if (stats) return select ? launch_stats<L, V, true>(a, f, sms, s) : launch_stats<L, V, false>(a, f, sms, s);
+  if (stats) return select ? launch_stats<L, V, FULL, true>(a, f, sms, s) : launch_stats<L, V, FULL, false>(a, f, sms, s);
   // few rows: four warps a CTA spread them over the SMs
   const unsigned warps = a.tokens <= 8 * sms ? 4 : kRouteWarps, ctas = (a.tokens + warps - 1) / warps;
-  route_kernel<L, V, true, kStatsNone><<<warps == 4 || ctas < sms ? ctas : sms, 32 * warps, 0, s>>>(a, f);
+  route_kernel<L, V, FULL, true, kStatsNone><<<warps == 4 || ctas < sms ? ctas : sms, 32 * warps, 0, s>>>(a, f);
   return cudaGetLastError();
 }
 inline cudaError_t launch_route(const RouteParams& a, const RouteFinish& f, unsigned type, bool select, bool stats,
@@ -719,25 +728,32 @@ inline cudaError_t launch_route(const RouteParams& a, const RouteFinish& f, unsi
   // neighbours a lane only where they leave no lane without logits: the
   // bound on the tenth largest needs the lanes' maxima
   const bool vec = rows_aligned(a.logits, a.stride, size) && a.experts * size >= 512;
-  if (type == FRC_BF16)
-    return vec ? launch_route<__nv_bfloat16, 8>(a, f, select, stats, sms, s)
-               : launch_route<__nv_bfloat16, 1>(a, f, select, stats, sms, s);
-  return vec ? launch_route<float, 4>(a, f, select, stats, sms, s) : launch_route<float, 1>(a, f, select, stats, sms, s);
+  const bool full = a.experts == kMaxExperts;
+  if (type == FRC_BF16) {
+    if (vec) return full ? launch_route<__nv_bfloat16, 8, true>(a, f, select, stats, sms, s) : launch_route<__nv_bfloat16, 8, false>(a, f, select, stats, sms, s);
+    return full ? launch_route<__nv_bfloat16, 1, true>(a, f, select, stats, sms, s) : launch_route<__nv_bfloat16, 1, false>(a, f, select, stats, sms, s);
+  }
+  if (vec) return full ? launch_route<float, 4, true>(a, f, select, stats, sms, s) : launch_route<float, 4, false>(a, f, select, stats, sms, s);
+  return full ? launch_route<float, 1, true>(a, f, select, stats, sms, s) : launch_route<float, 1, false>(a, f, select, stats, sms, s);
 }
 
-template <typename L, unsigned V>
+template <typename L, unsigned V, bool FULL>
 inline cudaError_t launch_backward(const RouteBackwardParams& a, unsigned sms, cudaStream_t s) {
   const unsigned warps = a.tokens <= 8 * sms ? 4 : 8, ctas = (a.tokens + warps - 1) / warps, grid = ctas < 3 * sms ? ctas : 3 * sms;
-  if (a.count) route_backward_kernel<L, V, true><<<grid, 32 * warps, 0, s>>>(a);
-  else route_backward_kernel<L, V, false><<<grid, 32 * warps, 0, s>>>(a);
+  if (a.count) route_backward_kernel<L, V, FULL, true><<<grid, 32 * warps, 0, s>>>(a);
+  else route_backward_kernel<L, V, FULL, false><<<grid, 32 * warps, 0, s>>>(a);
   return cudaGetLastError();
 }
 inline cudaError_t launch_backward(const RouteBackwardParams& a, unsigned type, unsigned sms, cudaStream_t s) {
   const size_t size = type == FRC_BF16 ? 2 : 4;
   const bool vec = rows_aligned(a.logits, a.stride, size) && rows_aligned(a.d_logits, a.d_stride, size);
-  if (type == FRC_BF16)
-    return vec ? launch_backward<__nv_bfloat16, 8>(a, sms, s) : launch_backward<__nv_bfloat16, 1>(a, sms, s);
-  return vec ? launch_backward<float, 4>(a, sms, s) : launch_backward<float, 1>(a, sms, s);
+  const bool full = a.experts == kMaxExperts;
+  if (type == FRC_BF16) {
+    if (vec) return full ? launch_backward<__nv_bfloat16, 8, true>(a, sms, s) : launch_backward<__nv_bfloat16, 8, false>(a, sms, s);
+    return full ? launch_backward<__nv_bfloat16, 1, true>(a, sms, s) : launch_backward<__nv_bfloat16, 1, false>(a, sms, s);
+  }
+  if (vec) return full ? launch_backward<float, 4, true>(a, sms, s) : launch_backward<float, 4, false>(a, sms, s);
+  return full ? launch_backward<float, 1, true>(a, sms, s) : launch_backward<float, 1, false>(a, sms, s);
 }
 
 }  // namespace frc
