@@ -30,7 +30,6 @@ namespace frc {
 
 constexpr unsigned kMvSpan = 256;          // weights of a row in one step
 constexpr unsigned kMvTile = 16;           // rows of one step
-constexpr unsigned kMvColPad = 64;         // bytes: columns start in alternate halves of the banks
 
 // Device layout: tile after tile (16 rows, the last one filled up with zero
 // rows), in it span after span of [scales][pieces], a piece being 64 weights
@@ -220,20 +219,25 @@ struct MvFrag {
   }
 };
 
-// The vectors of one K chunk in shared memory: columns of fp16 parts, per
-// token and span the power of two, and for Q4_K the sums over each 32 as
-// eight hi and eight lo parts (x 2^-5: they fit fp16).
+// The vectors of one K chunk in shared memory, as the products' B fragments:
+// per span and group of 32 a block of 8 NT columns of 64 bytes.
+//
+// With few columns (COLS = 1, 2, 4: tokens x parts, rounded up) the eight of
+// a product are shared by 8 / COLS groups: the block of group i holds its
+// values in columns (i mod (8 / COLS)) COLS + c and zeros elsewhere, so that
+// one accumulator keeps the groups' sums apart, each lane has the sums of its
+// own group, and a lane applies one scale where it would apply 8 / COLS.
 struct MvShared {
-  uint8_t* col;     // [tokens * P][chunk * 512 + pad]
-  float* scale;     // [tokens][chunk]
-  uint8_t* sums;    // [tokens][chunk][32]
+  uint8_t* col;     // [chunk][8 groups][NT][8 columns][64]
+  uint8_t* sums;    // Q4_K: [chunk][NT][8 columns][32]: sums over each 32 (x 2^-5, so they fit fp16), eight hi, eight
+                    // lo parts; zero in columns that are not the (hi part of a) token, or not its first group
+  float* scale;     // [tokens][chunk]: the power of two of each span
   float* part;      // [warps][values][32], when warps or CTAs share a tile
 };
-inline __host__ __device__ unsigned mv_col_bytes(unsigned chunk) { return chunk * 512 + kMvColPad; }
 
 // Spans first .. first + count of every token into shared memory, a warp a
 // (token, span) at a time with the values of U of them on their way.
-template <unsigned TYPE, unsigned P>
+template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS>
 __device__ __forceinline__ void mv_prepare(const MatvecParams& a, const MvShared& sh, unsigned first, unsigned count) {
   constexpr unsigned U = P == 2 ? 4 : 8, R = P == 2 ? 8 : 4;
   const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = blockDim.x / 32, units = a.tokens * count;
@@ -299,9 +303,10 @@ __device__ __forceinline__ void mv_prepare(const MatvecParams& a, const MvShared
         const __half2 l = __floats2half2_rn(p - b.x, q - b.y);
         lo[j] = *reinterpret_cast<const uint32_t*>(&l);
       }
-      uint8_t* c = sh.col + (t * P) * mv_col_bytes(a.chunk) + 512 * s + 16 * lane;
+      const unsigned grp = lane / 4, c0 = COLS < 8 ? (grp % (8 / COLS)) * COLS + t * P : t * P;
+      uint8_t* c = sh.col + ((s * 8 + grp) * NT + c0 / 8) * 512 + c0 % 8 * 64 + 16 * (lane % 4);
       *reinterpret_cast<uint4*>(c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      if (P == 2) *reinterpret_cast<uint4*>(c + mv_col_bytes(a.chunk)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      if (P == 2) *reinterpret_cast<uint4*>(c + 64) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       if (lane == 0) sh.scale[t * a.chunk + s] = finite ? __uint_as_float(static_cast<uint32_t>(127 + ex) << 23) : NAN;
       if (TYPE == kQ4K) {
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
@@ -309,7 +314,7 @@ __device__ __forceinline__ void mv_prepare(const MatvecParams& a, const MvShared
         sum *= 0.03125f;
         if (lane % 4 == 0) {
           const __half h = __float2half_rn(sum), l = __float2half_rn(sum - __half2float(h));
-          __half* o = reinterpret_cast<__half*>(sh.sums + (t * a.chunk + s) * 32) + lane / 4;
+          __half* o = reinterpret_cast<__half*>(sh.sums + (s * NT * 8 + t * P) * 32) + grp;
           o[0] = h;
           o[8] = l;
         }
@@ -318,154 +323,149 @@ __device__ __forceinline__ void mv_prepare(const MatvecParams& a, const MvShared
   }
 }
 
-// A lane's shared-memory addresses: its columns, their sums, its tokens' scales.
-template <unsigned P, unsigned NT>
+// A lane's part in the products: its fragment of a block, its tokens' scales
+// and, where groups share columns, which group's results it holds.
+template <unsigned P, unsigned NT, unsigned COLS>
 struct MvLane {
-  static constexpr unsigned kTok = P == 2 ? 1 : 2;  // tokens of a lane's results in a group of eight columns
-  uint32_t col[NT], sums[NT], scale[NT][kTok];
-  unsigned sel;  // bytes 2 q and 2 q + 1
+  static constexpr unsigned kTok = P == 2 || COLS == 1 ? 1 : 2;  // tokens of a lane's results in eight columns
+  uint32_t col, sums, scale[NT][kTok];
+  unsigned sel;      // bytes 2 q and 2 q + 1
+  unsigned mine[2];  // byte of the scale of the lane's first and second column, for a group set that starts at byte 0
+  __device__ __forceinline__ unsigned token(unsigned t, unsigned k, unsigned q) const {
+    if (COLS == 8) return P == 2 ? 4 * t + q : 8 * t + 2 * q + k;
+    return ((2 * q + k) % COLS) / P;
+  }
   __device__ __forceinline__ MvLane(const MatvecParams& a, const MvShared& sh, unsigned lane) {
-    const unsigned g = lane / 4, q = lane % 4, cols = a.tokens * P;
+    const unsigned g = lane / 4, q = lane % 4;
     sel = 2 * q | (2 * q + 1) << 4;
+    mine[0] = 2 * q / COLS;
+    mine[1] = (2 * q + 1) / COLS;
+    col = smem_u32(sh.col) + 64 * g + 16 * q;
+    sums = smem_u32(sh.sums) + 32 * g + 4 * q;
 #pragma unroll
-    for (unsigned t = 0; t < NT; ++t) {
-      const unsigned c = 8 * t + g < cols ? 8 * t + g : 0;  // columns past the tokens are not looked at
-      col[t] = smem_u32(sh.col) + c * mv_col_bytes(a.chunk) + 16 * q;
-      sums[t] = smem_u32(sh.sums) + (c / P) * a.chunk * 32 + 4 * q;
+    for (unsigned t = 0; t < NT; ++t)
 #pragma unroll
       for (unsigned k = 0; k < kTok; ++k) {
-        const unsigned tok = P == 2 ? 4 * t + q : 8 * t + 2 * q + k;
+        const unsigned tok = token(t, k, q);
         scale[t][k] = smem_u32(sh.scale) + 4 * ((tok < a.tokens ? tok : 0) * a.chunk);
       }
-    }
   }
 };
 
+// The fp16 operands of 32 columns of a tile from a lane's words (row g and row g + 8).
+template <unsigned TYPE>
+__device__ __forceinline__ void mv_weights(uint32_t w, uint32_t (&av)[4]) {
+  if (TYPE == kQ4K) {
+    const uint32_t u = w >> 8;
+    av[0] = w & 0x000f000fu;
+    av[1] = w & 0x00f000f0u;
+    av[2] = u & 0x000f000fu;
+    av[3] = u & 0x00f000f0u;
+  } else {
+    e2m1_f16(w, av);
+  }
+}
+// Byte `at` of the eight in {lo, hi} as a float: a 6-bit scale, or 2^(e - 127).
+template <unsigned TYPE>
+__device__ __forceinline__ float mv_scale(uint32_t lo, uint32_t hi, unsigned at) {
+  if (TYPE == kQ4K) return __uint_as_float(prmt(prmt(lo, hi, at), 0x4B000000u, 0x7440u)) - 8388608.0f;
+  return __uint_as_float((prmt(lo, hi, at) & 255u) << 23);
+}
+
 // One span (s of the chunk) of a tile times the columns; acc: [row g | row
-// g + 8] of the lane's token(s) in each group of eight columns.  FOLD: the
-// 6-bit scales of Q4_K go into the weights (eight half2 products per 32
-// columns of a tile), else onto the results (four fma per eight columns).
-template <unsigned TYPE, unsigned P, unsigned NT>
-__device__ __forceinline__ void mv_span(const MvLane<P, NT>& ln, const MvFrag<TYPE>& f, unsigned s, unsigned lane,
+// g + 8] of the lane's columns' tokens in each eight columns (the sum of both
+// columns for P = 2).  The 6-bit scales of Q4_K go onto the results, or with
+// NT = 4 (where that is more work) into the weights by half2 products.
+template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS>
+__device__ __forceinline__ void mv_span(const MvLane<P, NT, COLS>& ln, const MvFrag<TYPE>& f, unsigned s,
                                         float (&acc)[NT * (P == 2 ? 2 : 4)]) {
   constexpr bool FOLD = TYPE == kQ4K && NT > 2;
-  float sum[NT][4];
-#pragma unroll
-  for (unsigned t = 0; t < NT; ++t) sum[t][0] = sum[t][1] = sum[t][2] = sum[t][3] = 0.0f;
-  uint32_t xc[NT];
-#pragma unroll
-  for (unsigned t = 0; t < NT; ++t) xc[t] = ln.col[t] + 512 * s;
+  constexpr unsigned SHARE = 8 / COLS;  // groups in one accumulator
+  const uint32_t xc = ln.col + 4096 * NT * s;
+  uint32_t sc[2][2];  // eight scale bytes of rows g and g + 8
+  float d[2], dm[2], m[NT][4];
   if constexpr (TYPE == kQ4K) {
-    uint32_t sc[2][2], mi[2][2];
-    float d[2], dm[2], m[NT][4];
+    uint32_t mi[2][2];
 #pragma unroll
     for (unsigned h = 0; h < 2; ++h) {
       const uint4 b = f.s[h];
       d[h] = h2f(b.x & 0xffffu) * 16777216.0f;   // against q sc 2^-24
-      dm[h] = h2f(b.x >> 16) * 536870912.0f;     // against mi 2^-24 and sums 2^-5
+      dm[h] = h2f(b.x >> 16) * -536870912.0f;    // against mi 2^-24 and sums 2^-5
       sc[h][0] = b.y & 0x3f3f3f3fu;
       mi[h][0] = b.z & 0x3f3f3f3fu;
       sc[h][1] = (b.w & 0x0f0f0f0fu) | (b.y >> 2 & 0x30303030u);
       mi[h][1] = (b.w >> 4 & 0x0f0f0f0fu) | (b.z >> 2 & 0x30303030u);
     }
-    // minima of groups 2 q and 2 q + 1 as fp16 subnormals mi 2^-24, against the sums' hi and lo parts; the column
-    // of an fp32 token's lo part takes them too and is left out below
+    // minima of groups 2 q and 2 q + 1 as fp16 subnormals mi 2^-24, against the sums' hi and lo parts
     const uint32_t m0 = prmt(prmt(mi[0][0], mi[0][1], ln.sel), 0, 0x4140), m1 = prmt(prmt(mi[1][0], mi[1][1], ln.sel), 0, 0x4140);
 #pragma unroll
-    for (unsigned t = 0; t < NT; ++t) mma_f16_first(m[t], m0, m1, m0, m1, lds32(ln.sums[t] + 32 * s), lds32(ln.sums[t] + 32 * s + 16));
-#pragma unroll
-    for (unsigned j = 0; j < 4; ++j) {
-      const uint32_t w[4] = {f.w[j].x, f.w[j].y, f.w[j].z, f.w[j].w};
-#pragma unroll
-      for (unsigned e = 0; e < 2; ++e) {
-        const unsigned grp = 2 * j + e;
-        uint32_t av[2][4];
-        float k[2];
-#pragma unroll
-        for (unsigned h = 0; h < 2; ++h) {
-          const uint32_t v = w[2 * e + h], u = v >> 8;
-          av[h][0] = v & 0x000f000fu;
-          av[h][1] = v & 0x00f000f0u;
-          av[h][2] = u & 0x000f000fu;
-          av[h][3] = u & 0x00f000f0u;
-          if (FOLD) {
-            // 1024 + sc in both halves, less 1024
-            const uint32_t c = hsub2(prmt(sc[h][grp / 4], 0x64646464u, 0x4040u | (grp % 4) * 0x0101u), 0x64006400u);
-#pragma unroll
-            for (unsigned i = 0; i < 4; ++i) av[h][i] = hmul2(av[h][i], c);
-          } else {
-            k[h] = static_cast<float>(sc[h][grp / 4] >> (8 * (grp % 4)) & 255u);
-          }
-        }
-#pragma unroll
-        for (unsigned t = 0; t < NT; ++t) {
-          const uint4 b = lds128(xc[t] + 64 * grp);
-          if (FOLD) {
-            mma_f16(sum[t], av[0][0], av[1][0], av[0][1], av[1][1], b.x, b.y);
-            mma_f16(sum[t], av[0][2], av[1][2], av[0][3], av[1][3], b.z, b.w);
-          } else {
-            float c[4];
-            mma_f16_first(c, av[0][0], av[1][0], av[0][1], av[1][1], b.x, b.y);
-            mma_f16(c, av[0][2], av[1][2], av[0][3], av[1][3], b.z, b.w);
-#pragma unroll
-            for (unsigned i = 0; i < 4; ++i) sum[t][i] = fmaf(c[i], k[i / 2], sum[t][i]);
-          }
-        }
-      }
-    }
-#pragma unroll
     for (unsigned t = 0; t < NT; ++t) {
-#pragma unroll
-      for (unsigned h = 0; h < 2; ++h) {
-        if (P == 2) {
-          const float v = d[h] * (sum[t][2 * h] + sum[t][2 * h + 1]) - dm[h] * m[t][2 * h];
-          acc[2 * t + h] = fmaf(v, __uint_as_float(lds32(ln.scale[t][0] + 4 * s)), acc[2 * t + h]);
-        } else {
-#pragma unroll
-          for (unsigned c = 0; c < 2; ++c) {
-            const float v = d[h] * sum[t][2 * h + c] - dm[h] * m[t][2 * h + c];
-            acc[4 * t + 2 * h + c] = fmaf(v, __uint_as_float(lds32(ln.scale[t][P == 2 ? 0 : c] + 4 * s)), acc[4 * t + 2 * h + c]);
-          }
-        }
-      }
+      const uint32_t at = ln.sums + 256 * (NT * s + t);
+      mma_f16_first(m[t], m0, m1, m0, m1, lds32(at), lds32(at + 16));
     }
   } else {
-    const uint32_t ex[2][2] = {{f.s[0].x, f.s[0].y}, {f.s[0].z, f.s[0].w}};
+    sc[0][0] = f.s[0].x; sc[0][1] = f.s[0].y; sc[1][0] = f.s[0].z; sc[1][1] = f.s[0].w;
+  }
+  constexpr unsigned SV = P == 2 && !FOLD ? 2 : 4;
+  float sum[NT][SV], c[NT][4];
 #pragma unroll
-    for (unsigned j = 0; j < 4; ++j) {
-      const uint32_t w[4] = {f.w[j].x, f.w[j].y, f.w[j].z, f.w[j].w};
+  for (unsigned t = 0; t < NT; ++t)
 #pragma unroll
-      for (unsigned e = 0; e < 2; ++e) {
-        const unsigned grp = 2 * j + e;
-        uint32_t av[2][4];
-        float k[2];
+    for (unsigned i = 0; i < SV; ++i) sum[t][i] = 0.0f;
 #pragma unroll
-        for (unsigned h = 0; h < 2; ++h) {
-          e2m1_f16(w[2 * e + h], av[h]);
-          k[h] = __uint_as_float((ex[h][grp / 4] >> (8 * (grp % 4)) & 255u) << 23);
-        }
+  for (unsigned grp = 0; grp < 8; ++grp) {
+    const uint4 wv = f.w[grp / 2];
+    uint32_t a0[4], a1[4];
+    mv_weights<TYPE>(grp & 1 ? wv.z : wv.x, a0);
+    mv_weights<TYPE>(grp & 1 ? wv.w : wv.y, a1);
+    if (FOLD) {
+      // 1024 + sc in both halves, less 1024
+      const uint32_t sel = 0x4040u | (grp % 4) * 0x0101u;
+      const uint32_t k0 = hsub2(prmt(sc[0][grp / 4], 0x64646464u, sel), 0x64006400u), k1 = hsub2(prmt(sc[1][grp / 4], 0x64646464u, sel), 0x64006400u);
 #pragma unroll
-        for (unsigned t = 0; t < NT; ++t) {
-          const uint4 b = lds128(xc[t] + 64 * grp);
-          float c[4];
-          mma_f16_first(c, av[0][0], av[1][0], av[0][1], av[1][1], b.x, b.y);
-          mma_f16(c, av[0][2], av[1][2], av[0][3], av[1][3], b.z, b.w);
-#pragma unroll
-          for (unsigned i = 0; i < 4; ++i) sum[t][i] = fmaf(c[i], k[i / 2], sum[t][i]);
-        }
+      for (unsigned i = 0; i < 4; ++i) {
+        a0[i] = hmul2(a0[i], k0);
+        a1[i] = hmul2(a1[i], k1);
       }
     }
 #pragma unroll
     for (unsigned t = 0; t < NT; ++t) {
+      const uint4 b = lds128(xc + 512 * (NT * grp + t));
+      if (FOLD ? grp == 0 : grp % SHARE == 0) mma_f16_first(c[t], a0[0], a1[0], a0[1], a1[1], b.x, b.y);
+      else mma_f16(c[t], a0[0], a1[0], a0[1], a1[1], b.x, b.y);
+      mma_f16(c[t], a0[2], a1[2], a0[3], a1[3], b.z, b.w);
+    }
+    if (!FOLD && grp % SHARE == SHARE - 1) {  // the set's sums, each lane the group of its columns
+      constexpr unsigned K = COLS == 1 ? 2 : 1;
+      float k[2][K];
+#pragma unroll
+      for (unsigned h = 0; h < 2; ++h)
+#pragma unroll
+        for (unsigned i = 0; i < K; ++i) k[h][i] = mv_scale<TYPE>(sc[h][0], sc[h][1], grp + 1 - SHARE + (SHARE > 1 ? ln.mine[i] : 0));
+#pragma unroll
+      for (unsigned t = 0; t < NT; ++t)
+#pragma unroll
+        for (unsigned h = 0; h < 2; ++h) {
+          if (P == 2) {
+            sum[t][h] = fmaf(c[t][2 * h] + c[t][2 * h + 1], k[h][0], sum[t][h]);
+          } else {
+            sum[t][(2 * h) % SV] = fmaf(c[t][2 * h], k[h][0], sum[t][(2 * h) % SV]);
+            sum[t][(2 * h + 1) % SV] = fmaf(c[t][2 * h + 1], k[h][K - 1], sum[t][(2 * h + 1) % SV]);
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (unsigned t = 0; t < NT; ++t) {
+    constexpr unsigned A = P == 2 ? 1 : 2;  // results of a row a lane keeps
+#pragma unroll
+    for (unsigned k = 0; k < A; ++k) {
+      const float x = __uint_as_float(lds32(ln.scale[t][MvLane<P, NT, COLS>::kTok == 1 ? 0 : k] + 4 * s));
 #pragma unroll
       for (unsigned h = 0; h < 2; ++h) {
-        if (P == 2) {
-          acc[2 * t + h] = fmaf(sum[t][2 * h] + sum[t][2 * h + 1], __uint_as_float(lds32(ln.scale[t][0] + 4 * s)), acc[2 * t + h]);
-        } else {
-#pragma unroll
-          for (unsigned c = 0; c < 2; ++c)
-            acc[4 * t + 2 * h + c] = fmaf(sum[t][2 * h + c], __uint_as_float(lds32(ln.scale[t][P == 2 ? 0 : c] + 4 * s)), acc[4 * t + 2 * h + c]);
-        }
+        float v = P == 2 ? (FOLD ? c[t][2 * h] + c[t][2 * h + 1] : sum[t][h % SV]) : (FOLD ? c[t][2 * h + k] : sum[t][(2 * h + k) % SV]);
+        if (TYPE == kQ4K) v = fmaf(v, d[h], (P == 2 ? m[t][2 * h] : m[t][2 * h + k]) * dm[h]);
+        acc[(2 * t + h) * A + k] = fmaf(v, x, acc[(2 * t + h) * A + k]);
       }
     }
   }
@@ -479,17 +479,17 @@ __device__ __forceinline__ void mv_cluster_sync() {
 // a cluster share K.  Tiles are dealt round robin; x is prepared once a CTA,
 // or once a tile and chunk where it does not fit shared memory as a whole.
 // The next span's weights are on their way while one is worked on.
-template <unsigned TYPE, unsigned P, unsigned NT, unsigned W>
+template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS, unsigned W>
 __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 1) matvec_kernel(const MatvecParams a) {
   constexpr unsigned V = NT * (P == 2 ? 2 : 4), kBytes = MvFrag<TYPE>::kBytes;
   extern __shared__ __align__(128) uint8_t smem[];
   const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, q = lane % 4;
   MvShared sh;
   sh.col = smem;
-  sh.sums = smem + a.tokens * P * mv_col_bytes(a.chunk);
-  sh.scale = reinterpret_cast<float*>(sh.sums + (TYPE == kQ4K ? a.tokens * a.chunk * 32 : 0));
+  sh.sums = smem + 4096 * NT * a.chunk;
+  sh.scale = reinterpret_cast<float*>(sh.sums + (TYPE == kQ4K ? 256 * NT * a.chunk : 0));
   sh.part = sh.scale + a.tokens * a.chunk;
-  const MvLane<P, NT> ln(a, sh, lane);
+  const MvLane<P, NT, COLS> ln(a, sh, lane);
   const unsigned split = a.split, per_cta = W / split, sub = warp / split, ks = warp % split;
   const unsigned rank = a.cluster > 1 ? blockIdx.x % a.cluster : 0, cta = blockIdx.x / a.cluster, ctas = gridDim.x / a.cluster;
   const unsigned k_first = rank * a.slice, k_end = min(a.spans, k_first + a.slice);
@@ -509,8 +509,13 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 1) matvec_kernel(const Ma
       const auto fetch = [&](MvFrag<TYPE>& f, unsigned at) { f.load(p, at == last ? a.pieces_last : 4, lane); };
       if (any) fetch(f0, s);
       if (!prepared || a.chunk < a.slice) {
+        if (!prepared) {  // what no value goes to: columns of other groups, columns without sums
+          uint4* z = reinterpret_cast<uint4*>(COLS < 8 ? sh.col : sh.sums);
+          const unsigned n16 = static_cast<unsigned>(reinterpret_cast<uint8_t*>(sh.scale) - reinterpret_cast<uint8_t*>(z)) / 16;
+          for (unsigned i = threadIdx.x; i < n16; i += 32 * W) z[i] = make_uint4(0, 0, 0, 0);
+        }
         __syncthreads();  // every warp has left the chunk before
-        mv_prepare<TYPE, P>(a, sh, first, count);
+        mv_prepare<TYPE, P, NT, COLS>(a, sh, first, count);
         __syncthreads();
         prepared = true;
       }
@@ -519,15 +524,27 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 1) matvec_kernel(const Ma
         while (true) {
           p += step;
           if (s + split < count) fetch(f1, s + split);
-          mv_span<TYPE, P, NT>(ln, f0, s, lane, acc);
+          mv_span<TYPE, P, NT, COLS>(ln, f0, s, acc);
           s += split;
           if (s >= count) break;
           p += step;
           if (s + split < count) fetch(f0, s + split);
-          mv_span<TYPE, P, NT>(ln, f1, s, lane, acc);
+          mv_span<TYPE, P, NT, COLS>(ln, f1, s, acc);
           s += split;
           if (s >= count) break;
         }
+      }
+    }
+    if (COLS < 8) {  // the groups' lanes together
+      if (COLS == 1) {
+        acc[0] += acc[1];
+        acc[2 % V] += acc[3 % V];
+      }
+#pragma unroll
+      for (unsigned i = 0; i < V; ++i) {
+        if (COLS == 1 && (i & 1)) continue;
+        if (COLS <= 2) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 1);
+        acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 2);
       }
     }
     if (split > 1 || a.cluster > 1) {
@@ -575,9 +592,10 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 1) matvec_kernel(const Ma
         }
 #pragma unroll
         for (unsigned i = 0; i < V / 2; ++i) {
-          const unsigned tok = P == 2 ? 4 * i + q : 8 * (i / 2) + 2 * q + i % 2;
-          if (tok >= a.tokens) continue;
-          float v = acc[P == 2 ? 2 * i + h : 4 * (i / 2) + 2 * h + i % 2];
+          constexpr unsigned A = P == 2 ? 1 : 2;
+          const unsigned t = i / A, k = i % A, tok = ln.token(t, k, q);
+          if (tok >= a.tokens || (COLS < 8 && (2 * q + k) / COLS)) continue;
+          float v = acc[(2 * t + h) * A + k];
           if (TYPE == kMXFP4) v *= f;
           if (a.y_bf16) {
             const __nv_bfloat16 o = __float2bfloat16_rn(v);
@@ -603,9 +621,9 @@ struct MvPlan {
 constexpr unsigned kMvSmemSm = 228 * 1024, kMvSmemCta = 227 * 1024;
 
 // Shared memory of a CTA; the parts only where warps or CTAs share tiles.
-inline size_t mv_smem(unsigned type, unsigned P, unsigned tokens, unsigned values, unsigned warps, unsigned chunk, bool part) {
-  return static_cast<size_t>(tokens) * P * mv_col_bytes(chunk) +
-         static_cast<size_t>(tokens) * chunk * ((type == FRC_Q4_K ? 32 : 0) + 4) + (part ? static_cast<size_t>(warps) * values * 128 : 0);
+inline size_t mv_smem(unsigned type, unsigned nt, unsigned tokens, unsigned values, unsigned warps, unsigned chunk, bool part) {
+  return static_cast<size_t>(chunk) * (nt * (4096 + (type == FRC_Q4_K ? 256 : 0)) + 4 * tokens) +
+         (part ? static_cast<size_t>(warps) * values * 128 : 0);
 }
 
 // Chooses the warps a CTA, the CTAs that share K and the warps that share a
@@ -623,8 +641,8 @@ inline MvPlan mv_plan(unsigned type, unsigned P, unsigned nt, unsigned tokens, c
       p.cluster = cluster;
       p.slice = p.chunk = (l.spans + cluster - 1) / cluster;
       const size_t limit = warps == 8 ? (kMvSmemSm - 2048) / 2 : kMvSmemCta;
-      if (warps == 8 && mv_smem(type, P, tokens, values, warps, p.chunk, true) > limit) continue;
-      while (mv_smem(type, P, tokens, values, warps, p.chunk, true) > limit) p.chunk = (p.chunk + 1) / 2;
+      if (warps == 8 && mv_smem(type, nt, tokens, values, warps, p.chunk, true) > limit) continue;
+      while (mv_smem(type, nt, tokens, values, warps, p.chunk, true) > limit) p.chunk = (p.chunk + 1) / 2;
       // clusters do not tile the SMs of every GPC
       const unsigned resident = sms * (warps == 8 ? 2 : 1) / cluster * (cluster > 1 ? 7 : 8) / 8;
       if (!resident) continue;
@@ -642,14 +660,14 @@ inline MvPlan mv_plan(unsigned type, unsigned P, unsigned nt, unsigned tokens, c
       }
     }
   }
-  best.smem = static_cast<unsigned>(mv_smem(type, P, tokens, values, best.warps, best.chunk, best.split > 1 || best.cluster > 1));
+  best.smem = static_cast<unsigned>(mv_smem(type, nt, tokens, values, best.warps, best.chunk, best.split > 1 || best.cluster > 1));
   return best;
 }
 
-template <unsigned TYPE, unsigned P, unsigned NT, unsigned W>
+template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS, unsigned W>
 inline cudaError_t mv_launch(const MatvecParams& a, const MvPlan& p, cudaStream_t s) {
   if (p.smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(matvec_kernel<TYPE, P, NT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    const cudaError_t e = cudaFuncSetAttribute(matvec_kernel<TYPE, P, NT, COLS, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                static_cast<int>(p.smem));
     if (e != cudaSuccess) return e;
   }
@@ -664,11 +682,11 @@ inline cudaError_t mv_launch(const MatvecParams& a, const MvPlan& p, cudaStream_
   cfg.stream = s;
   cfg.attrs = &at;
   cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, matvec_kernel<TYPE, P, NT, W>, a);
+  return cudaLaunchKernelEx(&cfg, matvec_kernel<TYPE, P, NT, COLS, W>, a);
 }
-template <unsigned TYPE, unsigned P, unsigned NT>
+template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS>
 inline cudaError_t mv_launch_w(const MatvecParams& a, const MvPlan& p, cudaStream_t s) {
-  return p.warps == 8 ? mv_launch<TYPE, P, NT, 8>(a, p, s) : mv_launch<TYPE, P, NT, 16>(a, p, s);
+  return p.warps == 8 ? mv_launch<TYPE, P, NT, COLS, 8>(a, p, s) : mv_launch<TYPE, P, NT, COLS, 16>(a, p, s);
 }
 
 template <unsigned TYPE>
@@ -681,10 +699,10 @@ inline cudaError_t launch_matvec(MatvecParams& a, const MvLayout& l, unsigned x_
     if (sscanf(e, "%u,%u,%u", &w, &c, &sp) == 3) {
       const unsigned values = nt * (P == 2 ? 2 : 4);
       p.warps = w; p.cluster = c; p.split = sp; p.slice = p.chunk = (l.spans + c - 1) / c;
-      while (mv_smem(TYPE, P, a.tokens, values, w, p.chunk, true) > (w == 8 ? (kMvSmemSm - 2048) / 2 : kMvSmemCta)) p.chunk = (p.chunk + 1) / 2;
+      while (mv_smem(TYPE, nt, a.tokens, values, w, p.chunk, true) > (w == 8 ? (kMvSmemSm - 2048) / 2 : kMvSmemCta)) p.chunk = (p.chunk + 1) / 2;
       const unsigned per = w / sp, groups = (l.tiles + per - 1) / per, resident = sms * (w == 8 ? 2 : 1) / c * (c > 1 ? 7 : 8) / 8;
       p.grid = (groups < resident ? groups : resident) * c;
-      p.smem = mv_smem(TYPE, P, a.tokens, values, w, p.chunk, sp > 1 || c > 1);
+      p.smem = mv_smem(TYPE, nt, a.tokens, values, w, p.chunk, sp > 1 || c > 1);
     }
     fprintf(stderr, "plan warps %u cluster %u split %u slice %u chunk %u grid %u smem %u\n", p.warps, p.cluster, p.split, p.slice, p.chunk, p.grid, p.smem);
   }
@@ -692,12 +710,17 @@ inline cudaError_t launch_matvec(MatvecParams& a, const MvLayout& l, unsigned x_
   a.tile_bytes = l.tile_bytes; a.base_at = l.base_at; a.tiles = l.tiles; a.spans = l.spans; a.pieces_last = l.pieces_last;
   a.slice = p.slice; a.chunk = p.chunk; a.split = p.split; a.cluster = p.cluster;
   if (P == 2) {
-    if (nt == 1) return mv_launch_w<TYPE, 2, 1>(a, p, s);
-    if (nt == 2) return mv_launch_w<TYPE, 2, 2>(a, p, s);
-    return mv_launch_w<TYPE, 2, 4>(a, p, s);
+    if (cols <= 2) return mv_launch_w<TYPE, 2, 1, 2>(a, p, s);
+    if (cols <= 4) return mv_launch_w<TYPE, 2, 1, 4>(a, p, s);
+    if (nt == 1) return mv_launch_w<TYPE, 2, 1, 8>(a, p, s);
+    if (nt == 2) return mv_launch_w<TYPE, 2, 2, 8>(a, p, s);
+    return mv_launch_w<TYPE, 2, 4, 8>(a, p, s);
   }
-  if (nt == 1) return mv_launch_w<TYPE, 1, 1>(a, p, s);
-  return mv_launch_w<TYPE, 1, 2>(a, p, s);
+  if (cols <= 1) return mv_launch_w<TYPE, 1, 1, 1>(a, p, s);
+  if (cols <= 2) return mv_launch_w<TYPE, 1, 1, 2>(a, p, s);
+  if (cols <= 4) return mv_launch_w<TYPE, 1, 1, 4>(a, p, s);
+  if (nt == 1) return mv_launch_w<TYPE, 1, 1, 8>(a, p, s);
+  return mv_launch_w<TYPE, 1, 2, 8>(a, p, s);
 }
 
 }  // namespace frc
