@@ -132,7 +132,6 @@ struct MatvecParams {
   unsigned rows, n, tokens, tiles, spans, pieces_last;
   unsigned slice;             // spans of K a CTA works on (all, or a share where a cluster splits K)
   unsigned chunk;             // spans of x in shared memory at a time, at most the slice
-  unsigned split;             // warps that share a tile's spans
   unsigned cluster;           // CTAs that share K
   unsigned x_vec, y_bf16;     // x rows are 16-byte aligned; y is bf16
   unsigned* status;
@@ -174,13 +173,6 @@ __device__ __forceinline__ void e2m1_f16(uint32_t w, uint32_t (&h)[4]) {
       : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
       : "r"(w));
 }
-__device__ __forceinline__ uint4 ldg_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
@@ -192,29 +184,39 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   return v;
 }
 
-// A lane's share of one span of a tile.
+// A lane's share of one span of a tile, and the slots of shared memory that a
+// warp has its next spans copied to (a lane copies the words it will read;
+// the scales are read by other lanes too).
 template <unsigned TYPE>
 struct MvFrag {
   static constexpr unsigned kScale = TYPE == kQ4K ? 256 : 128, kBytes = kScale + 2048;
   uint4 w[4];
   uint4 s[TYPE == kQ4K ? 2 : 1];  // Q4_K: headers of rows g and g + 8; MXFP4: their exponents, 8 bytes each
 
-  __device__ __forceinline__ void load(const uint8_t* p, unsigned pieces, unsigned lane) {  // p: the span
+  static __device__ __forceinline__ void copy(uint32_t slot, const uint8_t* p, unsigned pieces, unsigned lane) {  // p: the span
     const uint8_t* q = p + 16 * lane + kScale;
-    if (TYPE == kQ4K || pieces == 4) {
+    const uint32_t d = slot + 16 * lane + kScale;
 #pragma unroll
-      for (unsigned j = 0; j < 4; ++j) w[j] = ldg_stream(q + 512 * j);
-    } else {
+    for (unsigned j = 0; j < 4; ++j)
+      if (TYPE == kQ4K || j < pieces)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + 512 * j), "l"(q + 512 * j) : "memory");
+    if (lane < kScale / 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d - kScale), "l"(q - kScale) : "memory");
+  }
+  __device__ __forceinline__ void read(uint32_t slot, unsigned pieces, unsigned lane) {
+    const uint32_t d = slot + 16 * lane + kScale, e = slot + (kScale / 16) * (lane / 4);
 #pragma unroll
-      for (unsigned j = 0; j < 4; ++j) w[j] = j < pieces ? ldg_stream(q + 512 * j) : make_uint4(0, 0, 0, 0);
-    }
+    for (unsigned j = 0; j < 4; ++j) w[j] = lds128(d + 512 * j);
     if (TYPE == kQ4K) {
-      s[0] = ldg_stream(p + 16 * (lane / 4));
-      s[TYPE == kQ4K ? 1 : 0] = ldg_stream(p + 128 + 16 * (lane / 4));
+      s[0] = lds128(e);
+      s[TYPE == kQ4K ? 1 : 0] = lds128(e + 128);
     } else {
-      const uint2 e0 = __ldg(reinterpret_cast<const uint2*>(p) + lane / 4);
-      const uint2 e1 = __ldg(reinterpret_cast<const uint2*>(p) + 8 + lane / 4);
-      s[0] = make_uint4(e0.x, e0.y, e1.x, e1.y);
+      asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(s[0].x), "=r"(s[0].y) : "r"(e));
+      asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(s[0].z), "=r"(s[0].w) : "r"(e + 64));
+      if (pieces < 4) {
+#pragma unroll
+        for (unsigned j = 1; j < 4; ++j)
+          if (j >= pieces) w[j] = make_uint4(0, 0, 0, 0);
+      }
     }
   }
 };
@@ -230,9 +232,11 @@ struct MvFrag {
 struct MvShared {
   uint8_t* col;     // [chunk][8 groups][NT][8 columns][64]
   uint8_t* sums;    // Q4_K: [chunk][NT][8 columns][32]: sums over each 32 (x 2^-5, so they fit fp16), eight hi, eight
-                    // lo parts; zero in columns that are not the (hi part of a) token, or not its first group
+                    // lo parts, in a token's (first) column of the first group; columns of other groups are zero
   float* scale;     // [tokens][chunk]: the power of two of each span
-  float* part;      // [warps][values][32], when warps or CTAs share a tile
+  float* part;      // [warps][values][32]: sums of tiles that a warp did not begin; in a cluster
+                    // [tiles][values][32] behind them: the CTA's share of its tiles
+  uint8_t* ring;    // [warps][DEPTH][span]
 };
 
 // Spans first .. first + count of every token into shared memory, a warp a
@@ -365,11 +369,19 @@ __device__ __forceinline__ void mv_weights(uint32_t w, uint32_t (&av)[4]) {
     e2m1_f16(w, av);
   }
 }
-// Byte `at` of the eight in {lo, hi} as a float: a 6-bit scale, or 2^(e - 127).
+// Byte `at` of the eight in {lo, hi} as a float: a 6-bit scale, or 2^(e - 127)
+// (e at most 127).
 template <unsigned TYPE>
 __device__ __forceinline__ float mv_scale(uint32_t lo, uint32_t hi, unsigned at) {
-  if (TYPE == kQ4K) return __uint_as_float(prmt(prmt(lo, hi, at), 0x4B000000u, 0x7440u)) - 8388608.0f;
-  return __uint_as_float((prmt(lo, hi, at) & 255u) << 23);
+  const uint32_t v = prmt(lo, hi, at);
+  if (TYPE == kQ4K) return __uint_as_float(prmt(v, 0x4B000000u, 0x7440u)) - 8388608.0f;
+  return __uint_as_float(v << 23 & 0x7f800000u);
+}
+template <unsigned TYPE>
+__device__ __forceinline__ float mv_scale_at(const uint32_t (&b)[2], unsigned at) {  // at known when compiled
+  const uint32_t v = b[at / 4];
+  if (TYPE == kQ4K) return __uint_as_float(prmt(v, 0x4B000000u, 0x7440u | at % 4)) - 8388608.0f;
+  return __uint_as_float((at % 4 == 3 ? v >> 1 : v << (23 - 8 * (at % 4))) & 0x7f800000u);
 }
 
 // One span (s of the chunk) of a tile times the columns; acc: [row g | row
@@ -441,7 +453,7 @@ __device__ __forceinline__ void mv_span(const MvLane<P, NT, COLS>& ln, const MvF
 #pragma unroll
       for (unsigned h = 0; h < 2; ++h)
 #pragma unroll
-        for (unsigned i = 0; i < K; ++i) k[h][i] = mv_scale<TYPE>(sc[h][0], sc[h][1], grp + 1 - SHARE + (SHARE > 1 ? ln.mine[i] : 0));
+        for (unsigned i = 0; i < K; ++i) k[h][i] = SHARE > 1 ? mv_scale<TYPE>(sc[h][0], sc[h][1], grp + 1 - SHARE + ln.mine[i]) : mv_scale_at<TYPE>(sc[h], grp);
 #pragma unroll
       for (unsigned t = 0; t < NT; ++t)
 #pragma unroll
@@ -475,138 +487,225 @@ __device__ __forceinline__ void mv_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// CTAs of W warps; `split` of them share the spans of a tile, and the CTAs of
-// a cluster share K.  Tiles are dealt round robin; x is prepared once a CTA,
-// or once a tile and chunk where it does not fit shared memory as a whole.
-// The next span's weights are on their way while one is worked on.
-template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS, unsigned W>
+// Stores the results of a tile (acc as mv_span leaves it).
+template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS>
+__device__ __forceinline__ bool mv_store(const MatvecParams& a, const MvLane<P, NT, COLS>& ln, unsigned tile, unsigned lane,
+                                         const float (&acc)[NT * (P == 2 ? 2 : 4)]) {
+  constexpr unsigned V = NT * (P == 2 ? 2 : 4), A = P == 2 ? 1 : 2;
+  const unsigned g = lane / 4, q = lane % 4;
+  bool bad = false;
+#pragma unroll
+  for (unsigned h = 0; h < 2; ++h) {
+    const unsigned row = tile * kMvTile + g + 8 * h;
+    if (row >= a.rows) continue;
+    float f = 1.0f;
+    if (TYPE == kMXFP4) {
+      const unsigned e = a.w[a.base_at + row];
+      f = __uint_as_float(e ? e << 23 : 0x00400000u);
+    }
+#pragma unroll
+    for (unsigned i = 0; i < V / 2; ++i) {
+      const unsigned t = i / A, k = i % A, tok = ln.token(t, k, q);
+      if (tok >= a.tokens || (COLS < 8 && (2 * q + k) / COLS)) continue;
+      float v = acc[(2 * t + h) * A + k];
+      if (TYPE == kMXFP4) v *= f;
+      if (a.y_bf16) {
+        const __nv_bfloat16 o = __float2bfloat16_rn(v);
+        v = __bfloat162float(o);
+        static_cast<__nv_bfloat16*>(a.y)[tok * a.y_stride + row] = o;
+      } else {
+        static_cast<float*>(a.y)[tok * a.y_stride + row] = v;
+      }
+      bad |= !isfinite(v);
+    }
+  }
+  return bad;
+}
+
+// The lanes that hold groups of the same columns together.
+template <unsigned P, unsigned NT, unsigned COLS>
+__device__ __forceinline__ void mv_join(float (&acc)[NT * (P == 2 ? 2 : 4)]) {
+  constexpr unsigned V = NT * (P == 2 ? 2 : 4);
+  if (COLS == 8) return;
+  if (COLS == 1) {
+    acc[0] += acc[1];
+    acc[2 % V] += acc[3 % V];
+  }
+#pragma unroll
+  for (unsigned i = 0; i < V; ++i) {
+    if (COLS == 1 && (i & 1)) continue;
+    if (COLS <= 2) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 1);
+    acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 2);
+  }
+}
+
+// A CTA (of each cluster: the CTAs of a cluster share K) takes a run of
+// tiles, and its W warps equal shares of the run's spans, wherever they fall:
+// a tile's sum is finished by the warp that began it, which adds the parts of
+// the warps behind it in order.  x is prepared once, while each warp has the
+// weights of its first DEPTH spans on their way.  Where the slice of x does
+// not fit shared memory (chunk < slice), a warp takes one tile at a time and
+// x is prepared anew for every W tiles, chunk by chunk.
+template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS, unsigned W, unsigned DEPTH>
 __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 1) matvec_kernel(const MatvecParams a) {
   constexpr unsigned V = NT * (P == 2 ? 2 : 4), kBytes = MvFrag<TYPE>::kBytes;
   extern __shared__ __align__(128) uint8_t smem[];
-  const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, q = lane % 4;
+  const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   MvShared sh;
-  sh.col = smem;
-  sh.sums = smem + 4096 * NT * a.chunk;
+  sh.ring = smem;
+  sh.col = smem + W * DEPTH * kBytes;
+  sh.sums = sh.col + 4096 * NT * a.chunk;
   sh.scale = reinterpret_cast<float*>(sh.sums + (TYPE == kQ4K ? 256 * NT * a.chunk : 0));
   sh.part = sh.scale + a.tokens * a.chunk;
   const MvLane<P, NT, COLS> ln(a, sh, lane);
-  const unsigned split = a.split, per_cta = W / split, sub = warp / split, ks = warp % split;
   const unsigned rank = a.cluster > 1 ? blockIdx.x % a.cluster : 0, cta = blockIdx.x / a.cluster, ctas = gridDim.x / a.cluster;
   const unsigned k_first = rank * a.slice, k_end = min(a.spans, k_first + a.slice);
-  bool prepared = false, bad = false;
-  for (unsigned base = cta * per_cta; base < a.tiles; base += ctas * per_cta) {
-    const unsigned tile = base + sub;
-    float acc[V];
+  const unsigned count = k_first < k_end ? k_end - k_first : 0;
+  // 32 bits hold these: tiles up to 2^20, a run of up to tiles / CTAs, 256 spans
+  const unsigned t0 = a.tiles * cta / ctas, t1 = a.tiles * (cta + 1) / ctas;
+  const uint32_t ring = smem_u32(sh.ring) + warp * DEPTH * kBytes;
+  unsigned in = 0, out = 0;
+  bool bad = false;
+  float acc[V];
 #pragma unroll
-    for (unsigned i = 0; i < V; ++i) acc[i] = 0.0f;
-    for (unsigned first = k_first; first < k_end; first += a.chunk) {
-      const unsigned count = min(a.chunk, k_end - first);
-      const bool any = tile < a.tiles && ks < count;
-      MvFrag<TYPE> f0, f1;
-      const uint8_t* p = a.w + tile * a.tile_bytes + static_cast<size_t>(first + ks) * kBytes;
-      const unsigned last = a.spans - 1 - first;  // the span that may be short
-      unsigned s = ks;
-      const auto fetch = [&](MvFrag<TYPE>& f, unsigned at) { f.load(p, at == last ? a.pieces_last : 4, lane); };
-      if (any) fetch(f0, s);
-      if (!prepared || a.chunk < a.slice) {
-        if (!prepared) {  // what no value goes to: columns of other groups, columns without sums
-          uint4* z = reinterpret_cast<uint4*>(COLS < 8 ? sh.col : sh.sums);
-          const unsigned n16 = static_cast<unsigned>(reinterpret_cast<uint8_t*>(sh.scale) - reinterpret_cast<uint8_t*>(z)) / 16;
-          for (unsigned i = threadIdx.x; i < n16; i += 32 * W) z[i] = make_uint4(0, 0, 0, 0);
-        }
+  for (unsigned i = 0; i < V; ++i) acc[i] = 0.0f;
+  const auto fill = [&]() {  // what no value goes to: columns of other groups
+    uint4* z = reinterpret_cast<uint4*>(sh.col);
+    const unsigned n16 = static_cast<unsigned>(reinterpret_cast<uint8_t*>(sh.scale) - sh.col) / 16;
+    for (unsigned i = threadIdx.x; i < n16; i += 32 * W) z[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+  };
+  const auto place = [&](unsigned tile, unsigned span) {
+    return a.w + static_cast<size_t>(tile) * a.tile_bytes + static_cast<size_t>(span) * kBytes;
+  };
+  if (a.chunk < a.slice) {
+    if (COLS < 8) fill();
+    for (unsigned base = t0; base < t1; base += W) {
+      const unsigned tile = base + warp;
+      for (unsigned first = k_first; first < k_end; first += a.chunk) {
+        const unsigned part = min(a.chunk, k_end - first);
         __syncthreads();  // every warp has left the chunk before
-        mv_prepare<TYPE, P, NT, COLS>(a, sh, first, count);
+        mv_prepare<TYPE, P, NT, COLS>(a, sh, first, part);
         __syncthreads();
-        prepared = true;
-      }
-      if (any) {
-        const size_t step = static_cast<size_t>(split) * kBytes;
-        while (true) {
-          p += step;
-          if (s + split < count) fetch(f1, s + split);
-          mv_span<TYPE, P, NT, COLS>(ln, f0, s, acc);
-          s += split;
-          if (s >= count) break;
-          p += step;
-          if (s + split < count) fetch(f0, s + split);
-          mv_span<TYPE, P, NT, COLS>(ln, f1, s, acc);
-          s += split;
-          if (s >= count) break;
+        if (tile >= t1) continue;
+        for (unsigned s = 0; s < part; ++s) {
+          const unsigned pieces = first + s + 1 == a.spans ? a.pieces_last : 4;
+          MvFrag<TYPE>::copy(ring, place(tile, first + s), pieces, lane);
+          asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+          __syncwarp();
+          MvFrag<TYPE> f;
+          f.read(ring, pieces, lane);
+          __syncwarp();
+          mv_span<TYPE, P, NT, COLS>(ln, f, s, acc);
         }
       }
+      if (tile < t1) {
+        mv_join<P, NT, COLS>(acc);
+        bad |= mv_store<TYPE, P, NT, COLS>(a, ln, tile, lane, acc);
+      }
+#pragma unroll
+      for (unsigned i = 0; i < V; ++i) acc[i] = 0.0f;
     }
-    if (COLS < 8) {  // the groups' lanes together
-      if (COLS == 1) {
-        acc[0] += acc[1];
-        acc[2 % V] += acc[3 % V];
-      }
-#pragma unroll
-      for (unsigned i = 0; i < V; ++i) {
-        if (COLS == 1 && (i & 1)) continue;
-        if (COLS <= 2) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 1);
-        acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 2);
-      }
-    }
-    if (split > 1 || a.cluster > 1) {
-      float* p = sh.part + (warp * V) * 32 + lane;
-#pragma unroll
-      for (unsigned i = 0; i < V; ++i) p[32 * i] = acc[i];
-      __syncthreads();
-      if (ks == 0 && split > 1) {
-        for (unsigned w = 1; w < split; ++w)
-#pragma unroll
-          for (unsigned i = 0; i < V; ++i) acc[i] += p[32 * (w * V + i)];
-        if (a.cluster > 1) {
-#pragma unroll
-          for (unsigned i = 0; i < V; ++i) p[32 * i] = acc[i];
+  } else {
+    const unsigned work = (t1 - t0) * count;
+    const auto share = [&](unsigned w) { return work * w / W; };
+    const unsigned l0 = share(warp), l1 = share(warp + 1);
+    unsigned tile = count ? t0 + l0 / count : t0, s = count ? l0 % count : 0;
+    // the copies run DEPTH spans ahead
+    unsigned at_tile = tile, at_s = s, at_left = l1 - l0;
+    const uint8_t* at = place(tile, k_first + s);
+    const auto copy = [&]() {
+      if (at_left) {
+        --at_left;
+        MvFrag<TYPE>::copy(ring + in, at, k_first + at_s + 1 == a.spans ? a.pieces_last : 4, lane);
+        at += kBytes;
+        if (++at_s == count) {
+          at_s = 0;
+          at = place(++at_tile, k_first);
         }
       }
-      if (a.cluster > 1) {
-        mv_cluster_sync();
-        if (rank == 0 && ks == 0) {
-          for (unsigned r = 1; r < a.cluster; ++r) {
-            uint32_t at;
-            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(r));
+      asm volatile("cp.async.commit_group;" ::: "memory");  // empty groups keep the count
+      in = in + kBytes == DEPTH * kBytes ? 0 : in + kBytes;
+    };
 #pragma unroll
-            for (unsigned i = 0; i < V; ++i) {
-              float v;
-              asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at + 128 * i) : "memory");
-              acc[i] += v;
-            }
-          }
-        }
-        mv_cluster_sync();
+    for (unsigned i = 0; i < DEPTH; ++i) copy();
+    if (COLS < 8) fill();
+    mv_prepare<TYPE, P, NT, COLS>(a, sh, k_first, count);
+    __syncthreads();
+    float* mine = sh.part + warp * V * 32 + lane;
+    float* tiles = sh.part + W * V * 32 + lane;  // of a cluster's CTA
+    const auto finish = [&](unsigned t) {
+      if (a.cluster == 1) {
+        bad |= mv_store<TYPE, P, NT, COLS>(a, ln, t, lane, acc);
       } else {
-        __syncthreads();
+#pragma unroll
+        for (unsigned i = 0; i < V; ++i) tiles[(t - t0) * V * 32 + 32 * i] = acc[i];
+      }
+    };
+    bool began = s == 0;
+    for (unsigned l = l0; l < l1; ++l) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+      __syncwarp();
+      MvFrag<TYPE> f;
+      f.read(ring + out, k_first + s + 1 == a.spans ? a.pieces_last : 4, lane);
+      __syncwarp();  // the slot has been read
+      out = out + kBytes == DEPTH * kBytes ? 0 : out + kBytes;
+      copy();
+      mv_span<TYPE, P, NT, COLS>(ln, f, s, acc);
+      if (++s == count) {
+        mv_join<P, NT, COLS>(acc);
+        if (began) {
+          finish(tile);
+        } else {
+#pragma unroll
+          for (unsigned i = 0; i < V; ++i) mine[32 * i] = acc[i];
+        }
+        began = true;
+        s = 0;
+        ++tile;
+#pragma unroll
+        for (unsigned i = 0; i < V; ++i) acc[i] = 0.0f;
       }
     }
-    if (ks == 0 && rank == 0 && tile < a.tiles) {
+    if (s && l0 < l1) {
+      mv_join<P, NT, COLS>(acc);
+      if (!began) {
 #pragma unroll
-      for (unsigned h = 0; h < 2; ++h) {
-        const unsigned row = tile * kMvTile + g + 8 * h;
-        if (row >= a.rows) continue;
-        float f = 1.0f;
-        if (TYPE == kMXFP4) {
-          const unsigned e = a.w[a.base_at + row];
-          f = __uint_as_float(e ? e << 23 : 0x00400000u);
-        }
-#pragma unroll
-        for (unsigned i = 0; i < V / 2; ++i) {
-          constexpr unsigned A = P == 2 ? 1 : 2;
-          const unsigned t = i / A, k = i % A, tok = ln.token(t, k, q);
-          if (tok >= a.tokens || (COLS < 8 && (2 * q + k) / COLS)) continue;
-          float v = acc[(2 * t + h) * A + k];
-          if (TYPE == kMXFP4) v *= f;
-          if (a.y_bf16) {
-            const __nv_bfloat16 o = __float2bfloat16_rn(v);
-            v = __bfloat162float(o);
-            static_cast<__nv_bfloat16*>(a.y)[tok * a.y_stride + row] = o;
-          } else {
-            static_cast<float*>(a.y)[tok * a.y_stride + row] = v;
-          }
-          bad |= !isfinite(v);
-        }
+        for (unsigned i = 0; i < V; ++i) mine[32 * i] = acc[i];
       }
+    }
+    __syncthreads();
+    if (s && l0 < l1 && began) {
+      const unsigned end = (tile - t0 + 1) * count;
+      for (unsigned w = warp + 1; w < W && share(w) < end; ++w) {
+        const float* p = sh.part + w * V * 32 + lane;
+        if (share(w) < share(w + 1))
+#pragma unroll
+          for (unsigned i = 0; i < V; ++i) acc[i] += p[32 * i];
+      }
+      finish(tile);
+    }
+    if (a.cluster > 1) {
+      if (!count) {  // a CTA past the end of K
+        for (unsigned i = threadIdx.x; i < (t1 - t0) * V * 32; i += 32 * W) sh.part[W * V * 32 + i] = 0.0f;
+      }
+      mv_cluster_sync();
+      for (unsigned t = t0 + rank + a.cluster * warp; t < t1; t += a.cluster * W) {  // the CTAs share the tiles
+#pragma unroll
+        for (unsigned i = 0; i < V; ++i) acc[i] = 0.0f;
+        for (unsigned r = 0; r < a.cluster; ++r) {
+          uint32_t from;
+          asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(smem_u32(tiles + (t - t0) * V * 32)), "r"(r));
+#pragma unroll
+          for (unsigned i = 0; i < V; ++i) {
+            float v;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(from + 128 * i) : "memory");
+            acc[i] += v;
+          }
+        }
+        bad |= mv_store<TYPE, P, NT, COLS>(a, ln, t, lane, acc);
+      }
+      mv_cluster_sync();  // no CTA leaves while another reads its shared memory
     }
   }
   if (bad) atomicOr(a.status, kStNumeric);
@@ -615,60 +714,67 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 1) matvec_kernel(const Ma
 // ------------------------------------------------------------ host side
 
 struct MvPlan {
-  unsigned warps, slice, chunk, split, cluster, grid, smem;
+  unsigned warps, slice, chunk, cluster, grid, smem, share;
 };
 
-constexpr unsigned kMvSmemSm = 228 * 1024, kMvSmemCta = 227 * 1024;
+constexpr unsigned kMvDepth = 2, kMvSmemSm = 228 * 1024, kMvSmemCta = 227 * 1024;
 
-// Shared memory of a CTA; the parts only where warps or CTAs share tiles.
-inline size_t mv_smem(unsigned type, unsigned nt, unsigned tokens, unsigned values, unsigned warps, unsigned chunk, bool part) {
-  return static_cast<size_t>(chunk) * (nt * (4096 + (type == FRC_Q4_K ? 256 : 0)) + 4 * tokens) +
-         (part ? static_cast<size_t>(warps) * values * 128 : 0);
+// Shared memory of a CTA with `tiles` results kept (in a cluster).
+inline size_t mv_smem(unsigned type, unsigned nt, unsigned tokens, unsigned values, unsigned warps, unsigned chunk,
+                      unsigned tiles) {
+  const unsigned scale = type == FRC_Q4_K ? 256 : 128;
+  return static_cast<size_t>(warps) * kMvDepth * (2048 + scale) +
+         static_cast<size_t>(chunk) * (nt * (4096 + (type == FRC_Q4_K ? 256 : 0)) + 4 * tokens) +
+         (static_cast<size_t>(warps) + tiles) * values * 128;
 }
+inline unsigned mv_ceil(unsigned a, unsigned b) { return (a + b - 1) / b; }
 
-// Chooses the warps a CTA, the CTAs that share K and the warps that share a
-// tile by an estimate of the time in steps of one span a warp (about 0.3 us):
-// the preparation of x (a batch of spans a warp, three steps), the rounds of
-// tiles, and four steps for a cluster's exchange.
+// Chooses the warps a CTA and the CTAs that share K by an estimate of the
+// time in us, fitted to sweeps over both: a span takes a warp 0.06 us (times
+// `heavy`, for the columns) for each warp of its SM, at least 0.4; preparing
+// x a microsecond a batch of spans a warp, a cluster's exchange 1.5.
 inline MvPlan mv_plan(unsigned type, unsigned P, unsigned nt, unsigned tokens, const MvLayout& l, unsigned sms) {
   const unsigned values = nt * (P == 2 ? 2 : 4), batch = P == 2 ? 4 : 8;
+  const double heavy = nt == 1 ? 1.0 : nt == 2 ? 1.5 : 2.3;
   MvPlan best{};
   double least = 1e30;
   for (unsigned warps = 8; warps <= 16; warps *= 2) {
+    const size_t limit = warps == 8 ? (kMvSmemSm - 2048) / 2 : kMvSmemCta;
     for (unsigned cluster = 1; cluster <= 8 && cluster <= l.spans; cluster *= 2) {
+      // clusters of more than two do not tile the SMs of every GPC
+      const unsigned resident = sms * (warps == 8 ? 2 : 1) / cluster * (cluster > 2 ? 7 : 8) / 8;
+      if (!resident) continue;
       MvPlan p{};
       p.warps = warps;
       p.cluster = cluster;
-      p.slice = p.chunk = (l.spans + cluster - 1) / cluster;
-      const size_t limit = warps == 8 ? (kMvSmemSm - 2048) / 2 : kMvSmemCta;
-      if (warps == 8 && mv_smem(type, nt, tokens, values, warps, p.chunk, true) > limit) continue;
-      while (mv_smem(type, nt, tokens, values, warps, p.chunk, true) > limit) p.chunk = (p.chunk + 1) / 2;
-      // clusters do not tile the SMs of every GPC
-      const unsigned resident = sms * (warps == 8 ? 2 : 1) / cluster * (cluster > 1 ? 7 : 8) / 8;
-      if (!resident) continue;
-      for (unsigned split = 1; split <= warps && (split == 1 || split / 2 < p.chunk); split *= 2) {
-        const unsigned per = warps / split, groups = (l.tiles + per - 1) / per, rounds = (groups + resident - 1) / resident;
-        const unsigned steps = (p.chunk + split - 1) / split * ((p.slice + p.chunk - 1) / p.chunk);
-        const double prep = 3.0 * ((tokens * p.chunk + warps * batch - 1) / (warps * batch)) * (p.chunk < p.slice ? rounds * ((p.slice + p.chunk - 1) / p.chunk) : 1);
-        const double t = prep + static_cast<double>(rounds) * (steps + (split > 1 ? 0.5 : 0.1) + (cluster > 1 ? 4 : 0));
-        if (t < least * 0.98) {
-          least = t;
-          best = p;
-          best.split = split;
-          best.grid = (groups < resident ? groups : resident) * cluster;
-        }
+      p.slice = p.chunk = mv_ceil(l.spans, cluster);
+      const unsigned groups = l.tiles < resident ? l.tiles : resident, tiles = mv_ceil(l.tiles, groups);
+      const unsigned kept = cluster > 1 ? tiles : 0;
+      if (mv_smem(type, nt, tokens, values, warps, p.chunk, kept) > limit) {
+        if (cluster > 1 || warps == 8) continue;
+        while (mv_smem(type, nt, tokens, values, warps, p.chunk, kept) > limit) p.chunk = mv_ceil(p.chunk, 2);
+      }
+      p.grid = groups * cluster;
+      p.smem = static_cast<unsigned>(mv_smem(type, nt, tokens, values, warps, p.chunk, kept));
+      const unsigned steps = mv_ceil(tiles * p.slice, warps), busy = warps * mv_ceil(p.grid, sms);
+      const double step = 0.06 * busy * heavy > 0.4 ? 0.06 * busy * heavy : 0.4;
+      double t = step * steps + 1.0 * mv_ceil(tokens * p.chunk, warps * batch) + (cluster > 1 ? 1.5 : 0.0);
+      if (p.chunk < p.slice) t += (step + 1.5 * mv_ceil(tokens * p.chunk, warps * batch)) * mv_ceil(tiles, warps) * mv_ceil(p.slice, p.chunk);
+      p.share = steps >= 6;
+      if (t < least * 0.98) {
+        least = t;
+        best = p;
       }
     }
   }
-  best.smem = static_cast<unsigned>(mv_smem(type, nt, tokens, values, best.warps, best.chunk, best.split > 1 || best.cluster > 1));
   return best;
 }
 
 template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS, unsigned W>
 inline cudaError_t mv_launch(const MatvecParams& a, const MvPlan& p, cudaStream_t s) {
   if (p.smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(matvec_kernel<TYPE, P, NT, COLS, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(p.smem));
+    const cudaError_t e = cudaFuncSetAttribute(matvec_kernel<TYPE, P, NT, COLS, W, kMvDepth>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(p.smem));
     if (e != cudaSuccess) return e;
   }
   cudaLaunchAttribute at{};
@@ -682,7 +788,7 @@ inline cudaError_t mv_launch(const MatvecParams& a, const MvPlan& p, cudaStream_
   cfg.stream = s;
   cfg.attrs = &at;
   cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, matvec_kernel<TYPE, P, NT, COLS, W>, a);
+  return cudaLaunchKernelEx(&cfg, matvec_kernel<TYPE, P, NT, COLS, W, kMvDepth>, a);
 }
 template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS>
 inline cudaError_t mv_launch_w(const MatvecParams& a, const MvPlan& p, cudaStream_t s) {
@@ -694,31 +800,35 @@ inline cudaError_t launch_matvec(MatvecParams& a, const MvLayout& l, unsigned x_
   const unsigned P = x_type == FRC_F32 ? 2 : 1, cols = a.tokens * P, nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
   MvPlan p = mv_plan(TYPE, P, nt, a.tokens, l, sms);
 #ifdef MV_ENV
-  if (const char* e = getenv("MV_PLAN")) {  // warps,cluster,split,grid groups per resident
-    unsigned w, c, sp;
-    if (sscanf(e, "%u,%u,%u", &w, &c, &sp) == 3) {
+  if (const char* e = getenv("MV_PLAN")) {  // warps,cluster,share
+    unsigned w, c, shr;
+    if (sscanf(e, "%u,%u,%u", &w, &c, &shr) == 3) {
       const unsigned values = nt * (P == 2 ? 2 : 4);
-      p.warps = w; p.cluster = c; p.split = sp; p.slice = p.chunk = (l.spans + c - 1) / c;
-      while (mv_smem(TYPE, nt, a.tokens, values, w, p.chunk, true) > (w == 8 ? (kMvSmemSm - 2048) / 2 : kMvSmemCta)) p.chunk = (p.chunk + 1) / 2;
-      const unsigned per = w / sp, groups = (l.tiles + per - 1) / per, resident = sms * (w == 8 ? 2 : 1) / c * (c > 1 ? 7 : 8) / 8;
-      p.grid = (groups < resident ? groups : resident) * c;
-      p.smem = mv_smem(TYPE, nt, a.tokens, values, w, p.chunk, sp > 1 || c > 1);
+      p.share = shr;
+      p.warps = w; p.cluster = c; p.slice = p.chunk = (l.spans + c - 1) / c;
+      const unsigned resident = sms * (w == 8 ? 2 : 1) / c * (c > 2 ? 7 : 8) / 8, groups = l.tiles < resident ? l.tiles : resident;
+      const unsigned kept = c > 1 ? mv_ceil(l.tiles, groups) : 0;
+      const size_t lim = w == 8 ? (kMvSmemSm - 2048) / 2 : kMvSmemCta;
+      if (mv_smem(TYPE, nt, a.tokens, values, w, p.chunk, kept) > lim) return cudaErrorInvalidValue;
+      p.grid = groups * c;
+      p.smem = mv_smem(TYPE, nt, a.tokens, values, w, p.chunk, kept);
     }
-    fprintf(stderr, "plan warps %u cluster %u split %u slice %u chunk %u grid %u smem %u\n", p.warps, p.cluster, p.split, p.slice, p.chunk, p.grid, p.smem);
+    static MvPlan shown{};
+    if (e[0] == 'p' && memcmp(&shown, &p, sizeof p)) { shown = p; fprintf(stderr, "plan warps %u cluster %u slice %u chunk %u grid %u smem %u share %u\n", p.warps, p.cluster, p.slice, p.chunk, p.grid, p.smem, p.share); }
   }
 #endif
   a.tile_bytes = l.tile_bytes; a.base_at = l.base_at; a.tiles = l.tiles; a.spans = l.spans; a.pieces_last = l.pieces_last;
-  a.slice = p.slice; a.chunk = p.chunk; a.split = p.split; a.cluster = p.cluster;
+  a.slice = p.slice; a.chunk = p.chunk; a.cluster = p.cluster;
   if (P == 2) {
-    if (cols <= 2) return mv_launch_w<TYPE, 2, 1, 2>(a, p, s);
-    if (cols <= 4) return mv_launch_w<TYPE, 2, 1, 4>(a, p, s);
+    if (cols <= 2 && p.share) return mv_launch_w<TYPE, 2, 1, 2>(a, p, s);
+    if (cols <= 4 && p.share) return mv_launch_w<TYPE, 2, 1, 4>(a, p, s);
     if (nt == 1) return mv_launch_w<TYPE, 2, 1, 8>(a, p, s);
     if (nt == 2) return mv_launch_w<TYPE, 2, 2, 8>(a, p, s);
     return mv_launch_w<TYPE, 2, 4, 8>(a, p, s);
   }
-  if (cols <= 1) return mv_launch_w<TYPE, 1, 1, 1>(a, p, s);
-  if (cols <= 2) return mv_launch_w<TYPE, 1, 1, 2>(a, p, s);
-  if (cols <= 4) return mv_launch_w<TYPE, 1, 1, 4>(a, p, s);
+  if (cols <= 1 && p.share) return mv_launch_w<TYPE, 1, 1, 1>(a, p, s);
+  if (cols <= 2 && p.share) return mv_launch_w<TYPE, 1, 1, 2>(a, p, s);
+  if (cols <= 4 && p.share) return mv_launch_w<TYPE, 1, 1, 4>(a, p, s);
   if (nt == 1) return mv_launch_w<TYPE, 1, 1, 8>(a, p, s);
   return mv_launch_w<TYPE, 1, 2, 8>(a, p, s);
 }

@@ -77,6 +77,19 @@ def test_shapes(ctx, type_, rows, n, tokens):
         check(host(y), host(xd), w, a, n, y_type)
 
 
+@pytest.mark.parametrize("type_", [fb.Q4_K, fb.MXFP4])
+@pytest.mark.parametrize("tokens,x_type", [(1, fb.F32), (4, fb.BF16), (16, fb.F32)])
+def test_long_rows(ctx, type_, tokens, x_type):
+    """The longest rows: the vectors do not fit a CTA's shared memory as a whole."""
+    n, rows = 65536 - (0 if type_ == fb.Q4_K else 96), 300
+    rng = np.random.default_rng(tokens)
+    raw = quant.random_rows(type_, rows, n, rng)
+    w, a = quant.weights(type_, raw, n)
+    xd = to_device(rng.standard_normal((tokens, n)), x_type)
+    y = run(ctx, type_, raw, n, xd, x_type, fb.F32)
+    check(host(y), host(xd), w, a, n, fb.F32)
+
+
 @pytest.mark.parametrize("type_,rows", [(fb.Q4_K, 70001), (fb.MXFP4, 65537)])
 def test_many_rows(ctx, type_, rows):
     """More row tiles than the GPU holds at a time."""
