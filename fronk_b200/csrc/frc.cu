@@ -1850,6 +1850,7 @@ int frc_matvec_device(frc_context* c, const frc_matrix* m, unsigned tokens, cons
   a.w = m->data; a.x = x; a.y = y; a.x_stride = x_stride; a.y_stride = y_stride;
   a.rows = m->rows; a.n = m->n; a.tokens = tokens;
   a.x_vec = aligned_to(x, 16) && (tokens == 1 || x_stride * type_size(x_type) % 16 == 0);
+  a.x_bf16 = x_type == FRC_BF16;
   a.y_bf16 = y_type == FRC_BF16;
   a.status = c->status;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);

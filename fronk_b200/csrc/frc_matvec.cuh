@@ -6,20 +6,26 @@
 //
 // The weights' bytes bound it, so the work per weight has to stay under the
 // ~1.5 integer and ~3 other lane operations that one weight may cost at the
-// HBM rate (43 weights a clock and SM).  Both formats are exact in fp16, so a
-// warp multiplies 16 rows x 256 columns ("a span of a tile") on the tensor
-// cores (m16n8k16, fp32 accumulators) with the vectors as the eight columns:
-//   Q4_K: nibble pairs masked out of a word are fp16 subnormals q 2^-24; one
-//     half2 product by sc makes q sc 2^-24 (10 bits, exact), so a whole span
-//     accumulates without touching the scales, and the minima are one more
-//     product, of mi with the sums of x over each 32.
-//   MXFP4: the hardware's E2M1 -> fp16 conversion, and per 32 weights one fma
-//     with 2^(e - base), base the row's largest exponent.
-// x is scaled by a power of two per span (largest value in [2^13, 2^14)) and
-// held in fp16: a bf16 value fits (P = 1), an fp32 value is the sum of two
-// (P = 2; 22 of its 24 bits, or 2^-34 of the span's largest value where that
-// is more: half a step of an fp16 hi, then of an fp16 lo part).  The two parts
-// are columns of their own.
+// HBM rate (43 weights a clock and SM).  A warp multiplies 16 rows x 256
+// columns ("a span of a tile") on the tensor cores by mma.sync, with the
+// vectors as the eight columns.  x is scaled by a power of two per span.
+//   Q4_K, one or two tokens: in integers.  The nibbles are the bytes of a u8
+//     operand after one mask each; x is held as four signed base-256 digits
+//     (32 bits under the span's largest value), a column each; the 6-bit
+//     scales multiply the int32 sums of each 32, so a span is exact.
+//   Q4_K, more tokens: in fp16, which holds q sc exactly (10 bits): masked
+//     nibbles are made 1024 + q and one half2 operation takes the 1024 off
+//     (and multiplies by sc where that saves work on the results).
+//   MXFP4: in fp16, by the hardware's E2M1 conversion, and per 32 weights one
+//     fma with 2^(e - base), base the row's largest exponent.
+//   In fp16 a bf16 x fits one value (P = 1); an fp32 x is the sum of two, hi
+//     and lo, a column each (P = 2): 22 of its 24 bits, or 2^-34 of the span's
+//     largest value where that is more.
+//   The minima of Q4_K are one more fp16 product, of mi with the sums of x
+//     over each 32 (hi and lo parts along K).
+// (fp16 subnormals as operands would save the half2 operations, but mma.sync
+// aligns its sums by the operands' exponents: measured, q 2^-24 costs 20 times
+// the rounding error.)
 #pragma once
 #include <cuda_bf16.h>
 
@@ -35,7 +41,8 @@ constexpr unsigned kMvTile = 16;           // rows of one step
 // rows), in it span after span of [scales][pieces], a piece being 64 weights
 // of the 16 rows: lane (g = lane / 4, q = lane % 4) owns 16 bytes {row g
 // group 0, row g + 8 group 0, row g group 1, row g + 8 group 1}, a word of
-// eight weights 32 group + 8 q + 0..7 each, so that a load is the fragment.
+// eight weights 32 group + 8 q + 0..7 each, so that a load is the fragment
+// (Q4_K: 0..3 in the low nibbles of its bytes, 4..7 in the high ones).
 // The last span stops at the last piece that holds weights.
 //   Q4_K scales: the 16 header bytes of each row (d, dmin, packed 6 bits).
 //   MXFP4 scales: 8 exponents a row, relative to the row's largest (127 is
@@ -109,8 +116,7 @@ __global__ void __launch_bounds__(256) matrix_layout_kernel(const uint8_t* __res
         if (TYPE == kQ4K) {
           const uint8_t* q = b + 144 * s + 16 + 32 * (grp / 2) + k0;
 #pragma unroll
-          for (unsigned j = 0; j < 8; ++j)  // pair j / 2: its two weights in the word's halves
-            v |= (q[j] >> (4 * (grp & 1)) & 15u) << (4 * (j / 2) + 16 * (j & 1));
+          for (unsigned j = 0; j < 8; ++j) v |= (q[j] >> (4 * (grp & 1)) & 15u) << (8 * (j % 4) + 4 * (j / 4));
         } else {
           const uint8_t* q = b + 17 * (8 * s + grp) + 1 + (k0 & 8);
 #pragma unroll
@@ -133,7 +139,7 @@ struct MatvecParams {
   unsigned slice;             // spans of K a CTA works on (all, or a share where a cluster splits K)
   unsigned chunk;             // spans of x in shared memory at a time, at most the slice
   unsigned cluster;           // CTAs that share K
-  unsigned x_vec, y_bf16;     // x rows are 16-byte aligned; y is bf16
+  unsigned x_vec, x_bf16, y_bf16;  // x rows are 16-byte aligned; x, y are bf16
   unsigned* status;
 };
 
@@ -151,6 +157,25 @@ __device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// m16n8k32, unsigned by signed bytes, int32 accumulators.
+__device__ __forceinline__ void mma_u8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1, bool first) {
+  if (first)
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
 }
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -222,7 +247,8 @@ struct MvFrag {
 };
 
 // The vectors of one K chunk in shared memory, as the products' B fragments:
-// per span and group of 32 a block of 8 NT columns of 64 bytes.
+// per span and group of 32 a block of 8 NT columns of 64 bytes (32 for the
+// digits of P = 4).
 //
 // With few columns (COLS = 1, 2, 4: tokens x parts, rounded up) the eight of
 // a product are shared by 8 / COLS groups: the block of group i holds its
@@ -243,7 +269,8 @@ struct MvShared {
 // (token, span) at a time with the values of U of them on their way.
 template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS>
 __device__ __forceinline__ void mv_prepare(const MatvecParams& a, const MvShared& sh, unsigned first, unsigned count) {
-  constexpr unsigned U = P == 2 ? 4 : 8, R = P == 2 ? 8 : 4;
+  constexpr unsigned U = P == 1 ? 8 : 4, R = P == 1 ? 4 : 8;
+  const bool bf16 = P == 1 || (P == 4 && a.x_bf16);
   const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = blockDim.x / 32, units = a.tokens * count;
   for (unsigned u0 = warp; u0 < units; u0 += U * warps) {
     uint32_t raw[U][R];
@@ -253,7 +280,7 @@ __device__ __forceinline__ void mv_prepare(const MatvecParams& a, const MvShared
 #pragma unroll
       for (unsigned j = 0; j < R; ++j) raw[i][j] = 0;
       if (u >= units || k >= a.n) continue;
-      if (P == 2) {
+      if (!bf16) {
         const float* x = static_cast<const float*>(a.x) + t * a.x_stride + k;
         if (a.x_vec) {
           const uint4 p = reinterpret_cast<const uint4*>(x)[0], q = reinterpret_cast<const uint4*>(x)[1];
@@ -281,41 +308,59 @@ __device__ __forceinline__ void mv_prepare(const MatvecParams& a, const MvShared
       float v[8];
 #pragma unroll
       for (unsigned j = 0; j < 8; ++j)
-        v[j] = __uint_as_float(P == 2 ? raw[i][j % R] : j & 1 ? raw[i][j / 2] & 0xffff0000u : raw[i][j / 2] << 16);
+        v[j] = __uint_as_float(!bf16 ? raw[i][j % R] : j & 1 ? raw[i][j / 2] & 0xffff0000u : raw[i][j / 2] << 16);
       unsigned top = 0;
 #pragma unroll
       for (unsigned j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
       top = __reduce_max_sync(0xffffffffu, top);
-      // x = v 2^ex; a span that is not finite has the scale NaN and so its results
-      int ex = static_cast<int>(top >> 23) - 127 - 13;
+      // x = v 2^ex, the largest |v| in [2^13, 2^14), or [2^29, 2^30) as digits; a span that is not finite has the
+      // scale NaN and so its results
+      constexpr int TOP = P == 4 ? 29 : 13;
+      int ex = static_cast<int>(top >> 23) - 127 - TOP;
       if (ex < -126) ex = -126;
       const bool finite = top < 0x7f800000u;
-      const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-      float sum = 0.0f;
-      uint32_t hi[4], lo[4];
+      const float inv = finite ? __uint_as_float(static_cast<uint32_t>(127 - ex) << 23) : 0.0f;
 #pragma unroll
-      for (unsigned j = 0; j < 4; ++j) {
-        // odd pairs of a Q4_K word carry 16 q
-        const float f = TYPE == kQ4K && (j & 1) ? 0.0625f : 1.0f;
-        float p = finite ? v[2 * j] * inv : 0.0f, q = finite ? v[2 * j + 1] * inv : 0.0f;
-        sum += p + q;
-        p *= f;
-        q *= f;
-        const __half2 h = __floats2half2_rn(p, q);
-        hi[j] = *reinterpret_cast<const uint32_t*>(&h);
-        const float2 b = __half22float2(h);
-        const __half2 l = __floats2half2_rn(p - b.x, q - b.y);
-        lo[j] = *reinterpret_cast<const uint32_t*>(&l);
-      }
+      for (unsigned j = 0; j < 8; ++j) v[j] = finite ? v[j] * inv : 0.0f;
+      const float sum8 = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
       const unsigned grp = lane / 4, c0 = COLS < 8 ? (grp % (8 / COLS)) * COLS + t * P : t * P;
-      uint8_t* c = sh.col + ((s * 8 + grp) * NT + c0 / 8) * 512 + c0 % 8 * 64 + 16 * (lane % 4);
-      *reinterpret_cast<uint4*>(c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      if (P == 2) *reinterpret_cast<uint4*>(c + 64) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      if (P == 4) {
+        // signed digits: with 128 added to the three low bytes they are the bytes less 128
+        uint32_t w[8];
+#pragma unroll
+        for (unsigned j = 0; j < 8; ++j) w[j] = (static_cast<uint32_t>(__float2int_rn(v[j])) + 0x00808080u) ^ 0x00808080u;
+        uint8_t* c = sh.col + (s * 8 + grp) * 256 + c0 * 32 + 8 * (lane % 4);
+#pragma unroll
+        for (unsigned d = 0; d < 4; ++d) {
+          const uint32_t sel = d | (4 + d) << 4;
+          const uint32_t lo = prmt(prmt(w[0], w[1], sel), prmt(w[2], w[3], sel), 0x5410);
+          const uint32_t hi = prmt(prmt(w[4], w[5], sel), prmt(w[6], w[7], sel), 0x5410);
+          *reinterpret_cast<uint2*>(c + 32 * d) = make_uint2(lo, hi);
+        }
+      } else {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (unsigned j = 0; j < 4; ++j) {
+          // a Q4_K word gives the pairs 0 2, 4 6, 1 3, 5 7, of them 4..7 as 16 q
+          const float f = TYPE == kQ4K && (j & 1) ? 0.0625f : 1.0f;
+          const unsigned e0 = TYPE == kQ4K ? 4 * (j & 1) + j / 2 : 2 * j, e1 = TYPE == kQ4K ? e0 + 2 : e0 + 1;
+          const float p = v[e0] * f, q = v[e1] * f;
+          const __half2 h = __floats2half2_rn(p, q);
+          hi[j] = *reinterpret_cast<const uint32_t*>(&h);
+          const float2 b = __half22float2(h);
+          const __half2 l = __floats2half2_rn(p - b.x, q - b.y);
+          lo[j] = *reinterpret_cast<const uint32_t*>(&l);
+        }
+        uint8_t* c = sh.col + ((s * 8 + grp) * NT + c0 / 8) * 512 + c0 % 8 * 64 + 16 * (lane % 4);
+        *reinterpret_cast<uint4*>(c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (P == 2) *reinterpret_cast<uint4*>(c + 64) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
       if (lane == 0) sh.scale[t * a.chunk + s] = finite ? __uint_as_float(static_cast<uint32_t>(127 + ex) << 23) : NAN;
       if (TYPE == kQ4K) {
+        float sum = sum8;
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        sum *= 0.03125f;
+        sum *= P == 4 ? 0x1p-21f : 0x1p-5f;  // fits fp16
         if (lane % 4 == 0) {
           const __half h = __float2half_rn(sum), l = __float2half_rn(sum - __half2float(h));
           __half* o = reinterpret_cast<__half*>(sh.sums + (s * NT * 8 + t * P) * 32) + grp;
@@ -331,20 +376,24 @@ __device__ __forceinline__ void mv_prepare(const MatvecParams& a, const MvShared
 // and, where groups share columns, which group's results it holds.
 template <unsigned P, unsigned NT, unsigned COLS>
 struct MvLane {
-  static constexpr unsigned kTok = P == 2 || COLS == 1 ? 1 : 2;  // tokens of a lane's results in eight columns
+  static constexpr unsigned kTok = P >= 2 || COLS == 1 ? 1 : 2;  // tokens of a lane's results in eight columns
   uint32_t col, sums, scale[NT][kTok];
   unsigned sel;      // bytes 2 q and 2 q + 1
   unsigned mine[2];  // byte of the scale of the lane's first and second column, for a group set that starts at byte 0
   __device__ __forceinline__ unsigned token(unsigned t, unsigned k, unsigned q) const {
-    if (COLS == 8) return P == 2 ? 4 * t + q : 8 * t + 2 * q + k;
+    if (COLS == 8) return P == 4 ? q / 2 : P == 2 ? 4 * t + q : 8 * t + 2 * q + k;
     return ((2 * q + k) % COLS) / P;
+  }
+  // Whether the lane has its column's results when the lanes have been joined.
+  __device__ __forceinline__ bool holds(unsigned k, unsigned q) const {
+    return (COLS == 8 || (2 * q + k) / COLS == 0) && (P != 4 || q % 2 == 0);
   }
   __device__ __forceinline__ MvLane(const MatvecParams& a, const MvShared& sh, unsigned lane) {
     const unsigned g = lane / 4, q = lane % 4;
     sel = 2 * q | (2 * q + 1) << 4;
     mine[0] = 2 * q / COLS;
     mine[1] = (2 * q + 1) / COLS;
-    col = smem_u32(sh.col) + 64 * g + 16 * q;
+    col = smem_u32(sh.col) + (P == 4 ? 32 * g + 8 * q : 64 * g + 16 * q);
     sums = smem_u32(sh.sums) + 32 * g + 4 * q;
 #pragma unroll
     for (unsigned t = 0; t < NT; ++t)
@@ -356,15 +405,16 @@ struct MvLane {
   }
 };
 
-// The fp16 operands of 32 columns of a tile from a lane's words (row g and row g + 8).
+// The fp16 operands of 32 columns of a tile from a lane's word of one row: for
+// Q4_K 1024 + q (pairs 0, 2) and 1024 + 16 q (pairs 1, 3).
 template <unsigned TYPE>
 __device__ __forceinline__ void mv_weights(uint32_t w, uint32_t (&av)[4]) {
   if (TYPE == kQ4K) {
     const uint32_t u = w >> 8;
-    av[0] = w & 0x000f000fu;
-    av[1] = w & 0x00f000f0u;
-    av[2] = u & 0x000f000fu;
-    av[3] = u & 0x00f000f0u;
+    av[0] = (w & 0x000f000fu) | 0x64006400u;
+    av[1] = (w & 0x00f000f0u) | 0x64006400u;
+    av[2] = (u & 0x000f000fu) | 0x64006400u;
+    av[3] = (u & 0x00f000f0u) | 0x64006400u;
   } else {
     e2m1_f16(w, av);
   }
@@ -384,40 +434,82 @@ __device__ __forceinline__ float mv_scale_at(const uint32_t (&b)[2], unsigned at
   return __uint_as_float((at % 4 == 3 ? v >> 1 : v << (23 - 8 * (at % 4))) & 0x7f800000u);
 }
 
+// The header of a Q4_K row's super-block: d, -dmin, the eight 6-bit scales and
+// minima as bytes.
+__device__ __forceinline__ void mv_header(uint4 b, float& d, float& dm, uint32_t (&sc)[2], uint32_t (&mi)[2]) {
+  d = h2f(b.x & 0xffffu);
+  dm = -h2f(b.x >> 16);
+  sc[0] = b.y & 0x3f3f3f3fu;
+  mi[0] = b.z & 0x3f3f3f3fu;
+  sc[1] = (b.w & 0x0f0f0f0fu) | (b.y >> 2 & 0x30303030u);
+  mi[1] = (b.w >> 4 & 0x0f0f0f0fu) | (b.z >> 2 & 0x30303030u);
+}
+// Minima of groups 2 q and 2 q + 1 of a row as fp16 (sel: their bytes).
+__device__ __forceinline__ uint32_t mv_minima(const uint32_t (&mi)[2], unsigned sel) {
+  return hsub2(prmt(prmt(mi[0], mi[1], sel), 0x64646464u, 0x4140u), 0x64006400u);
+}
+
 // One span (s of the chunk) of a tile times the columns; acc: [row g | row
 // g + 8] of the lane's columns' tokens in each eight columns (the sum of both
-// columns for P = 2).  The 6-bit scales of Q4_K go onto the results, or with
-// NT = 4 (where that is more work) into the weights by half2 products.
+// columns for P = 2).  The 6-bit scales of Q4_K go onto the results of each
+// 32, or for several groups of columns (where that is more work) into the
+// weights.
 template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS>
 __device__ __forceinline__ void mv_span(const MvLane<P, NT, COLS>& ln, const MvFrag<TYPE>& f, unsigned s,
-                                        float (&acc)[NT * (P == 2 ? 2 : 4)]) {
-  constexpr bool FOLD = TYPE == kQ4K && NT > 2;
+                                        float (&acc)[NT * (P >= 2 ? 2 : 4)]) {
+  constexpr bool FOLD = TYPE == kQ4K && NT > 1;
   constexpr unsigned SHARE = 8 / COLS;  // groups in one accumulator
-  const uint32_t xc = ln.col + 4096 * NT * s;
   uint32_t sc[2][2];  // eight scale bytes of rows g and g + 8
   float d[2], dm[2], m[NT][4];
   if constexpr (TYPE == kQ4K) {
     uint32_t mi[2][2];
-#pragma unroll
-    for (unsigned h = 0; h < 2; ++h) {
-      const uint4 b = f.s[h];
-      d[h] = h2f(b.x & 0xffffu) * 16777216.0f;   // against q sc 2^-24
-      dm[h] = h2f(b.x >> 16) * -536870912.0f;    // against mi 2^-24 and sums 2^-5
-      sc[h][0] = b.y & 0x3f3f3f3fu;
-      mi[h][0] = b.z & 0x3f3f3f3fu;
-      sc[h][1] = (b.w & 0x0f0f0f0fu) | (b.y >> 2 & 0x30303030u);
-      mi[h][1] = (b.w >> 4 & 0x0f0f0f0fu) | (b.z >> 2 & 0x30303030u);
-    }
-    // minima of groups 2 q and 2 q + 1 as fp16 subnormals mi 2^-24, against the sums' hi and lo parts
-    const uint32_t m0 = prmt(prmt(mi[0][0], mi[0][1], ln.sel), 0, 0x4140), m1 = prmt(prmt(mi[1][0], mi[1][1], ln.sel), 0, 0x4140);
+    mv_header(f.s[0], d[0], dm[0], sc[0], mi[0]);
+    mv_header(f.s[TYPE == kQ4K ? 1 : 0], d[1], dm[1], sc[1], mi[1]);
+    const uint32_t m0 = mv_minima(mi[0], ln.sel), m1 = mv_minima(mi[1], ln.sel);
 #pragma unroll
     for (unsigned t = 0; t < NT; ++t) {
       const uint32_t at = ln.sums + 256 * (NT * s + t);
       mma_f16_first(m[t], m0, m1, m0, m1, lds32(at), lds32(at + 16));
     }
+    // the sums were scaled down
+    dm[0] *= P == 4 ? 0x1p21f : 0x1p5f;
+    dm[1] *= P == 4 ? 0x1p21f : 0x1p5f;
   } else {
     sc[0][0] = f.s[0].x; sc[0][1] = f.s[0].y; sc[1][0] = f.s[0].z; sc[1][1] = f.s[0].w;
   }
+  if constexpr (P == 4) {
+    const uint32_t xc = ln.col + 2048 * s;
+    int c[4], sum[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (unsigned grp = 0; grp < 8; ++grp) {
+      const uint4 wv = f.w[grp / 2];
+      const uint32_t w0 = grp & 1 ? wv.z : wv.x, w1 = grp & 1 ? wv.w : wv.y;
+      uint32_t b0, b1;
+      asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(b0), "=r"(b1) : "r"(xc + 256 * grp));
+      mma_u8(c, w0 & 0x0f0f0f0fu, w1 & 0x0f0f0f0fu, w0 >> 4 & 0x0f0f0f0fu, w1 >> 4 & 0x0f0f0f0fu, b0, b1, grp % SHARE == 0);
+      if (grp % SHARE == SHARE - 1) {
+        // |c| <= 32 x 15 x 128, times 63, eight times: below 2^25
+#pragma unroll
+        for (unsigned h = 0; h < 2; ++h) {
+          const int k = static_cast<int>(SHARE > 1 ? prmt(prmt(sc[h][0], sc[h][1], grp + 1 - SHARE + ln.mine[0]), 0, 0x4440u)
+                                                   : prmt(sc[h][grp / 4], 0, 0x4440u | grp % 4));
+          sum[2 * h] += c[2 * h] * k;
+          sum[2 * h + 1] += c[2 * h + 1] * k;
+        }
+      }
+    }
+    // two digits of the four: the upper two are 2^16 up
+    const float x = __uint_as_float(lds32(ln.scale[0][0] + 4 * s));
+    const float xd = (threadIdx.x & 1) ? x * 65536.0f : x;
+#pragma unroll
+    for (unsigned h = 0; h < 2; ++h) {
+      const float v = fmaf(static_cast<float>(sum[2 * h + 1]), 256.0f, static_cast<float>(sum[2 * h]));
+      // the sums are in the first digit's column; a span is one term of acc, whichever warps share the tile
+      acc[h] += fmaf(v * d[h], xd, ((threadIdx.x & 1) ? 0.0f : m[0][2 * h] * dm[h]) * x);
+    }
+    return;
+  }
+  const uint32_t xc = ln.col + 4096 * NT * s;
   constexpr unsigned SV = P == 2 && !FOLD ? 2 : 4;
   float sum[NT][SV], c[NT][4];
 #pragma unroll
@@ -431,13 +523,20 @@ __device__ __forceinline__ void mv_span(const MvLane<P, NT, COLS>& ln, const MvF
     mv_weights<TYPE>(grp & 1 ? wv.z : wv.x, a0);
     mv_weights<TYPE>(grp & 1 ? wv.w : wv.y, a1);
     if (FOLD) {
-      // 1024 + sc in both halves, less 1024
+      // sc as 1024 + sc less 1024, and -1024 sc
       const uint32_t sel = 0x4040u | (grp % 4) * 0x0101u;
       const uint32_t k0 = hsub2(prmt(sc[0][grp / 4], 0x64646464u, sel), 0x64006400u), k1 = hsub2(prmt(sc[1][grp / 4], 0x64646464u, sel), 0x64006400u);
+      const uint32_t n0 = hmul2(k0, 0xe400e400u), n1 = hmul2(k1, 0xe400e400u);
 #pragma unroll
       for (unsigned i = 0; i < 4; ++i) {
-        a0[i] = hmul2(a0[i], k0);
-        a1[i] = hmul2(a1[i], k1);
+        a0[i] = hfma2(a0[i], k0, n0);
+        a1[i] = hfma2(a1[i], k1, n1);
+      }
+    } else if (TYPE == kQ4K) {
+#pragma unroll
+      for (unsigned i = 0; i < 4; ++i) {
+        a0[i] = hsub2(a0[i], 0x64006400u);
+        a1[i] = hsub2(a1[i], 0x64006400u);
       }
     }
 #pragma unroll
@@ -490,8 +589,8 @@ __device__ __forceinline__ void mv_cluster_sync() {
 // Stores the results of a tile (acc as mv_span leaves it).
 template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS>
 __device__ __forceinline__ bool mv_store(const MatvecParams& a, const MvLane<P, NT, COLS>& ln, unsigned tile, unsigned lane,
-                                         const float (&acc)[NT * (P == 2 ? 2 : 4)]) {
-  constexpr unsigned V = NT * (P == 2 ? 2 : 4), A = P == 2 ? 1 : 2;
+                                         const float (&acc)[NT * (P >= 2 ? 2 : 4)]) {
+  constexpr unsigned V = NT * (P >= 2 ? 2 : 4), A = P >= 2 ? 1 : 2;
   const unsigned g = lane / 4, q = lane % 4;
   bool bad = false;
 #pragma unroll
@@ -506,7 +605,7 @@ __device__ __forceinline__ bool mv_store(const MatvecParams& a, const MvLane<P, 
 #pragma unroll
     for (unsigned i = 0; i < V / 2; ++i) {
       const unsigned t = i / A, k = i % A, tok = ln.token(t, k, q);
-      if (tok >= a.tokens || (COLS < 8 && (2 * q + k) / COLS)) continue;
+      if (tok >= a.tokens || !ln.holds(k, q)) continue;
       float v = acc[(2 * t + h) * A + k];
       if (TYPE == kMXFP4) v *= f;
       if (a.y_bf16) {
@@ -524,9 +623,9 @@ __device__ __forceinline__ bool mv_store(const MatvecParams& a, const MvLane<P, 
 
 // The lanes that hold groups of the same columns together.
 template <unsigned P, unsigned NT, unsigned COLS>
-__device__ __forceinline__ void mv_join(float (&acc)[NT * (P == 2 ? 2 : 4)]) {
-  constexpr unsigned V = NT * (P == 2 ? 2 : 4);
-  if (COLS == 8) return;
+__device__ __forceinline__ void mv_join(float (&acc)[NT * (P >= 2 ? 2 : 4)]) {
+  constexpr unsigned V = NT * (P >= 2 ? 2 : 4);
+  if (COLS == 8 && P != 4) return;
   if (COLS == 1) {
     acc[0] += acc[1];
     acc[2 % V] += acc[3 % V];
@@ -534,8 +633,8 @@ __device__ __forceinline__ void mv_join(float (&acc)[NT * (P == 2 ? 2 : 4)]) {
 #pragma unroll
   for (unsigned i = 0; i < V; ++i) {
     if (COLS == 1 && (i & 1)) continue;
-    if (COLS <= 2) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 1);
-    acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 2);
+    if (COLS <= 2 || P == 4) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 1);
+    if (COLS < 8) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 2);
   }
 }
 
@@ -548,13 +647,13 @@ __device__ __forceinline__ void mv_join(float (&acc)[NT * (P == 2 ? 2 : 4)]) {
 // x is prepared anew for every W tiles, chunk by chunk.
 template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS, unsigned W, unsigned DEPTH>
 __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 1) matvec_kernel(const MatvecParams a) {
-  constexpr unsigned V = NT * (P == 2 ? 2 : 4), kBytes = MvFrag<TYPE>::kBytes;
+  constexpr unsigned V = NT * (P >= 2 ? 2 : 4), kBytes = MvFrag<TYPE>::kBytes;
   extern __shared__ __align__(128) uint8_t smem[];
   const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   MvShared sh;
   sh.ring = smem;
   sh.col = smem + W * DEPTH * kBytes;
-  sh.sums = sh.col + 4096 * NT * a.chunk;
+  sh.sums = sh.col + (P == 4 ? 2048 : 4096 * NT) * a.chunk;
   sh.scale = reinterpret_cast<float*>(sh.sums + (TYPE == kQ4K ? 256 * NT * a.chunk : 0));
   sh.part = sh.scale + a.tokens * a.chunk;
   const MvLane<P, NT, COLS> ln(a, sh, lane);
@@ -720,11 +819,11 @@ struct MvPlan {
 constexpr unsigned kMvDepth = 2, kMvSmemSm = 228 * 1024, kMvSmemCta = 227 * 1024;
 
 // Shared memory of a CTA with `tiles` results kept (in a cluster).
-inline size_t mv_smem(unsigned type, unsigned nt, unsigned tokens, unsigned values, unsigned warps, unsigned chunk,
-                      unsigned tiles) {
+inline size_t mv_smem(unsigned type, unsigned P, unsigned nt, unsigned tokens, unsigned values, unsigned warps,
+                      unsigned chunk, unsigned tiles) {
   const unsigned scale = type == FRC_Q4_K ? 256 : 128;
   return static_cast<size_t>(warps) * kMvDepth * (2048 + scale) +
-         static_cast<size_t>(chunk) * (nt * (4096 + (type == FRC_Q4_K ? 256 : 0)) + 4 * tokens) +
+         static_cast<size_t>(chunk) * ((P == 4 ? 2048 : 4096 * nt) + (type == FRC_Q4_K ? 256 * nt : 0) + 4 * tokens) +
          (static_cast<size_t>(warps) + tiles) * values * 128;
 }
 inline unsigned mv_ceil(unsigned a, unsigned b) { return (a + b - 1) / b; }
@@ -732,9 +831,11 @@ inline unsigned mv_ceil(unsigned a, unsigned b) { return (a + b - 1) / b; }
 // Chooses the warps a CTA and the CTAs that share K by an estimate of the
 // time in us, fitted to sweeps over both: a span takes a warp 0.06 us (times
 // `heavy`, for the columns) for each warp of its SM, at least 0.4; preparing
-// x a microsecond a batch of spans a warp, a cluster's exchange 1.5.
+// x 0.25 a span and warp, a cluster's exchange 0.5 and 0.02 a tile.  Measured
+// both ways: 5120 x 2560 and 8 tokens 8.7 us with clusters of 4, 10.2 without;
+// 4096 x 8192 and one token 8.6 and 9.8; 513 x 2048 and one token 3.8 and 3.4.
 inline MvPlan mv_plan(unsigned type, unsigned P, unsigned nt, unsigned tokens, const MvLayout& l, unsigned sms) {
-  const unsigned values = nt * (P == 2 ? 2 : 4), batch = P == 2 ? 4 : 8;
+  const unsigned values = nt * (P >= 2 ? 2 : 4);
   const double heavy = nt == 1 ? 1.0 : nt == 2 ? 1.5 : 2.3;
   MvPlan best{};
   double least = 1e30;
@@ -750,16 +851,17 @@ inline MvPlan mv_plan(unsigned type, unsigned P, unsigned nt, unsigned tokens, c
       p.slice = p.chunk = mv_ceil(l.spans, cluster);
       const unsigned groups = l.tiles < resident ? l.tiles : resident, tiles = mv_ceil(l.tiles, groups);
       const unsigned kept = cluster > 1 ? tiles : 0;
-      if (mv_smem(type, nt, tokens, values, warps, p.chunk, kept) > limit) {
+      if (mv_smem(type, P, nt, tokens, values, warps, p.chunk, kept) > limit) {
         if (cluster > 1 || warps == 8) continue;
-        while (mv_smem(type, nt, tokens, values, warps, p.chunk, kept) > limit) p.chunk = mv_ceil(p.chunk, 2);
+        while (mv_smem(type, P, nt, tokens, values, warps, p.chunk, kept) > limit) p.chunk = mv_ceil(p.chunk, 2);
       }
       p.grid = groups * cluster;
-      p.smem = static_cast<unsigned>(mv_smem(type, nt, tokens, values, warps, p.chunk, kept));
+      p.smem = static_cast<unsigned>(mv_smem(type, P, nt, tokens, values, warps, p.chunk, kept));
       const unsigned steps = mv_ceil(tiles * p.slice, warps), busy = warps * mv_ceil(p.grid, sms);
       const double step = 0.06 * busy * heavy > 0.4 ? 0.06 * busy * heavy : 0.4;
-      double t = step * steps + 1.0 * mv_ceil(tokens * p.chunk, warps * batch) + (cluster > 1 ? 1.5 : 0.0);
-      if (p.chunk < p.slice) t += (step + 1.5 * mv_ceil(tokens * p.chunk, warps * batch)) * mv_ceil(tiles, warps) * mv_ceil(p.slice, p.chunk);
+      const double prep = 0.4 + 0.25 * mv_ceil(tokens * p.chunk, warps);
+      double t = step * steps + prep + (cluster > 1 ? 0.5 + 0.02 * tiles : 0.0);
+      if (p.chunk < p.slice) t += (step + prep) * mv_ceil(tiles, warps) * mv_ceil(p.slice, p.chunk);
       p.share = steps >= 6;
       if (t < least * 0.98) {
         least = t;
@@ -797,21 +899,21 @@ inline cudaError_t mv_launch_w(const MatvecParams& a, const MvPlan& p, cudaStrea
 
 template <unsigned TYPE>
 inline cudaError_t launch_matvec(MatvecParams& a, const MvLayout& l, unsigned x_type, unsigned sms, cudaStream_t s) {
-  const unsigned P = x_type == FRC_F32 ? 2 : 1, cols = a.tokens * P, nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
+  const unsigned P = TYPE == kQ4K && a.tokens <= 2 ? 4 : x_type == FRC_F32 ? 2 : 1, cols = a.tokens * P, nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
   MvPlan p = mv_plan(TYPE, P, nt, a.tokens, l, sms);
 #ifdef MV_ENV
   if (const char* e = getenv("MV_PLAN")) {  // warps,cluster,share
     unsigned w, c, shr;
     if (sscanf(e, "%u,%u,%u", &w, &c, &shr) == 3) {
-      const unsigned values = nt * (P == 2 ? 2 : 4);
+      const unsigned values = nt * (P >= 2 ? 2 : 4);
       p.share = shr;
       p.warps = w; p.cluster = c; p.slice = p.chunk = (l.spans + c - 1) / c;
       const unsigned resident = sms * (w == 8 ? 2 : 1) / c * (c > 2 ? 7 : 8) / 8, groups = l.tiles < resident ? l.tiles : resident;
       const unsigned kept = c > 1 ? mv_ceil(l.tiles, groups) : 0;
       const size_t lim = w == 8 ? (kMvSmemSm - 2048) / 2 : kMvSmemCta;
-      if (mv_smem(TYPE, nt, a.tokens, values, w, p.chunk, kept) > lim) return cudaErrorInvalidValue;
+      if (mv_smem(TYPE, P, nt, a.tokens, values, w, p.chunk, kept) > lim) return cudaErrorInvalidValue;
       p.grid = groups * c;
-      p.smem = mv_smem(TYPE, nt, a.tokens, values, w, p.chunk, kept);
+      p.smem = mv_smem(TYPE, P, nt, a.tokens, values, w, p.chunk, kept);
     }
     static MvPlan shown{};
     if (e[0] == 'p' && memcmp(&shown, &p, sizeof p)) { shown = p; fprintf(stderr, "plan warps %u cluster %u slice %u chunk %u grid %u smem %u share %u\n", p.warps, p.cluster, p.slice, p.chunk, p.grid, p.smem, p.share); }
@@ -819,15 +921,19 @@ inline cudaError_t launch_matvec(MatvecParams& a, const MvLayout& l, unsigned x_
 #endif
   a.tile_bytes = l.tile_bytes; a.base_at = l.base_at; a.tiles = l.tiles; a.spans = l.spans; a.pieces_last = l.pieces_last;
   a.slice = p.slice; a.chunk = p.chunk; a.cluster = p.cluster;
+  if constexpr (TYPE == kQ4K) {
+    if (P == 4) return mv_launch_w<TYPE, 4, 1, 8>(a, p, s);
+  } else {
+    if (P == 2 && cols <= 2 && p.share) return mv_launch_w<TYPE, 2, 1, 2>(a, p, s);
+    if (P == 2 && cols <= 4 && p.share) return mv_launch_w<TYPE, 2, 1, 4>(a, p, s);
+    if (P == 1 && cols <= 1 && p.share) return mv_launch_w<TYPE, 1, 1, 1>(a, p, s);
+    if (P == 1 && cols <= 2 && p.share) return mv_launch_w<TYPE, 1, 1, 2>(a, p, s);
+  }
   if (P == 2) {
-    if (cols <= 2 && p.share) return mv_launch_w<TYPE, 2, 1, 2>(a, p, s);
-    if (cols <= 4 && p.share) return mv_launch_w<TYPE, 2, 1, 4>(a, p, s);
     if (nt == 1) return mv_launch_w<TYPE, 2, 1, 8>(a, p, s);
     if (nt == 2) return mv_launch_w<TYPE, 2, 2, 8>(a, p, s);
     return mv_launch_w<TYPE, 2, 4, 8>(a, p, s);
   }
-  if (cols <= 1 && p.share) return mv_launch_w<TYPE, 1, 1, 1>(a, p, s);
-  if (cols <= 2 && p.share) return mv_launch_w<TYPE, 1, 1, 2>(a, p, s);
   if (cols <= 4 && p.share) return mv_launch_w<TYPE, 1, 1, 4>(a, p, s);
   if (nt == 1) return mv_launch_w<TYPE, 1, 1, 8>(a, p, s);
   return mv_launch_w<TYPE, 1, 2, 8>(a, p, s);
