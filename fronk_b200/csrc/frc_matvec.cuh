@@ -9,7 +9,7 @@
 // HBM rate (43 weights a clock and SM).  A warp multiplies 16 rows x 256
 // columns ("a span of a tile") on the tensor cores by mma.sync, with the
 // vectors as the eight columns.  x is scaled by a power of two per span.
-//   Q4_K, one or two tokens: in integers.  The nibbles are the bytes of a u8
+//   Q4_K, up to four tokens: in integers.  The nibbles are the bytes of a u8
 //     operand after one mask each; x is held as four signed base-256 digits
 //     (32 bits under the span's largest value), a column each; the 6-bit
 //     scales multiply the int32 sums of each 32, so a span is exact.
@@ -158,19 +158,12 @@ __device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
-// m16n8k32, unsigned by signed bytes, int32 accumulators.
-__device__ __forceinline__ void mma_u8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                       uint32_t b1, bool first) {
-  if (first)
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// m16n8k32, unsigned by signed bytes, int32: c = a b.
+__device__ __forceinline__ void mma_u8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
@@ -329,7 +322,7 @@ __device__ __forceinline__ void mv_prepare(const MatvecParams& a, const MvShared
         uint32_t w[8];
 #pragma unroll
         for (unsigned j = 0; j < 8; ++j) w[j] = (static_cast<uint32_t>(__float2int_rn(v[j])) + 0x00808080u) ^ 0x00808080u;
-        uint8_t* c = sh.col + (s * 8 + grp) * 256 + c0 * 32 + 8 * (lane % 4);
+        uint8_t* c = sh.col + ((s * 8 + grp) * NT + c0 / 8) * 256 + c0 % 8 * 32 + 8 * (lane % 4);
 #pragma unroll
         for (unsigned d = 0; d < 4; ++d) {
           const uint32_t sel = d | (4 + d) << 4;
@@ -381,7 +374,7 @@ struct MvLane {
   unsigned sel;      // bytes 2 q and 2 q + 1
   unsigned mine[2];  // byte of the scale of the lane's first and second column, for a group set that starts at byte 0
   __device__ __forceinline__ unsigned token(unsigned t, unsigned k, unsigned q) const {
-    if (COLS == 8) return P == 4 ? q / 2 : P == 2 ? 4 * t + q : 8 * t + 2 * q + k;
+    if (COLS == 8) return P == 4 ? 2 * t + q / 2 : P == 2 ? 4 * t + q : 8 * t + 2 * q + k;
     return ((2 * q + k) % COLS) / P;
   }
   // Whether the lane has its column's results when the lanes have been joined.
@@ -478,34 +471,39 @@ __device__ __forceinline__ void mv_span(const MvLane<P, NT, COLS>& ln, const MvF
     sc[0][0] = f.s[0].x; sc[0][1] = f.s[0].y; sc[1][0] = f.s[0].z; sc[1][1] = f.s[0].w;
   }
   if constexpr (P == 4) {
-    const uint32_t xc = ln.col + 2048 * s;
-    int c[4], sum[4] = {0, 0, 0, 0};
+    const uint32_t xc = ln.col + 2048 * NT * s;
+    int sum[NT][4];
+#pragma unroll
+    for (unsigned t = 0; t < NT; ++t) sum[t][0] = sum[t][1] = sum[t][2] = sum[t][3] = 0;
 #pragma unroll
     for (unsigned grp = 0; grp < 8; ++grp) {
       const uint4 wv = f.w[grp / 2];
       const uint32_t w0 = grp & 1 ? wv.z : wv.x, w1 = grp & 1 ? wv.w : wv.y;
-      uint32_t b0, b1;
-      asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(b0), "=r"(b1) : "r"(xc + 256 * grp));
-      mma_u8(c, w0 & 0x0f0f0f0fu, w1 & 0x0f0f0f0fu, w0 >> 4 & 0x0f0f0f0fu, w1 >> 4 & 0x0f0f0f0fu, b0, b1, grp % SHARE == 0);
-      if (grp % SHARE == SHARE - 1) {
-        // |c| <= 32 x 15 x 128, times 63, eight times: below 2^25
+      const uint32_t a0 = w0 & 0x0f0f0f0fu, a1 = w1 & 0x0f0f0f0fu, a2 = w0 >> 4 & 0x0f0f0f0fu, a3 = w1 >> 4 & 0x0f0f0f0fu;
+      const int k0 = static_cast<int>(prmt(sc[0][grp / 4], 0, 0x4440u | grp % 4)), k1 = static_cast<int>(prmt(sc[1][grp / 4], 0, 0x4440u | grp % 4));
 #pragma unroll
-        for (unsigned h = 0; h < 2; ++h) {
-          const int k = static_cast<int>(SHARE > 1 ? prmt(prmt(sc[h][0], sc[h][1], grp + 1 - SHARE + ln.mine[0]), 0, 0x4440u)
-                                                   : prmt(sc[h][grp / 4], 0, 0x4440u | grp % 4));
-          sum[2 * h] += c[2 * h] * k;
-          sum[2 * h + 1] += c[2 * h + 1] * k;
-        }
+      for (unsigned t = 0; t < NT; ++t) {
+        uint32_t b0, b1;
+        int c[4];
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(b0), "=r"(b1) : "r"(xc + 256 * (NT * grp + t)));
+        mma_u8(c, a0, a1, a2, a3, b0, b1);
+        // |c| <= 32 x 15 x 128, times 63, eight times: below 2^25
+        sum[t][0] += c[0] * k0;
+        sum[t][1] += c[1] * k0;
+        sum[t][2] += c[2] * k1;
+        sum[t][3] += c[3] * k1;
       }
     }
-    // two digits of the four: the upper two are 2^16 up
-    const float x = __uint_as_float(lds32(ln.scale[0][0] + 4 * s));
-    const float xd = (threadIdx.x & 1) ? x * 65536.0f : x;
+    const bool upper = threadIdx.x & 1;  // two digits of the four: the upper two are 2^16 up
 #pragma unroll
-    for (unsigned h = 0; h < 2; ++h) {
-      const float v = fmaf(static_cast<float>(sum[2 * h + 1]), 256.0f, static_cast<float>(sum[2 * h]));
-      // the sums are in the first digit's column; a span is one term of acc, whichever warps share the tile
-      acc[h] += fmaf(v * d[h], xd, ((threadIdx.x & 1) ? 0.0f : m[0][2 * h] * dm[h]) * x);
+    for (unsigned t = 0; t < NT; ++t) {
+      const float x = __uint_as_float(lds32(ln.scale[t][0] + 4 * s)), xd = upper ? x * 65536.0f : x;
+#pragma unroll
+      for (unsigned h = 0; h < 2; ++h) {
+        const float v = fmaf(static_cast<float>(sum[t][2 * h + 1]), 256.0f, static_cast<float>(sum[t][2 * h]));
+        // the sums of x are in the first digit's column
+        acc[2 * t + h] += fmaf(v * d[h], xd, (upper ? 0.0f : m[t][2 * h] * dm[h]) * x);
+      }
     }
     return;
   }
@@ -653,7 +651,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 2 : 1) matvec_kernel(const Ma
   MvShared sh;
   sh.ring = smem;
   sh.col = smem + W * DEPTH * kBytes;
-  sh.sums = sh.col + (P == 4 ? 2048 : 4096 * NT) * a.chunk;
+  sh.sums = sh.col + (P == 4 ? 2048 : 4096) * NT * a.chunk;
   sh.scale = reinterpret_cast<float*>(sh.sums + (TYPE == kQ4K ? 256 * NT * a.chunk : 0));
   sh.part = sh.scale + a.tokens * a.chunk;
   const MvLane<P, NT, COLS> ln(a, sh, lane);
@@ -823,7 +821,7 @@ inline size_t mv_smem(unsigned type, unsigned P, unsigned nt, unsigned tokens, u
                       unsigned chunk, unsigned tiles) {
   const unsigned scale = type == FRC_Q4_K ? 256 : 128;
   return static_cast<size_t>(warps) * kMvDepth * (2048 + scale) +
-         static_cast<size_t>(chunk) * ((P == 4 ? 2048 : 4096 * nt) + (type == FRC_Q4_K ? 256 * nt : 0) + 4 * tokens) +
+         static_cast<size_t>(chunk) * ((P == 4 ? 2048 : 4096) * nt + (type == FRC_Q4_K ? 256 * nt : 0) + 4 * tokens) +
          (static_cast<size_t>(warps) + tiles) * values * 128;
 }
 inline unsigned mv_ceil(unsigned a, unsigned b) { return (a + b - 1) / b; }
@@ -899,7 +897,7 @@ inline cudaError_t mv_launch_w(const MatvecParams& a, const MvPlan& p, cudaStrea
 
 template <unsigned TYPE>
 inline cudaError_t launch_matvec(MatvecParams& a, const MvLayout& l, unsigned x_type, unsigned sms, cudaStream_t s) {
-  const unsigned P = TYPE == kQ4K && a.tokens <= 2 ? 4 : x_type == FRC_F32 ? 2 : 1, cols = a.tokens * P, nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
+  const unsigned P = TYPE == kQ4K && a.tokens <= 4 ? 4 : x_type == FRC_F32 ? 2 : 1, cols = a.tokens * P, nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
   MvPlan p = mv_plan(TYPE, P, nt, a.tokens, l, sms);
 #ifdef MV_ENV
   if (const char* e = getenv("MV_PLAN")) {  // warps,cluster,share
@@ -922,19 +920,19 @@ inline cudaError_t launch_matvec(MatvecParams& a, const MvLayout& l, unsigned x_
   a.tile_bytes = l.tile_bytes; a.base_at = l.base_at; a.tiles = l.tiles; a.spans = l.spans; a.pieces_last = l.pieces_last;
   a.slice = p.slice; a.chunk = p.chunk; a.cluster = p.cluster;
   if constexpr (TYPE == kQ4K) {
-    if (P == 4) return mv_launch_w<TYPE, 4, 1, 8>(a, p, s);
+    if (P == 4) return nt == 1 ? mv_launch_w<TYPE, 4, 1, 8>(a, p, s) : mv_launch_w<TYPE, 4, 2, 8>(a, p, s);
   } else {
     if (P == 2 && cols <= 2 && p.share) return mv_launch_w<TYPE, 2, 1, 2>(a, p, s);
     if (P == 2 && cols <= 4 && p.share) return mv_launch_w<TYPE, 2, 1, 4>(a, p, s);
     if (P == 1 && cols <= 1 && p.share) return mv_launch_w<TYPE, 1, 1, 1>(a, p, s);
     if (P == 1 && cols <= 2 && p.share) return mv_launch_w<TYPE, 1, 1, 2>(a, p, s);
+    if (P == 1 && cols <= 4 && p.share) return mv_launch_w<TYPE, 1, 1, 4>(a, p, s);
   }
   if (P == 2) {
     if (nt == 1) return mv_launch_w<TYPE, 2, 1, 8>(a, p, s);
     if (nt == 2) return mv_launch_w<TYPE, 2, 2, 8>(a, p, s);
     return mv_launch_w<TYPE, 2, 4, 8>(a, p, s);
   }
-  if (cols <= 4 && p.share) return mv_launch_w<TYPE, 1, 1, 4>(a, p, s);
   if (nt == 1) return mv_launch_w<TYPE, 1, 1, 8>(a, p, s);
   return mv_launch_w<TYPE, 1, 2, 8>(a, p, s);
 }
