@@ -564,54 +564,70 @@ __device__ __forceinline__ void store_row(L* row, unsigned E, unsigned lane, con
 
 // One warp a row: the balance term of every logit is stored first, then lanes
 // 0-9 store the chosen ones' sum with the routing term.  BALANCE off: only
-// the chosen logits are read.
+// the chosen logits are read.  Ids are fetched two rows ahead and the chosen
+// logits one, like the row itself.
 template <typename L, unsigned V, bool FULL, bool BALANCE>
-__global__ void __launch_bounds__(256, 3) route_backward_kernel(const RouteBackwardParams a) {
+__global__ void __launch_bounds__(256, BALANCE ? 3 : 6) route_backward_kernel(const RouteBackwardParams a) {
+  // k = scale count (the balance term is p_e (k_e - sum p k)): by column, and as the lanes' slots
+  __shared__ float s_k[BALANCE ? kMaxExperts : 1];
+  __shared__ __align__(16) float s_slots[BALANCE ? kRouteSlots / 4 : 1][32][4];
   const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = blockDim.x / 32, E = a.experts;
   const L* logits = static_cast<const L*>(a.logits);
   const unsigned step = gridDim.x * warps;
   unsigned t = blockIdx.x * warps + warp;
   RowLoad<L, V, FULL> next;
-  bool next_valid = false;
-  unsigned next_id = E + 1;
-  float next_dg = 0.0f;
-  const auto fetch = [&](unsigned r) {
-    next_valid = !a.valid || a.valid[r];
+  unsigned id = E + 1, id1 = E + 1;
+  float dg = 0.0f, dg1 = 0.0f, val1 = -INFINITY;
+  bool valid1 = false, valid2 = false;
+  // the chosen experts in lanes 0-9, the shared logit in lane 10
+  const auto ids = [&](unsigned r) {
+    valid2 = !a.valid || a.valid[r];
     if (a.d_gate) {
-      if (lane < kTopK) next_id = a.expert[static_cast<size_t>(r) * kTopK + lane];
-      if (lane < kGates) next_dg = a.d_gate[static_cast<size_t>(r) * kGates + lane];
+      if (lane < kTopK) id1 = a.expert[static_cast<size_t>(r) * kTopK + lane];
+      if (lane < kGates) dg1 = a.d_gate[static_cast<size_t>(r) * kGates + lane];
     }
-    if (BALANCE) next.load(logits + r * a.stride, E, lane);
   };
-  if (t < a.tokens) fetch(t);
-  // the balance term as p_e (k_e - sum p k), k = scale count
-  float scale = 0.0f;
-  F2 k2[BALANCE ? kRouteSlots / 2 : 1];
+  const auto chosen_logit = [&](unsigned r, unsigned e) {
+    const L* row = logits + r * a.stride;
+    if (a.d_gate && lane < kTopK && e < E) return logit(row + e);
+    if (a.d_gate && lane == kTopK && a.shared) return logit(row + E);
+    return -INFINITY;
+  };
+  if (t < a.tokens) {
+    ids(t);
+    if (BALANCE) next.load(logits + t * a.stride, E, lane);
+  }
   if (BALANCE) {
     const float n = static_cast<float>(a.count[E]);
-    scale = n > 0.0f ? *a.d_loss * static_cast<float>(E) / (static_cast<float>(kTopK) * n * n) : 0.0f;
-#pragma unroll
-    for (unsigned i = 0; i < kRouteSlots / 2; ++i) {
-      const unsigned c = col<V>(2 * i, lane), d = col<V>(2 * i + 1, lane);
-      k2[i] = pack2(c < E ? scale * static_cast<float>(a.count[c]) : 0.0f, d < E ? scale * static_cast<float>(a.count[d]) : 0.0f);
-    }
+    const float scale = n > 0.0f ? *a.d_loss * static_cast<float>(E) / (static_cast<float>(kTopK) * n * n) : 0.0f;
+    for (unsigned e = threadIdx.x; e < kMaxExperts; e += blockDim.x) s_k[e] = e < E ? scale * static_cast<float>(a.count[e]) : 0.0f;
+    __syncthreads();
+    for (unsigned i = threadIdx.x; i < kMaxExperts; i += blockDim.x)
+      s_slots[i / 128][i / 4 % 32][i % 4] = s_k[col<V>(i / 128 * 4 + i % 4, i / 4 % 32)];
+    __syncthreads();
+  }
+  if (t < a.tokens) {
+    id = id1;
+    dg = dg1;
+    valid1 = valid2;
+    val1 = chosen_logit(t, id);
+    if (t + step < a.tokens) ids(t + step);
   }
   for (; t < a.tokens; t += step) {
-    const L* row = logits + t * a.stride;
     L* out = static_cast<L*>(a.d_logits) + t * a.d_stride;
-    const bool valid = next_valid;
+    const bool valid = valid1;
+    const float val = val1, cdg = dg;
+    const unsigned cid = id;
     float d[kRouteSlots];
-    // the chosen experts of lanes 0-9, the shared logit in lane 10
-    const unsigned id = next_id;
-    const float dg = next_dg;
-    float val = -INFINITY;
-    if (a.d_gate && valid && (lane < kTopK ? id < E : lane == kTopK && a.shared)) val = logit(row + (lane < kTopK ? id : E));
 #pragma unroll
     for (unsigned i = 0; i < kRouteSlots; ++i) d[i] = BALANCE ? next.value(i) : 0.0f;
-    if (t + step < a.tokens) fetch(t + step);
-    if (lane < kTopK && a.d_gate && valid) {
-      if (id >= E) atomicOr(a.status, kStInvalid);
-      if (!(val < INFINITY)) atomicOr(a.status, kStNumeric);
+    if (t + step < a.tokens) {
+      id = id1;
+      dg = dg1;
+      valid1 = valid2;
+      val1 = chosen_logit(t + step, id);
+      if (step < a.tokens - t - step) ids(t + 2 * step);
+      if (BALANCE) next.load(logits + (t + step) * a.stride, E, lane);
     }
     float m = -INFINITY, zi = 0.0f, dot = 0.0f;
     if (BALANCE) {
@@ -621,7 +637,11 @@ __global__ void __launch_bounds__(256, 3) route_backward_kernel(const RouteBackw
         F2 e[kRouteSlots / 2], s2 = pack2(0.0f, 0.0f);
         const float z = exp_row(d, m, e);
 #pragma unroll
-        for (unsigned i = 0; i < kRouteSlots / 2; ++i) s2 = fma2(e[i], k2[i], s2);
+        for (unsigned i = 0; i < kRouteSlots / 4; ++i) {
+          const float4 k = *reinterpret_cast<const float4*>(s_slots[i][lane]);
+          s2 = fma2(e[2 * i], pack2(k.x, k.y), s2);
+          s2 = fma2(e[2 * i + 1], pack2(k.z, k.w), s2);
+        }
         unpack2(s2, dot, zi);
         dot += zi;
         zi = rcp(warp_sum(z));
@@ -629,7 +649,11 @@ __global__ void __launch_bounds__(256, 3) route_backward_kernel(const RouteBackw
         // (e / z) (k - dot) = e (k / z - dot / z)
         const F2 z2 = pack2(zi, zi), c2 = pack2(-dot * zi, -dot * zi);
 #pragma unroll
-        for (unsigned i = 0; i < kRouteSlots / 2; ++i) unpack2(mul2(e[i], fma2(k2[i], z2, c2)), d[2 * i], d[2 * i + 1]);
+        for (unsigned i = 0; i < kRouteSlots / 4; ++i) {
+          const float4 k = *reinterpret_cast<const float4*>(s_slots[i][lane]);
+          unpack2(mul2(e[2 * i], fma2(pack2(k.x, k.y), z2, c2)), d[4 * i], d[4 * i + 1]);
+          unpack2(mul2(e[2 * i + 1], fma2(pack2(k.z, k.w), z2, c2)), d[4 * i + 2], d[4 * i + 3]);
+        }
       } else {
 #pragma unroll
         for (unsigned i = 0; i < kRouteSlots; ++i) d[i] = 0.0f;
@@ -638,14 +662,16 @@ __global__ void __launch_bounds__(256, 3) route_backward_kernel(const RouteBackw
     __syncwarp();  // d_logits may be logits: every lane has read the row
     store_row<L, V, FULL>(out, E, lane, d);
     if (a.d_gate) {
-      const float chosen = lane < kTopK ? val : -INFINITY, mk = warp_max(chosen);
+      if (lane < kTopK && valid) {
+        if (cid >= E) atomicOr(a.status, kStInvalid);
+        if (!(val < INFINITY)) atomicOr(a.status, kStNumeric);
+      }
+      const float chosen = lane < kTopK && valid ? val : -INFINITY, mk = warp_max(chosen);
       float g = mk > -INFINITY ? exp2f((chosen - mk) * 1.4426950408889634f) : 0.0f;  // subnormal gates count
-      const float s = warp_sum(g);
-      g = s > 0.0f ? g * rcp(s) : 0.0f;
-      const float gd = warp_sum(g * dg);
-      const float own = g * (dg - gd);
+      const float s = warp_sum(g), gd0 = warp_sum(g * cdg), si = s > 0.0f ? rcp(s) : 0.0f;
+      const float own = g * si * (cdg - gd0 * si);
       float term = own;
-      const unsigned same = __match_any_sync(0xffffffffu, id) & 0x3ffu;
+      const unsigned same = __match_any_sync(0xffffffffu, cid) & 0x3ffu;
       const bool twice = lane < kTopK && same != 1u << lane;
       if (__any_sync(0xffffffffu, twice)) {  // the same index twice adds twice
         if (twice) term = 0.0f;
@@ -654,13 +680,13 @@ __global__ void __launch_bounds__(256, 3) route_backward_kernel(const RouteBackw
           if (twice && (same >> r & 1u)) term += o;
         }
       }
-      if (BALANCE && lane < kTopK && zi > 0.0f && id < E) term += exp_below(val, m) * fmaf(scale * static_cast<float>(a.count[id]), zi, -dot * zi);
+      if (BALANCE && lane < kTopK && zi > 0.0f && cid < E) term += exp_below(val, m) * fmaf(s_k[cid], zi, -dot * zi);
       __syncwarp();  // behind the row's stores
-      if (valid && lane < kTopK && id < E) store_grad(out + id, term);
+      if (valid && lane < kTopK && cid < E) store_grad(out + cid, term);
     }
     if (a.shared && lane == kTopK) {
       const float sg = a.d_gate && valid ? sigmoid(val) : 0.0f;
-      store_grad(out + E, sg * (1.0f - sg) * dg);
+      store_grad(out + E, sg * (1.0f - sg) * cdg);
     }
   }
 }
@@ -739,7 +765,7 @@ inline cudaError_t launch_route(const RouteParams& a, const RouteFinish& f, unsi
 
 template <typename L, unsigned V, bool FULL>
 inline cudaError_t launch_backward(const RouteBackwardParams& a, unsigned sms, cudaStream_t s) {
-  const unsigned warps = a.tokens <= 8 * sms ? 4 : 8, ctas = (a.tokens + warps - 1) / warps, grid = ctas < 3 * sms ? ctas : 3 * sms;
+  const unsigned warps = a.tokens <= 8 * sms ? 4 : 8, ctas = (a.tokens + warps - 1) / warps, limit = (a.count ? 3 : 6) * sms, grid = ctas < limit ? ctas : limit;
   if (a.count) route_backward_kernel<L, V, FULL, true><<<grid, 32 * warps, 0, s>>>(a);
   else route_backward_kernel<L, V, FULL, false><<<grid, 32 * warps, 0, s>>>(a);
   return cudaGetLastError();
