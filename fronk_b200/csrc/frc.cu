@@ -1807,25 +1807,31 @@ int frc_matrix_open(frc_context* c, unsigned type, unsigned rows, unsigned n, co
   if (!m) return fail(c, FRC_IO, "out of memory");
   m->device = c->device; m->type = type; m->rows = rows; m->n = n;
   m->layout = mv_layout(type, rows, n);
-  // the rows as given (freed again) behind a word for the scale check
-  uint8_t* raw = nullptr;
+  // rows in this device's memory are laid out from where they are, others from a copy (freed again); a word behind
+  // the layout takes the scale check
+  const size_t flag_at = (m->layout.total + 15) / 16 * 16;
+  cudaPointerAttributes where{};
+  cudaError_t e = cudaPointerGetAttributes(&where, bytes);
+  const bool here = e == cudaSuccess && where.type == cudaMemoryTypeDevice && where.device == c->device;
+  uint8_t* copy = nullptr;
   unsigned bad = 0;
-  cudaError_t e = cudaMalloc(&m->data, m->layout.total);
-  if (e == cudaSuccess) e = cudaMalloc(&raw, 16 + total);
-  unsigned* flag = reinterpret_cast<unsigned*>(raw);
+  if (e == cudaSuccess) e = cudaMalloc(&m->data, flag_at + 16);
+  if (e == cudaSuccess && !here) e = cudaMalloc(&copy, total);
+  if (e == cudaSuccess && !here) e = cudaMemcpyAsync(copy, bytes, total, cudaMemcpyDefault, c->stream);
+  unsigned* flag = reinterpret_cast<unsigned*>(m->data + flag_at);
   if (e == cudaSuccess) e = cudaMemsetAsync(flag, 0, sizeof bad, c->stream);
-  if (e == cudaSuccess) e = cudaMemcpyAsync(raw + 16, bytes, total, cudaMemcpyDefault, c->stream);
   if (e == cudaSuccess) {
+    const uint8_t* raw = here ? static_cast<const uint8_t*>(bytes) : copy;
     if (type == FRC_Q4_K)
-      matrix_layout_kernel<kQ4K><<<m->layout.tiles, 256, 0, c->stream>>>(raw + 16, m->data, m->layout, rows, n, static_cast<unsigned>(rowb), flag);
+      matrix_layout_kernel<kQ4K><<<m->layout.tiles, 256, 0, c->stream>>>(raw, m->data, m->layout, rows, n, static_cast<unsigned>(rowb), flag);
     else
-      matrix_layout_kernel<kMXFP4><<<m->layout.tiles, 256, 0, c->stream>>>(raw + 16, m->data, m->layout, rows, n, static_cast<unsigned>(rowb), flag);
+      matrix_layout_kernel<kMXFP4><<<m->layout.tiles, 256, 0, c->stream>>>(raw, m->data, m->layout, rows, n, static_cast<unsigned>(rowb), flag);
     e = cudaGetLastError();
     ++c->launches;
   }
   if (e == cudaSuccess) e = cudaMemcpyAsync(&bad, flag, sizeof bad, cudaMemcpyDeviceToHost, c->stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
-  cudaFree(raw);
+  cudaFree(copy);
   if (e != cudaSuccess || bad) {
     frc_matrix_close(m);
     return bad ? fail(c, FRC_NUMERIC, "matrix: a scale is not finite") : fail(c, FRC_IO, "matrix: %s", cudaGetErrorString(e));
