@@ -1783,6 +1783,7 @@ struct frc_matrix {
   int device = 0;
   unsigned type = 0, rows = 0, n = 0;
   MvLayout layout{};
+  MvPlan plan[2][FRC_MAX_TOKENS];  // [type of x][tokens - 1]
   uint8_t* data = nullptr;
 };
 
@@ -1807,6 +1808,9 @@ int frc_matrix_open(frc_context* c, unsigned type, unsigned rows, unsigned n, co
   if (!m) return fail(c, FRC_IO, "out of memory");
   m->device = c->device; m->type = type; m->rows = rows; m->n = n;
   m->layout = mv_layout(type, rows, n);
+  for (unsigned t = 0; t < 2 * FRC_MAX_TOKENS; ++t)
+    m->plan[t / FRC_MAX_TOKENS][t % FRC_MAX_TOKENS] =
+        mv_plan(type, t % FRC_MAX_TOKENS + 1, t / FRC_MAX_TOKENS, m->layout, static_cast<unsigned>(c->sms));
   // rows in this device's memory are laid out from where they are, others from a copy (freed again); a word behind
   // the layout takes the scale check
   const size_t flag_at = (m->layout.total + 15) / 16 * 16;
@@ -1860,8 +1864,10 @@ int frc_matvec_device(frc_context* c, const frc_matrix* m, unsigned tokens, cons
   a.y_bf16 = y_type == FRC_BF16;
   a.status = c->status;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  CK(m->type == FRC_Q4_K ? launch_matvec<kQ4K>(a, m->layout, x_type, static_cast<unsigned>(c->sms), s)
-                         : launch_matvec<kMXFP4>(a, m->layout, x_type, static_cast<unsigned>(c->sms), s));
+  const MvPlan& p = m->plan[x_type][tokens - 1];
+  const unsigned sms = static_cast<unsigned>(c->sms);
+  CK(m->type == FRC_Q4_K ? launch_matvec<kQ4K>(a, m->layout, p, x_type, sms, c->device, s)
+                         : launch_matvec<kMXFP4>(a, m->layout, p, x_type, sms, c->device, s));
   ++c->launches;
   return FRC_OK;
 }

@@ -27,6 +27,7 @@
 // aligns its sums by the operands' exponents: measured, q 2^-24 costs 20 times
 // the rounding error.)
 #pragma once
+#include <atomic>
 #include <cuda_bf16.h>
 
 #include "../../include/fronk_b200.h"
@@ -871,11 +872,14 @@ inline MvPlan mv_plan(unsigned type, unsigned P, unsigned nt, unsigned tokens, c
 }
 
 template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS, unsigned W>
-inline cudaError_t mv_launch(const MatvecParams& a, const MvPlan& p, cudaStream_t s) {
-  if (p.smem > 48 * 1024) {
+inline cudaError_t mv_launch(const MatvecParams& a, const MvPlan& p, int device, cudaStream_t s) {
+  static std::atomic<unsigned long long> allowed{0};  // devices on which the kernel may use kMvSmemCta bytes
+  const unsigned long long bit = 1ull << (device & 63);
+  if (p.smem > 48 * 1024 && (device > 63 || !(allowed.load(std::memory_order_relaxed) & bit))) {
     const cudaError_t e = cudaFuncSetAttribute(matvec_kernel<TYPE, P, NT, COLS, W, kMvDepth>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(p.smem));
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, kMvSmemCta);
     if (e != cudaSuccess) return e;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
@@ -891,14 +895,24 @@ inline cudaError_t mv_launch(const MatvecParams& a, const MvPlan& p, cudaStream_
   return cudaLaunchKernelEx(&cfg, matvec_kernel<TYPE, P, NT, COLS, W, kMvDepth>, a);
 }
 template <unsigned TYPE, unsigned P, unsigned NT, unsigned COLS>
-inline cudaError_t mv_launch_w(const MatvecParams& a, const MvPlan& p, cudaStream_t s) {
-  return p.warps == 8 ? mv_launch<TYPE, P, NT, COLS, 8>(a, p, s) : mv_launch<TYPE, P, NT, COLS, 16>(a, p, s);
+inline cudaError_t mv_launch_w(const MatvecParams& a, const MvPlan& p, int device, cudaStream_t s) {
+  return p.warps == 8 ? mv_launch<TYPE, P, NT, COLS, 8>(a, p, device, s) : mv_launch<TYPE, P, NT, COLS, 16>(a, p, device, s);
+}
+
+// Parts of x and groups of eight columns of a call.
+inline unsigned mv_parts(unsigned type, unsigned tokens, unsigned x_type) {
+  return type == FRC_Q4_K && tokens <= 4 ? 4 : x_type == FRC_F32 ? 2 : 1;
+}
+inline unsigned mv_groups(unsigned cols) { return cols <= 8 ? 1 : cols <= 16 ? 2 : 4; }
+inline MvPlan mv_plan(unsigned type, unsigned tokens, unsigned x_type, const MvLayout& l, unsigned sms) {
+  const unsigned P = mv_parts(type, tokens, x_type);
+  return mv_plan(type, P, mv_groups(tokens * P), tokens, l, sms);
 }
 
 template <unsigned TYPE>
-inline cudaError_t launch_matvec(MatvecParams& a, const MvLayout& l, unsigned x_type, unsigned sms, cudaStream_t s) {
-  const unsigned P = TYPE == kQ4K && a.tokens <= 4 ? 4 : x_type == FRC_F32 ? 2 : 1, cols = a.tokens * P, nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
-  MvPlan p = mv_plan(TYPE, P, nt, a.tokens, l, sms);
+inline cudaError_t launch_matvec(MatvecParams& a, const MvLayout& l, MvPlan p, unsigned x_type, unsigned sms, int device,
+                                 cudaStream_t s) {
+  const unsigned P = mv_parts(TYPE, a.tokens, x_type), cols = a.tokens * P, nt = mv_groups(cols);
 #ifdef MV_ENV
   if (const char* e = getenv("MV_PLAN")) {  // warps,cluster,share
     unsigned w, c, shr;
@@ -920,21 +934,21 @@ inline cudaError_t launch_matvec(MatvecParams& a, const MvLayout& l, unsigned x_
   a.tile_bytes = l.tile_bytes; a.base_at = l.base_at; a.tiles = l.tiles; a.spans = l.spans; a.pieces_last = l.pieces_last;
   a.slice = p.slice; a.chunk = p.chunk; a.cluster = p.cluster;
   if constexpr (TYPE == kQ4K) {
-    if (P == 4) return nt == 1 ? mv_launch_w<TYPE, 4, 1, 8>(a, p, s) : mv_launch_w<TYPE, 4, 2, 8>(a, p, s);
+    if (P == 4) return nt == 1 ? mv_launch_w<TYPE, 4, 1, 8>(a, p, device, s) : mv_launch_w<TYPE, 4, 2, 8>(a, p, device, s);
   } else {
-    if (P == 2 && cols <= 2 && p.share) return mv_launch_w<TYPE, 2, 1, 2>(a, p, s);
-    if (P == 2 && cols <= 4 && p.share) return mv_launch_w<TYPE, 2, 1, 4>(a, p, s);
-    if (P == 1 && cols <= 1 && p.share) return mv_launch_w<TYPE, 1, 1, 1>(a, p, s);
-    if (P == 1 && cols <= 2 && p.share) return mv_launch_w<TYPE, 1, 1, 2>(a, p, s);
-    if (P == 1 && cols <= 4 && p.share) return mv_launch_w<TYPE, 1, 1, 4>(a, p, s);
+    if (P == 2 && cols <= 2 && p.share) return mv_launch_w<TYPE, 2, 1, 2>(a, p, device, s);
+    if (P == 2 && cols <= 4 && p.share) return mv_launch_w<TYPE, 2, 1, 4>(a, p, device, s);
+    if (P == 1 && cols <= 1 && p.share) return mv_launch_w<TYPE, 1, 1, 1>(a, p, device, s);
+    if (P == 1 && cols <= 2 && p.share) return mv_launch_w<TYPE, 1, 1, 2>(a, p, device, s);
+    if (P == 1 && cols <= 4 && p.share) return mv_launch_w<TYPE, 1, 1, 4>(a, p, device, s);
   }
   if (P == 2) {
-    if (nt == 1) return mv_launch_w<TYPE, 2, 1, 8>(a, p, s);
-    if (nt == 2) return mv_launch_w<TYPE, 2, 2, 8>(a, p, s);
-    return mv_launch_w<TYPE, 2, 4, 8>(a, p, s);
+    if (nt == 1) return mv_launch_w<TYPE, 2, 1, 8>(a, p, device, s);
+    if (nt == 2) return mv_launch_w<TYPE, 2, 2, 8>(a, p, device, s);
+    return mv_launch_w<TYPE, 2, 4, 8>(a, p, device, s);
   }
-  if (nt == 1) return mv_launch_w<TYPE, 1, 1, 8>(a, p, s);
-  return mv_launch_w<TYPE, 1, 2, 8>(a, p, s);
+  if (nt == 1) return mv_launch_w<TYPE, 1, 1, 8>(a, p, device, s);
+  return mv_launch_w<TYPE, 1, 2, 8>(a, p, device, s);
 }
 
 }  // namespace frc
