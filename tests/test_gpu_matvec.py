@@ -77,6 +77,50 @@ def test_shapes(ctx, type_, rows, n, tokens):
         check(host(y), host(xd), w, a, n, y_type)
 
 
+@pytest.mark.parametrize("type_,n", [(fb.Q4_K, 256), (fb.Q4_K, 2304), (fb.Q4_K, 5120), (fb.MXFP4, 32), (fb.MXFP4, 672),
+                                     (fb.MXFP4, 2560)])
+@pytest.mark.parametrize("tokens", [5, 8, 9, 16])
+def test_bursts_of_many_rows(ctx, type_, n, tokens):
+    """Bursts of five tokens and more over matrices of many rows; rows between the runs of the CTAs, odd strides."""
+    import torch
+    rows = 19111
+    rng = np.random.default_rng(n + tokens)
+    base = quant.random_rows(type_, 509, n, rng)
+    raw = np.tile(base, (rows // 509 + 1, 1))[:rows]
+    w, a = quant.weights(type_, base, n)
+    for x_type, y_type in [(fb.F32, fb.F32), (fb.BF16, fb.BF16)]:
+        xb = torch.full((tokens, n + 3), float("nan"), dtype=torch.bfloat16 if x_type == fb.BF16 else torch.float32, device="cuda")
+        xb[:, :n] = to_device(rng.standard_normal((tokens, n)), x_type)
+        yb = torch.full((tokens, rows + 1), -7.0, dtype=torch.bfloat16 if y_type == fb.BF16 else torch.float32, device="cuda")
+        s = torch.cuda.current_stream().cuda_stream
+        with ctx.matrix(type_, rows, n, raw) as m:
+            m.matvec_device(tokens, xb.data_ptr(), yb.data_ptr(), x_type, y_type, n + 3, rows + 1, s)
+            assert ctx.status(s) == fb.OK
+            first = yb.clone()
+            m.matvec_device(tokens, xb.data_ptr(), yb.data_ptr(), x_type, y_type, n + 3, rows + 1, s)
+            assert ctx.status(s) == fb.OK and torch.equal(first, yb)
+        assert bool((yb[:, rows] == -7).all())
+        y, x = host(yb[:, :rows]), host(xb[:, :n])
+        for r in range(0, rows, 509):
+            k = min(509, rows - r)
+            check(y[:, r:r + k], x, w[:k], a[:k], n, y_type)
+
+
+def test_bursts_with_scales_far_apart(ctx):
+    """MXFP4 rows whose exponents differ by more than fp16 holds, in a matrix of many rows."""
+    n, rows, tokens = 512, 19000, 7
+    rng = np.random.default_rng(77)
+    base = quant.random_rows(fb.MXFP4, 100, n, rng, exponents=(90, 127))
+    raw = np.tile(base, (rows // 100, 1))
+    w, a = quant.weights(fb.MXFP4, base, n)
+    x = rng.standard_normal((tokens, n))
+    x[3, :480] = 0  # only one block of each row counts
+    xd = to_device(x, fb.F32)
+    y = host(run(ctx, fb.MXFP4, raw, n, xd, fb.F32, fb.F32))
+    for r in range(0, rows, 100):
+        check(y[:, r:r + 100], host(xd), w, a, n, fb.F32)
+
+
 @pytest.mark.parametrize("type_", [fb.Q4_K, fb.MXFP4])
 @pytest.mark.parametrize("tokens,x_type", [(1, fb.F32), (4, fb.BF16), (16, fb.F32)])
 def test_long_rows(ctx, type_, tokens, x_type):
