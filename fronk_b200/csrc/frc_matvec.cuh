@@ -830,9 +830,10 @@ inline unsigned mv_ceil(unsigned a, unsigned b) { return (a + b - 1) / b; }
 // Chooses the warps a CTA and the CTAs that share K by an estimate of the
 // time in us, fitted to sweeps over both: a span takes a warp 0.06 us (times
 // `heavy`, for the columns) for each warp of its SM, at least 0.4; preparing
-// x 0.25 a span and warp, a cluster's exchange 0.5 and 0.02 a tile.  Measured
-// both ways: 5120 x 2560 and 8 tokens 8.7 us with clusters of 4, 10.2 without;
-// 4096 x 8192 and one token 8.6 and 9.8; 513 x 2048 and one token 3.8 and 3.4.
+// x 0.35 a span and warp, a cluster's exchange 0.1 a CTA and 0.02 a tile.
+// Measured both ways: 5120 x 2560 and 8 tokens 9.0 us with clusters of 4, 10.1
+// without; 4096 x 8192 and one token 8.6 and 9.0; 513 x 2048 and one token 3.8
+// and 3.4; 50021 x 2560 and 16 tokens 26.2 with clusters of 2, 24.9 without.
 inline MvPlan mv_plan(unsigned type, unsigned P, unsigned nt, unsigned tokens, const MvLayout& l, unsigned sms) {
   const unsigned values = nt * (P >= 2 ? 2 : 4);
   const double heavy = nt == 1 ? 1.0 : nt == 2 ? 1.5 : 2.3;
@@ -858,8 +859,8 @@ inline MvPlan mv_plan(unsigned type, unsigned P, unsigned nt, unsigned tokens, c
       p.smem = static_cast<unsigned>(mv_smem(type, P, nt, tokens, values, warps, p.chunk, kept));
       const unsigned steps = mv_ceil(tiles * p.slice, warps), busy = warps * mv_ceil(p.grid, sms);
       const double step = 0.06 * busy * heavy > 0.4 ? 0.06 * busy * heavy : 0.4;
-      const double prep = 0.4 + 0.25 * mv_ceil(tokens * p.chunk, warps);
-      double t = step * steps + prep + (cluster > 1 ? 0.5 + 0.02 * tiles : 0.0);
+      const double prep = 0.4 + 0.35 * mv_ceil(tokens * p.chunk, warps);
+      double t = step * steps + prep + (cluster > 1 ? 0.3 + 0.1 * cluster + 0.02 * tiles : 0.0) + (warps == 16 ? 0.3 : 0.0);
       if (p.chunk < p.slice) t += (step + prep) * mv_ceil(tiles, warps) * mv_ceil(p.slice, p.chunk);
       p.share = steps >= 6;
       if (t < least * 0.98) {
