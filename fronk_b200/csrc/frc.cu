@@ -1837,6 +1837,7 @@ int frc_matrix_open(frc_context* c, unsigned type, unsigned rows, unsigned n, co
   if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
   cudaFree(copy);
   if (e != cudaSuccess || bad) {
+    cudaGetLastError();  // reported here, not by a later call
     frc_matrix_close(m);
     return bad ? fail(c, FRC_NUMERIC, "matrix: a scale is not finite") : fail(c, FRC_IO, "matrix: %s", cudaGetErrorString(e));
   }
@@ -1865,9 +1866,8 @@ int frc_matvec_device(frc_context* c, const frc_matrix* m, unsigned tokens, cons
   a.status = c->status;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const MvPlan& p = m->plan[x_type][tokens - 1];
-  const unsigned sms = static_cast<unsigned>(c->sms);
-  CK(m->type == FRC_Q4_K ? launch_matvec<kQ4K>(a, m->layout, p, x_type, sms, c->device, s)
-                         : launch_matvec<kMXFP4>(a, m->layout, p, x_type, sms, c->device, s));
+  CK(m->type == FRC_Q4_K ? launch_matvec<kQ4K>(a, m->layout, p, x_type, c->device, s)
+                         : launch_matvec<kMXFP4>(a, m->layout, p, x_type, c->device, s));
   ++c->launches;
   return FRC_OK;
 }

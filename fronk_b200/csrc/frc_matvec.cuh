@@ -911,27 +911,9 @@ inline MvPlan mv_plan(unsigned type, unsigned tokens, unsigned x_type, const MvL
 }
 
 template <unsigned TYPE>
-inline cudaError_t launch_matvec(MatvecParams& a, const MvLayout& l, MvPlan p, unsigned x_type, unsigned sms, int device,
+inline cudaError_t launch_matvec(MatvecParams& a, const MvLayout& l, const MvPlan& p, unsigned x_type, int device,
                                  cudaStream_t s) {
   const unsigned P = mv_parts(TYPE, a.tokens, x_type), cols = a.tokens * P, nt = mv_groups(cols);
-#ifdef MV_ENV
-  if (const char* e = getenv("MV_PLAN")) {  // warps,cluster,share
-    unsigned w, c, shr;
-    if (sscanf(e, "%u,%u,%u", &w, &c, &shr) == 3) {
-      const unsigned values = nt * (P >= 2 ? 2 : 4);
-      p.share = shr;
-      p.warps = w; p.cluster = c; p.slice = p.chunk = (l.spans + c - 1) / c;
-      const unsigned resident = sms * (w == 8 ? 2 : 1) / c * (c > 2 ? 7 : 8) / 8, groups = l.tiles < resident ? l.tiles : resident;
-      const unsigned kept = c > 1 ? mv_ceil(l.tiles, groups) : 0;
-      const size_t lim = w == 8 ? (kMvSmemSm - 2048) / 2 : kMvSmemCta;
-      if (mv_smem(TYPE, P, nt, a.tokens, values, w, p.chunk, kept) > lim) return cudaErrorInvalidValue;
-      p.grid = groups * c;
-      p.smem = mv_smem(TYPE, P, nt, a.tokens, values, w, p.chunk, kept);
-    }
-    static MvPlan shown{};
-    if (e[0] == 'p' && memcmp(&shown, &p, sizeof p)) { shown = p; fprintf(stderr, "plan warps %u cluster %u slice %u chunk %u grid %u smem %u share %u\n", p.warps, p.cluster, p.slice, p.chunk, p.grid, p.smem, p.share); }
-  }
-#endif
   a.tile_bytes = l.tile_bytes; a.base_at = l.base_at; a.tiles = l.tiles; a.spans = l.spans; a.pieces_last = l.pieces_last;
   a.slice = p.slice; a.chunk = p.chunk; a.cluster = p.cluster;
   if constexpr (TYPE == kQ4K) {

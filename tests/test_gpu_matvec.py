@@ -154,6 +154,31 @@ def test_many_rows(ctx, type_, rows):
         assert np.array_equal(again, y)
 
 
+def test_offsets_past_32_bits(ctx):
+    """A matrix of more than 4 GiB (rows given on the device): its first and last rows."""
+    import torch
+    rows, n = 130001, 65536
+    rng = np.random.default_rng(8)
+    few = quant.random_rows(fb.MXFP4, 64, n, rng)
+    w, a = quant.weights(fb.MXFP4, few, n)
+    raw = torch.zeros(rows, few.shape[1], dtype=torch.uint8, device="cuda")
+    raw[:32] = torch.from_numpy(few[:32]).cuda()
+    raw[-32:] = torch.from_numpy(few[32:]).cuda()
+    raw[32:-32, ::17] = 120
+    assert raw.numel() > 1 << 32
+    torch.cuda.synchronize()
+    s = torch.cuda.current_stream().cuda_stream
+    with ctx.matrix(fb.MXFP4, rows, n, raw.data_ptr(), raw.numel()) as m:
+        for tokens in (1, 6):
+            xd = to_device(rng.standard_normal((tokens, n)), fb.F32)
+            y = torch.full((tokens, rows), float("nan"), device="cuda")
+            m.matvec_device(tokens, xd.data_ptr(), y.data_ptr(), stream=s)
+            assert ctx.status(s) == fb.OK
+            got = host(torch.cat([y[:, :32], y[:, -32:]], 1))
+            check(got, host(xd), w, a, n, fb.F32)
+            assert not bool(y[:, 32:-32].any())
+
+
 @pytest.mark.parametrize("type_", [fb.Q4_K, fb.MXFP4])
 @pytest.mark.parametrize("x_type,y_type", [(fb.F32, fb.F32), (fb.BF16, fb.BF16)])
 def test_strides_and_alignment(ctx, type_, x_type, y_type):

@@ -407,11 +407,40 @@ def test_refusals(ctx):
     assert ctx.launches == before and ctx.status() == fb.OK
 
 
-def test_graphs_and_streams(ctx):
+def test_offsets_past_32_bits(ctx):
+    """More than 2^32 elements between the first and the last row."""
+    import torch
+    rng = np.random.default_rng(25)
+    T, E, stride, last = 1050000, 64, 4100, 40
+    logits = torch.zeros(T, stride, dtype=torch.bfloat16, device="cuda")
+    assert logits.numel() > 1 << 32
+    logits[-last:, :E] = torch.from_numpy(rng.standard_normal((last, E)).astype(np.float32)).cuda()
+    expert = torch.full((T, 10), -1, dtype=torch.int16, device="cuda")
+    gate = torch.full((T, 11), float("nan"), device="cuda")
+    ctx.route_device(T, E, logits.data_ptr(), expert.data_ptr(), gate.data_ptr(), stride=stride, type_=fb.BF16)
+    assert ctx.status() == fb.OK
+    ref = Reference(logits[-last:, :E].float().cpu().numpy().astype(np.float64))
+    assert np.array_equal(expert[-last:].cpu().numpy().astype(np.int64), ref.expert)
+    assert bool((expert[:-last] == torch.arange(10, device="cuda", dtype=torch.int16)).all())
+    assert np.all(np.abs(gate[-last:, :10].cpu().numpy() - ref.g) <= (2 * ref.Rg + 20) * U * ref.g + TINY)
+    dg = torch.zeros(T, 11, device="cuda")
+    d = rng.standard_normal((last, 11)).astype(np.float32)
+    dg[-last:] = torch.from_numpy(d).cuda()
+    ctx.route_backward_device(T, E, logits.data_ptr(), expert.data_ptr(), logits.data_ptr(), d_gate_ptr=dg.data_ptr(),
+                              stride=stride, d_stride=stride, type_=fb.BF16)
+    assert ctx.status() == fb.OK
+    want, tol = ref.backward(d.astype(np.float64))
+    got = logits[-last:, :E].float().cpu().numpy().astype(np.float64)
+    assert np.all(np.abs(got - want) <= tol + 2.0 ** -8 * np.abs(want) + 2.0 ** -133)
+    assert not bool(logits[:-last].any())
+
+
+@pytest.mark.parametrize("T", [300, 2000])
+def test_graphs_and_streams(ctx, T):
     """Two captured graphs with workspaces of their own, replayed side by side on new logits."""
     import torch
     rng = np.random.default_rng(23)
-    T, E = 300, 512
+    E = 512
     bs = [Buffers(np.zeros((T, E))) for _ in range(2)]
     outs = [torch.zeros(T, E, device="cuda") for _ in range(2)]
     d_loss = torch.ones(1, device="cuda")
