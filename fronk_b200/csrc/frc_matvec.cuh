@@ -509,7 +509,7 @@ __device__ __forceinline__ void mv_span(const MvLane<P, NT, COLS>& ln, const MvF
     return;
   }
   const uint32_t xc = ln.col + 4096 * NT * s;
-  constexpr unsigned SV = P == 2 && !FOLD ? 2 : 4;
+  constexpr unsigned SV = P == 2 ? 2 : 4;
   float sum[NT][SV], c[NT][4];
 #pragma unroll
   for (unsigned t = 0; t < NT; ++t)
@@ -541,9 +541,21 @@ __device__ __forceinline__ void mv_span(const MvLane<P, NT, COLS>& ln, const MvF
 #pragma unroll
     for (unsigned t = 0; t < NT; ++t) {
       const uint4 b = lds128(xc + 512 * (NT * grp + t));
-      if (FOLD ? grp == 0 : grp % SHARE == 0) mma_f16_first(c[t], a0[0], a1[0], a0[1], a1[1], b.x, b.y);
+      if (FOLD ? grp % 4 == 0 : grp % SHARE == 0) mma_f16_first(c[t], a0[0], a1[0], a0[1], a1[1], b.x, b.y);
       else mma_f16(c[t], a0[0], a1[0], a0[1], a1[1], b.x, b.y);
       mma_f16(c[t], a0[2], a1[2], a0[3], a1[3], b.z, b.w);
+    }
+    if (FOLD && grp % 4 == 3) {  // mma.sync truncates at each step: halves of a span are added in fp32
+#pragma unroll
+      for (unsigned t = 0; t < NT; ++t) {
+        if (P == 2) {
+          sum[t][0] += c[t][0] + c[t][1];
+          sum[t][1] += c[t][2] + c[t][3];
+        } else {
+#pragma unroll
+          for (unsigned i = 0; i < 4; ++i) sum[t][i % SV] += c[t][i];
+        }
+      }
     }
     if (!FOLD && grp % SHARE == SHARE - 1) {  // the set's sums, each lane the group of its columns
       constexpr unsigned K = COLS == 1 ? 2 : 1;
@@ -573,7 +585,7 @@ __device__ __forceinline__ void mv_span(const MvLane<P, NT, COLS>& ln, const MvF
       const float x = __uint_as_float(lds32(ln.scale[t][MvLane<P, NT, COLS>::kTok == 1 ? 0 : k] + 4 * s));
 #pragma unroll
       for (unsigned h = 0; h < 2; ++h) {
-        float v = P == 2 ? (FOLD ? c[t][2 * h] + c[t][2 * h + 1] : sum[t][h % SV]) : (FOLD ? c[t][2 * h + k] : sum[t][(2 * h + k) % SV]);
+        float v = P == 2 ? sum[t][h % SV] : sum[t][(2 * h + k) % SV];
         if (TYPE == kQ4K) v = fmaf(v, d[h], (P == 2 ? m[t][2 * h] : m[t][2 * h + k]) * dm[h]);
         acc[(2 * t + h) * A + k] = fmaf(v, x, acc[(2 * t + h) * A + k]);
       }
