@@ -277,7 +277,11 @@ int frc_matrix_close(frc_matrix *m);
  * between tokens), y: [tokens][rows] (y_type, y_stride); strides are not read
  * for one token.  x and y must not overlap.  A result that is not finite
  * (or whose x is not) sets FRC_NUMERIC in the context's device status
- * (frc_status).  Concurrent calls on several streams are independent. */
+ * (frc_status).  Concurrent calls on several streams are independent.  The
+ * same call repeats its bits; the last bits of a row may depend on where it
+ * lies in the matrix.  x is carried to 2^-30 (Q4_K, up to 4 tokens) or to 22
+ * bits and 2^-34 of the largest value among its 256 neighbours that share a
+ * block of columns. */
 int frc_matvec_device(frc_context *c, const frc_matrix *m, unsigned tokens, const void *x, size_t x_stride,
                       unsigned x_type, void *y, size_t y_stride, unsigned y_type, void *stream);
 
@@ -289,8 +293,10 @@ int frc_matvec_device(frc_context *c, const frc_matrix *m, unsigned tokens, cons
  * experts: 10..512; a logit of -inf masks its expert out.
  * valid: [tokens] bytes or NULL (all); a row with 0 is padding: its logits
  * are not looked at.  A NaN or +inf logit of a valid row sets FRC_NUMERIC in
- * the device status, and the row counts as padding.  No reference counterpart
- * (its router belongs to the external engine). */
+ * the device status, and the row counts as padding (its gradient is not
+ * defined).  A layer call behind frc_route_device on the stream must not use
+ * FRC_RUN_OVERLAP.  No reference counterpart (its router belongs to the
+ * external engine). */
 enum { FRC_ROUTE_SHARED = 1 };
 enum { FRC_ROUTE_MAX_TOKENS = 1 << 24 };
 /* FRC_OK when a routing call with these sizes is accepted.  Host only. */
