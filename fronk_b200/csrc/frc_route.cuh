@@ -225,12 +225,17 @@ __device__ __forceinline__ float exp_row(const float (&v)[kRouteSlots], float m,
   return x + y;
 }
 
-// A warp's room for its candidates: first each lane's columns, then keys.
+// A warp's room for its candidates: their columns, then their keys.
 constexpr unsigned kLaneCand = 4;
 union RouteCand {
-  uint16_t column[32][kLaneCand];
+  uint16_t column[32];
   uint64_t key[32];
 };
+// Slot of a lane's column set whose number is not known when compiled.
+template <unsigned V>
+__device__ __forceinline__ unsigned col_at(unsigned i, unsigned lane) {
+  return V == 1 ? lane + 32 * i : (i / V) * (32 * V) + V * lane + (i & (V - 1));
+}
 
 // The ten largest of a row in order, ties by the lower column: lane r < 10
 // gets the r-th one's column and value.
@@ -252,36 +257,28 @@ __device__ __forceinline__ void choose(const float (&v)[kRouteSlots], const L* r
   }
   bool done = false;
   if (bound > -INFINITY) {
-    const uint32_t mine = smem_u32(cand->column[lane]);
-    uint32_t at = mine;  // past a lane's fourth, stores go to it again
+    unsigned mine = 0, total = 0;  // the lane's slots at or above the bound
 #pragma unroll
-    for (unsigned i = 0; i < kRouteSlots; ++i)
-      if (v[i] >= bound) {
-        asm volatile("st.shared.u16 [%0], %1;" ::"r"(min(at, mine + 2 * (kLaneCand - 1))), "h"(static_cast<uint16_t>(col<V>(i, lane))) : "memory");
-        at += 2;
-      }
-    const unsigned n = (at - mine) / 2;
-    unsigned base = 0, total = 0, columns[2];
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(columns[0]), "=r"(columns[1]) : "r"(mine) : "memory");
-    __syncwarp();
-    unsigned place[kLaneCand];
-#pragma unroll
-    for (unsigned k = 0; k < kLaneCand; ++k) {
-      const unsigned m = __ballot_sync(0xffffffffu, n > k);
-      place[k] = base + __popc(m & ((1u << lane) - 1u));
-      base += __popc(m);
-    }
-    total = base;
-    done = total <= 32 && !__any_sync(0xffffffffu, n > kLaneCand);
+    for (unsigned i = 0; i < kRouteSlots; ++i) mine |= v[i] >= bound ? 1u << i : 0u;
+    done = !__any_sync(0xffffffffu, __popc(mine) > kLaneCand);
     if (done) {
-      uint16_t* list = &cand->column[0][0];
+      const unsigned before = (1u << lane) - 1u;
 #pragma unroll
-      for (unsigned k = 0; k < kLaneCand; ++k)
-        if (n > k) list[place[k]] = static_cast<uint16_t>(columns[k / 2] >> (16 * (k & 1)));
+      for (unsigned k = 0; k < kLaneCand; ++k) {
+        const unsigned with = __ballot_sync(0xffffffffu, mine);
+        if (!with) break;
+        const unsigned place = total + __popc(with & before);
+        if (mine && place < 32) cand->column[place] = static_cast<uint16_t>(col_at<V>(__ffs(mine) - 1, lane));
+        mine &= mine - 1;
+        total += __popc(with);
+      }
+      done = total <= 32;
+    }
+    if (done) {
       __syncwarp();
       uint64_t key = 0;
       if (lane < total) {
-        const unsigned c = list[lane];
+        const unsigned c = cand->column[lane];
         key = static_cast<uint64_t>(order_key(logit(row + c) + 0.0f)) << 32 | ~c;  // -0 becomes +0: equal logits are ties
       }
       __syncwarp();
@@ -526,6 +523,8 @@ __global__ void __cluster_dims__(kRouteCluster, 1, 1) __launch_bounds__(kFinishT
   __shared__ unsigned s_c[kFinishSplit][kMaxExperts / kRouteCluster];
   const unsigned own = kMaxExperts / kRouteCluster, i = threadIdx.x % own, k0 = threadIdx.x / own;
   const unsigned e = cluster_rank() * own + i;
+  // the first CTA gets the terms of the others in its shared memory: it must have started by then
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   double p = 0.0;
   unsigned c = 0;
@@ -556,6 +555,8 @@ __global__ void __cluster_dims__(kRouteCluster, 1, 1) __launch_bounds__(kFinishT
     }
     term = finish_expert(f, e, p, c, n);
   }
+  __syncwarp();  // the barriers are a whole warp's
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   finish_loss(f, term, n, s_term);
 }
 

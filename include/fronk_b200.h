@@ -292,9 +292,10 @@ int frc_matvec_device(frc_context *c, const frc_matrix *m, unsigned tokens, cons
  * FRC_ROUTE_SHARED column `experts` holds the shared expert's gate logit.
  * experts: 10..512; a logit of -inf masks its expert out.
  * valid: [tokens] bytes or NULL (all); a row with 0 is padding: its logits
- * are not looked at.  A NaN or +inf logit of a valid row sets FRC_NUMERIC in
- * the device status, and the row counts as padding (its gradient is not
- * defined).  A layer call behind frc_route_device on the stream must not use
+ * are not looked at.  A NaN or +inf expert logit of a valid row sets
+ * FRC_NUMERIC in the device status, and the row counts as padding (its
+ * gradient is not defined); a NaN shared logit sets it and its gate is 0.  A
+ * layer call behind frc_route_device on the stream must not use
  * FRC_RUN_OVERLAP.  No reference counterpart (its router belongs to the
  * external engine). */
 enum { FRC_ROUTE_SHARED = 1 };
