@@ -85,6 +85,12 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (unsigned o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// Over lanes 0-15, for each of them.
+__device__ __forceinline__ float chosen_sum(float v) {
+#pragma unroll
+  for (unsigned o = 8; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
 // Maxima that are NaN when a value is.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
@@ -99,6 +105,11 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 __device__ __forceinline__ float warp_max(float v) {
   float d;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
+  return d;
+}
+__device__ __forceinline__ float warp_min(float v) {
+  float d;
+  asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
   return d;
 }
 __device__ __forceinline__ float rcp(float v) {  // within one step; v is a sum of exponentials, at least 1
@@ -228,6 +239,7 @@ __device__ __forceinline__ float exp_row(const float (&v)[kRouteSlots], float m,
 // A warp's room for its candidates: their columns, then their keys.
 constexpr unsigned kLaneCand = 4;
 union RouteCand {
+  __nv_bfloat16 top[32];
   uint16_t column[32];
   uint64_t key[32];
 };
@@ -248,13 +260,25 @@ __device__ __forceinline__ unsigned col_at(unsigned i, unsigned lane) {
 // the whole row choose one by one.
 template <typename L, unsigned V>
 __device__ __forceinline__ void choose(const float (&v)[kRouteSlots], const L* row, unsigned E, unsigned lane, float top,
-                                       RouteCand* cand, unsigned* id, float* val) {
-  float rest = top, bound = 0.0f;
+                                       float m, RouteCand* cand, unsigned* id, float* val) {
+  const __nv_bfloat16 rough = __float2bfloat16_rn(top - m);
+  cand->top[lane] = rough;
+  __syncwarp();
+  const __nv_bfloat162 own = __bfloat162bfloat162(rough);
+  __nv_bfloat162 above[4];
 #pragma unroll
-  for (unsigned r = 0; r < kTopK; ++r) {
-    bound = warp_max(rest);
-    rest = rest == bound ? -INFINITY : rest;
+  for (unsigned k = 0; k < 4; ++k) {
+    const uint4 w = reinterpret_cast<const uint4*>(cand->top)[k];
+    const uint32_t o[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j) {
+      const __nv_bfloat162 gt = __hgt2(*reinterpret_cast<const __nv_bfloat162*>(&o[j]), own);
+      above[j] = k ? __hadd2(above[j], gt) : gt;
+    }
   }
+  const __nv_bfloat162 sum = __hadd2(__hadd2(above[0], above[1]), __hadd2(above[2], above[3]));
+  const float bound = warp_min(__low2float(sum) + __high2float(sum) < kTopK ? top : INFINITY);
+  __syncwarp();
   bool done = false;
   if (bound > -INFINITY) {
     unsigned mine = 0, total = 0;  // the lane's slots at or above the bound
@@ -426,9 +450,9 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteP
     if (SELECT) {
       float g = 0.0f;
       if (use) {
-        choose<L, V>(v, row, E, lane, top, &s_cand[warp], &id, &val);
+        choose<L, V>(v, row, E, lane, top, m, &s_cand[warp], &id, &val);
         const float e = lane < kTopK && m > -INFINITY ? expf(val - m) : 0.0f;
-        const float sum = warp_sum(e);
+        const float sum = chosen_sum(e);
         g = sum > 0.0f ? e * rcp(sum) : 0.0f;
         if (lane == kTopK && a.shared) {
           const float s = logit(row + E);
