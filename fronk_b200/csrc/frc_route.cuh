@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteP
     __syncthreads();
   }
   const unsigned step = gridDim.x * warps;
-  unsigned t = blockIdx.x * warps + warp;
+  unsigned t = warp * gridDim.x + blockIdx.x;  // runs of padding are dealt over the CTAs
   RowLoad<L, V, FULL> next;
   bool next_valid = false;
   unsigned next_id = 0;
