@@ -25,7 +25,9 @@ namespace frc {
 constexpr unsigned kTopK = 10, kGates = 11, kMaxExperts = 512;
 constexpr unsigned kRouteSlots = kMaxExperts / 32;  // logits a lane holds
 constexpr unsigned kRouteWarps = 24;                // warps a CTA, at most
+constexpr unsigned kStagedWarps = 32;               // warps a CTA whose rows come through shared memory
 constexpr unsigned kRouteSums = 16;                 // arrays of sums a CTA folds its warps into; warps of a cluster's CTA
+constexpr unsigned kRouteRows = 8;                  // rows a CTA that makes statistics, at least, while SMs are free
 constexpr unsigned kRouteCtas = 160;                // CTAs that make statistics (one an SM), at most
 constexpr unsigned kRouteCluster = 8;               // CTAs that finish them
 
@@ -217,6 +219,23 @@ struct RowLoad {
   }
 };
 
+// A row on its way through shared memory: a lane fetches the columns that it
+// holds into the warp's buffer, columns past E are -inf.
+template <typename L, unsigned V, bool FULL>
+__device__ __forceinline__ void stage_row(L* buf, const L* row, unsigned E, unsigned lane) {
+  static_assert(V * sizeof(L) == 16, "16 bytes a copy");
+#pragma unroll
+  for (unsigned j = 0; j < kRouteSlots / V; ++j) {
+    const unsigned c = col<V>(j * V, lane);
+    if (FULL || c + V <= E) {
+      cp_async16(buf + c, row + c);
+    } else {
+#pragma unroll
+      for (unsigned k = 0; k < V; ++k) buf[c + k] = c + k < E ? row[c + k] : static_cast<L>(-INFINITY);
+    }
+  }
+}
+
 // e = exp(v - m) of a lane's slots, in pairs; returns their sum.
 __device__ __forceinline__ float exp_row(const float (&v)[kRouteSlots], float m, F2 (&e)[kRouteSlots / 2]) {
   const F2 shift = pack2(-m, -m), log2e = pack2(1.4426950408889634f, 1.4426950408889634f);
@@ -398,15 +417,28 @@ __device__ __forceinline__ void finish_loss(const RouteFinish& f, double term, u
 // Statistics: none, as parts for route_finish_kernel, or finished by the one
 // cluster that runs (few rows).
 enum : int { kStatsNone = 0, kStatsParts = 1, kStatsCluster = 2 };
+// Warps of route_kernel, and whether its rows come through shared memory: many
+// aligned rows, two buffers a warp.  That leaves registers for 32 warps where
+// holding the next row in registers leaves them for 24.
+template <unsigned V, int STATS, bool MANY>
+struct RouteShape {
+  static constexpr bool kStaged = MANY && V > 1;
+  static constexpr unsigned kWarps = kStaged ? kStagedWarps : kRouteWarps;
+};
 
 // One warp a row; SELECT: choose experts and gates; STATS: sums of p and
 // counts of the chosen (or given) experts over the CTA's rows.  The next
 // row's logits are on their way while one is worked on.
-template <typename L, unsigned V, bool FULL, bool SELECT, int STATS>
-__global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteParams a, const RouteFinish f) {
-  __shared__ float s_psum[STATS ? kRouteSums : 1][STATS ? kMaxExperts : 1];
+template <typename L, unsigned V, bool FULL, bool SELECT, int STATS, bool MANY>
+__global__ void __launch_bounds__(32 * RouteShape<V, STATS, MANY>::kWarps, 1) route_kernel(const RouteParams a, const RouteFinish f) {
+  using Shape = RouteShape<V, STATS, MANY>;
+  extern __shared__ __align__(16) uint8_t s_rows[];  // [warps][2][kMaxExperts] of L where rows are staged
+  constexpr unsigned kSums = Shape::kStaged ? Shape::kWarps : kRouteSums;
+  constexpr bool kOwnSums = STATS && !Shape::kStaged;  // else they lie where the rows passed through
+  __shared__ __align__(16) float s_sums[kOwnSums ? kSums : 1][kOwnSums ? kMaxExperts : 1];
+  float(*const s_psum)[kMaxExperts] = reinterpret_cast<float(*)[kMaxExperts]>(Shape::kStaged ? reinterpret_cast<float*>(s_rows) : &s_sums[0][0]);
   __shared__ unsigned s_count[STATS ? kMaxExperts : 1], s_valid;
-  __shared__ __align__(16) RouteCand s_cand[SELECT ? kRouteWarps : 1];
+  __shared__ __align__(16) RouteCand s_cand[SELECT ? Shape::kWarps : 1];
   __shared__ double s_term[kRouteCluster * kOwnWarps];
   const unsigned warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = blockDim.x / 32, E = a.experts;
   const L* logits = static_cast<const L*>(a.logits);
@@ -424,16 +456,29 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteP
   RowLoad<L, V, FULL> next;
   bool next_valid = false;
   unsigned next_id = 0;
+  L* stage = reinterpret_cast<L*>(s_rows) + 2 * kMaxExperts * warp;
+  unsigned side = 0;  // the buffer that takes the next row
   const auto fetch = [&](unsigned r) {
     next_valid = !a.valid || a.valid[r];
     if (STATS && !SELECT && lane < kTopK) next_id = a.expert_in[r * kTopK + lane];
-    next.load(logits + r * a.stride, E, lane);
+    if constexpr (Shape::kStaged) {
+      stage_row<L, V, FULL>(stage + side, logits + r * a.stride, E, lane);
+      side ^= kMaxExperts;
+    } else {
+      next.load(logits + r * a.stride, E, lane);
+    }
   };
   if (t < a.tokens) fetch(t);
   for (; t < a.tokens; t += step) {
-    const L* row = logits + t * a.stride;
+    const L* row = logits + t * a.stride;  // where single logits are read again
     const bool valid = next_valid;
     float v[kRouteSlots];
+    if constexpr (Shape::kStaged) {
+      row = stage + (side ^ kMaxExperts);
+      cp_async_wait_all();
+      __syncwarp();
+      next.load(row, kMaxExperts, lane);
+    }
 #pragma unroll
     for (unsigned i = 0; i < kRouteSlots; ++i) v[i] = next.value(i);
     unsigned id = lane;
@@ -455,7 +500,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteP
         const float sum = chosen_sum(e);
         g = sum > 0.0f ? e * rcp(sum) : 0.0f;
         if (lane == kTopK && a.shared) {
-          const float s = logit(row + E);
+          const float s = logit(logits + t * a.stride + E);
           g = sigmoid(s);
           if (s != s) {
             g = 0.0f;
@@ -485,21 +530,31 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 1) route_kernel(const RouteP
   if (STATS) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (lane == 0) atomicAdd(&s_valid, nvalid);
-    for (unsigned w = 0; w < warps; w += kRouteSums) {  // in a fixed order
-      if (warp >= w && warp < w + kRouteSums)
+    if (Shape::kStaged) __syncthreads();
+    for (unsigned w = 0; w < warps; w += kSums) {  // in a fixed order
+      if (warp >= w && warp < w + kSums)
 #pragma unroll
-        for (unsigned i = 0; i < kRouteSlots; ++i) {
-          float x, y;
-          unpack2(psum[i / 2], x, y);
-          float* p = &s_psum[warp - w][col<V>(i, lane)];
-          *p = (w ? *p : 0.0f) + (i & 1 ? y : x);
+        for (unsigned i = 0; i < kRouteSlots / 2; i += 2) {
+          float x[4];
+          unpack2(psum[i], x[0], x[1]);
+          unpack2(psum[i + 1], x[2], x[3]);
+          float* p = &s_psum[warp - w][col<V>(2 * i, lane)];
+          if constexpr (V > 1) {
+            float4 q = w ? *reinterpret_cast<const float4*>(p) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            q.x += x[0]; q.y += x[1]; q.z += x[2]; q.w += x[3];
+            *reinterpret_cast<float4*>(p) = q;
+          } else {
+#pragma unroll
+            for (unsigned k = 0; k < 4; ++k) p[32 * k] = (w ? p[32 * k] : 0.0f) + x[k];
+          }
         }
       __syncthreads();
     }
-    const unsigned sums = warps < kRouteSums ? warps : kRouteSums;
+    const unsigned sums = warps < kSums ? warps : kSums;
     if (STATS == kStatsParts) {
       for (unsigned e = threadIdx.x; e < E; e += blockDim.x) {
         float s = 0.0f;
+#pragma unroll 8
         for (unsigned w = 0; w < sums; ++w) s += s_psum[w][e];
         a.part[static_cast<size_t>(blockIdx.x) * E + e] = make_float2(s, __uint_as_float(s_count[e]));
       }
@@ -755,7 +810,7 @@ constexpr unsigned kRouteOneCluster = 512;
 
 // CTAs that make statistics of `tokens` rows: one part of the sums each.
 inline unsigned route_parts(unsigned tokens, unsigned sms) {
-  const unsigned n = (tokens + kRouteWarps - 1) / kRouteWarps;
+  const unsigned n = (tokens + kRouteRows - 1) / kRouteRows;
   return n < sms ? n : sms;
 }
 inline bool rows_aligned(const void* p, size_t stride, size_t size) {
@@ -776,8 +831,27 @@ inline cudaError_t launch_finish(const RouteFinish& f, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, route_finish_kernel, f);
 }
 
+// route_kernel for many rows.
+template <typename L, unsigned V, bool FULL, bool SELECT, int STATS>
+inline cudaError_t launch_many(const RouteParams& a, const RouteFinish& f, unsigned ctas, int device, cudaStream_t s) {
+  using Shape = RouteShape<V, STATS, true>;
+  constexpr unsigned smem = Shape::kStaged ? Shape::kWarps * 2 * kMaxExperts * sizeof(L) : 0;
+  static_assert(!smem || Shape::kWarps * kMaxExperts * sizeof(float) <= smem, "the warps' sums");
+  const unsigned rows = (a.tokens + ctas - 1) / ctas, warps = rows < Shape::kWarps ? rows : Shape::kWarps;
+  static std::atomic<unsigned long long> allowed{0};  // devices on which the kernel may take its shared memory
+  const unsigned long long bit = 1ull << (device & 63);
+  if (smem > 48 * 1024 && (device > 63 || !(allowed.load(std::memory_order_relaxed) & bit))) {
+    const cudaError_t e = cudaFuncSetAttribute(route_kernel<L, V, FULL, SELECT, STATS, true>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  route_kernel<L, V, FULL, SELECT, STATS, true><<<ctas, 32 * warps, smem / Shape::kWarps * warps, s>>>(a, f);
+  return cudaGetLastError();
+}
+
 template <typename L, unsigned V, bool FULL, bool SELECT>
-inline cudaError_t launch_stats(const RouteParams& a, const RouteFinish& f, unsigned sms, cudaStream_t s) {
+inline cudaError_t launch_stats(const RouteParams& a, const RouteFinish& f, int device, cudaStream_t s) {
   if (a.tokens <= kRouteOneCluster) {
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
@@ -789,35 +863,38 @@ inline cudaError_t launch_stats(const RouteParams& a, const RouteFinish& f, unsi
     cfg.stream = s;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, route_kernel<L, V, FULL, SELECT, kStatsCluster>, a, f);
+    return cudaLaunchKernelEx(&cfg, route_kernel<L, V, FULL, SELECT, kStatsCluster, false>, a, f);
   }
-  route_kernel<L, V, FULL, SELECT, kStatsParts><<<f.parts, 32 * kRouteWarps, 0, s>>>(a, f);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_many<L, V, FULL, SELECT, kStatsParts>(a, f, f.parts, device, s);
   return e == cudaSuccess ? launch_finish(f, s) : e;
 }
 
 template <typename L, unsigned V, bool FULL>
 inline cudaError_t launch_route(const RouteParams& a, const RouteFinish& f, bool select, bool stats, unsigned sms,
-                                cudaStream_t s) {
-  if (stats) return select ? launch_stats<L, V, FULL, true>(a, f, sms, s) : launch_stats<L, V, FULL, false>(a, f, sms, s);
+                                int device, cudaStream_t s) {
+  if (stats) return select ? launch_stats<L, V, FULL, true>(a, f, device, s) : launch_stats<L, V, FULL, false>(a, f, device, s);
   // few rows: four warps a CTA spread them over the SMs
-  const unsigned warps = a.tokens <= 8 * sms ? 4 : kRouteWarps, ctas = (a.tokens + warps - 1) / warps;
-  route_kernel<L, V, FULL, true, kStatsNone><<<warps == 4 || ctas < sms ? ctas : sms, 32 * warps, 0, s>>>(a, f);
-  return cudaGetLastError();
+  if (a.tokens <= 8 * sms) {
+    route_kernel<L, V, FULL, true, kStatsNone, false><<<(a.tokens + 3) / 4, 128, 0, s>>>(a, f);
+    return cudaGetLastError();
+  }
+  constexpr unsigned warps = RouteShape<V, kStatsNone, true>::kWarps;
+  const unsigned ctas = (a.tokens + warps - 1) / warps;
+  return launch_many<L, V, FULL, true, kStatsNone>(a, f, ctas < sms ? ctas : sms, device, s);
 }
 inline cudaError_t launch_route(const RouteParams& a, const RouteFinish& f, unsigned type, bool select, bool stats,
-                                unsigned sms, cudaStream_t s) {
+                                unsigned sms, int device, cudaStream_t s) {
   const size_t size = type == FRC_BF16 ? 2 : 4;
   // neighbours a lane only where they leave no lane without logits: the
   // bound on the tenth largest needs the lanes' maxima
   const bool vec = rows_aligned(a.logits, a.stride, size) && a.experts * size >= 512;
   const bool full = a.experts == kMaxExperts;
   if (type == FRC_BF16) {
-    if (vec) return full ? launch_route<__nv_bfloat16, 8, true>(a, f, select, stats, sms, s) : launch_route<__nv_bfloat16, 8, false>(a, f, select, stats, sms, s);
-    return full ? launch_route<__nv_bfloat16, 1, true>(a, f, select, stats, sms, s) : launch_route<__nv_bfloat16, 1, false>(a, f, select, stats, sms, s);
+    if (vec) return full ? launch_route<__nv_bfloat16, 8, true>(a, f, select, stats, sms, device, s) : launch_route<__nv_bfloat16, 8, false>(a, f, select, stats, sms, device, s);
+    return full ? launch_route<__nv_bfloat16, 1, true>(a, f, select, stats, sms, device, s) : launch_route<__nv_bfloat16, 1, false>(a, f, select, stats, sms, device, s);
   }
-  if (vec) return full ? launch_route<float, 4, true>(a, f, select, stats, sms, s) : launch_route<float, 4, false>(a, f, select, stats, sms, s);
-  return full ? launch_route<float, 1, true>(a, f, select, stats, sms, s) : launch_route<float, 1, false>(a, f, select, stats, sms, s);
+  if (vec) return full ? launch_route<float, 4, true>(a, f, select, stats, sms, device, s) : launch_route<float, 4, false>(a, f, select, stats, sms, device, s);
+  return full ? launch_route<float, 1, true>(a, f, select, stats, sms, device, s) : launch_route<float, 1, false>(a, f, select, stats, sms, device, s);
 }
 
 template <typename L, unsigned V, bool FULL>
