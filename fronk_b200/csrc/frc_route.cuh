@@ -25,7 +25,6 @@ namespace frc {
 constexpr unsigned kTopK = 10, kGates = 11, kMaxExperts = 512;
 constexpr unsigned kRouteSlots = kMaxExperts / 32;  // logits a lane holds
 constexpr unsigned kRouteWarps = 24;                // warps a CTA, at most
-constexpr unsigned kStagedWarps = 32;               // warps a CTA whose rows come through shared memory
 constexpr unsigned kRouteSums = 16;                 // arrays of sums a CTA folds its warps into; warps of a cluster's CTA
 constexpr unsigned kRouteRows = 8;                  // rows a CTA that makes statistics, at least, while SMs are free
 constexpr unsigned kRouteCtas = 160;                // CTAs that make statistics (one an SM), at most
@@ -417,21 +416,22 @@ __device__ __forceinline__ void finish_loss(const RouteFinish& f, double term, u
 // Statistics: none, as parts for route_finish_kernel, or finished by the one
 // cluster that runs (few rows).
 enum : int { kStatsNone = 0, kStatsParts = 1, kStatsCluster = 2 };
-// Warps of route_kernel, and whether its rows come through shared memory: many
-// aligned rows, two buffers a warp.  That leaves registers for 32 warps where
-// holding the next row in registers leaves them for 24.
-template <unsigned V, int STATS, bool MANY>
+// Warps of a CTA, and whether its rows come through shared memory: many
+// aligned rows, two buffers a warp.  Without the next row in registers there is
+// room for 32 warps, or 28 where experts are chosen and sums kept (65,536 rows
+// of 512, all of it: 44.7 us; with 24 warps 46.5, with 32, which spill, 45.7).
+template <unsigned V, bool SELECT, int STATS, bool MANY>
 struct RouteShape {
   static constexpr bool kStaged = MANY && V > 1;
-  static constexpr unsigned kWarps = kStaged ? kStagedWarps : kRouteWarps;
+  static constexpr unsigned kWarps = !kStaged ? kRouteWarps : SELECT && STATS ? 28 : 32;
 };
 
 // One warp a row; SELECT: choose experts and gates; STATS: sums of p and
 // counts of the chosen (or given) experts over the CTA's rows.  The next
 // row's logits are on their way while one is worked on.
 template <typename L, unsigned V, bool FULL, bool SELECT, int STATS, bool MANY>
-__global__ void __launch_bounds__(32 * RouteShape<V, STATS, MANY>::kWarps, 1) route_kernel(const RouteParams a, const RouteFinish f) {
-  using Shape = RouteShape<V, STATS, MANY>;
+__global__ void __launch_bounds__(32 * RouteShape<V, SELECT, STATS, MANY>::kWarps, 1) route_kernel(const RouteParams a, const RouteFinish f) {
+  using Shape = RouteShape<V, SELECT, STATS, MANY>;
   extern __shared__ __align__(16) uint8_t s_rows[];  // [warps][2][kMaxExperts] of L where rows are staged
   constexpr unsigned kSums = Shape::kStaged ? Shape::kWarps : kRouteSums;
   constexpr bool kOwnSums = STATS && !Shape::kStaged;  // else they lie where the rows passed through
@@ -595,6 +595,7 @@ __global__ void __launch_bounds__(32 * RouteShape<V, STATS, MANY>::kWarps, 1) ro
 
 // Sums the CTAs' parts in order, in double, and forms the loss: one cluster,
 // 16 threads an expert that take every 16th part, all of them in flight.
+static_assert(kRouteCtas % 32 == 0, "whole warps of parts");
 constexpr unsigned kFinishSplit = 16, kFinishThreads = kMaxExperts / kRouteCluster * kFinishSplit;
 __global__ void __cluster_dims__(kRouteCluster, 1, 1) __launch_bounds__(kFinishThreads)
     route_finish_kernel(const RouteFinish f) {
@@ -606,7 +607,12 @@ __global__ void __cluster_dims__(kRouteCluster, 1, 1) __launch_bounds__(kFinishT
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   double p = 0.0;
-  unsigned c = 0;
+  unsigned c = 0, valid[kRouteCtas / 32], n = 0;
+#pragma unroll
+  for (unsigned j = 0; j < kRouteCtas / 32; ++j) {
+    const unsigned k = 32 * j + (threadIdx.x & 31);
+    valid[j] = k < f.parts ? f.pvalid[k] : 0u;
+  }
   if (e < f.experts) {
     float2 v[kRouteCtas / kFinishSplit];
 #pragma unroll
@@ -620,8 +626,8 @@ __global__ void __cluster_dims__(kRouteCluster, 1, 1) __launch_bounds__(kFinishT
       c += __float_as_uint(v[j].y);
     }
   }
-  unsigned n = 0;
-  for (unsigned k = threadIdx.x & 31; k < f.parts; k += 32) n += f.pvalid[k];
+#pragma unroll
+  for (unsigned j = 0; j < kRouteCtas / 32; ++j) n += valid[j];
   n = __reduce_add_sync(0xffffffffu, n);
   s_p[k0][i] = p;
   s_c[k0][i] = c;
@@ -834,13 +840,13 @@ inline cudaError_t launch_finish(const RouteFinish& f, cudaStream_t s) {
 // route_kernel for many rows.
 template <typename L, unsigned V, bool FULL, bool SELECT, int STATS>
 inline cudaError_t launch_many(const RouteParams& a, const RouteFinish& f, unsigned ctas, int device, cudaStream_t s) {
-  using Shape = RouteShape<V, STATS, true>;
+  using Shape = RouteShape<V, SELECT, STATS, true>;
   constexpr unsigned smem = Shape::kStaged ? Shape::kWarps * 2 * kMaxExperts * sizeof(L) : 0;
   static_assert(!smem || Shape::kWarps * kMaxExperts * sizeof(float) <= smem, "the warps' sums");
   const unsigned rows = (a.tokens + ctas - 1) / ctas, warps = rows < Shape::kWarps ? rows : Shape::kWarps;
   static std::atomic<unsigned long long> allowed{0};  // devices on which the kernel may take its shared memory
   const unsigned long long bit = 1ull << (device & 63);
-  if (smem > 48 * 1024 && (device > 63 || !(allowed.load(std::memory_order_relaxed) & bit))) {
+  if (smem && (device > 63 || !(allowed.load(std::memory_order_relaxed) & bit))) {
     const cudaError_t e = cudaFuncSetAttribute(route_kernel<L, V, FULL, SELECT, STATS, true>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
@@ -878,9 +884,7 @@ inline cudaError_t launch_route(const RouteParams& a, const RouteFinish& f, bool
     route_kernel<L, V, FULL, true, kStatsNone, false><<<(a.tokens + 3) / 4, 128, 0, s>>>(a, f);
     return cudaGetLastError();
   }
-  constexpr unsigned warps = RouteShape<V, kStatsNone, true>::kWarps;
-  const unsigned ctas = (a.tokens + warps - 1) / warps;
-  return launch_many<L, V, FULL, true, kStatsNone>(a, f, ctas < sms ? ctas : sms, device, s);
+  return launch_many<L, V, FULL, true, kStatsNone>(a, f, sms, device, s);
 }
 inline cudaError_t launch_route(const RouteParams& a, const RouteFinish& f, unsigned type, bool select, bool stats,
                                 unsigned sms, int device, cudaStream_t s) {
