@@ -714,12 +714,22 @@ __global__ void __launch_bounds__(256, BALANCE ? 3 : 6) route_backward_kernel(co
     if (BALANCE) next.load(logits + t * a.stride, E, lane);
   }
   if (BALANCE) {
-    const float n = static_cast<float>(a.count[E]);
-    const float scale = n > 0.0f ? *a.d_loss * static_cast<float>(E) / (static_cast<float>(kTopK) * n * n) : 0.0f;
-    for (unsigned e = threadIdx.x; e < kMaxExperts; e += blockDim.x) s_k[e] = e < E ? scale * static_cast<float>(a.count[e]) : 0.0f;
-    __syncthreads();
-    for (unsigned i = threadIdx.x; i < kMaxExperts; i += blockDim.x)
-      s_slots[i / 128][i / 4 % 32][i % 4] = s_k[col<V>(i / 128 * 4 + i % 4, i / 4 % 32)];
+    unsigned count[4];  // all of a thread's loads at once
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j) {
+      const unsigned e = threadIdx.x + j * blockDim.x;
+      count[j] = e < E ? a.count[e] : 0u;
+    }
+    const float n = static_cast<float>(a.count[E]), d_loss = *a.d_loss;
+    const float scale = n > 0.0f ? d_loss * static_cast<float>(E) / (static_cast<float>(kTopK) * n * n) : 0.0f;
+#pragma unroll
+    for (unsigned j = 0; j < 4; ++j) {
+      const unsigned e = threadIdx.x + j * blockDim.x;
+      if (e < kMaxExperts) {
+        const unsigned i = e / (32 * V) * V + e % V;  // the column's slot
+        s_k[e] = s_slots[i / 4][e / V % 32][i % 4] = scale * static_cast<float>(count[j]);
+      }
+    }
     __syncthreads();
   }
   if (t < a.tokens) {
