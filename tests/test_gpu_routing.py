@@ -288,6 +288,37 @@ def test_gradient_against_differences(ctx):
             assert abs((value(up) - value(down)) / (2 * h) - float(out[t, e])) < 1e-6 * (1 + abs(c[t]).max())
 
 
+@pytest.mark.parametrize("kind", ["normal", "ties", "zeros", "masked", "few", "lowest"])
+@pytest.mark.parametrize("T,E,dtype,pad", [(1301, 300, fb.F32, 0), (1400, 130, fb.F32, 2), (4999, 512, fb.F32, 4),
+                                           (5000, 512, fb.BF16, 0), (1300, 261, fb.BF16, 3), (1299, 505, fb.BF16, 7)])
+def test_large_calls(ctx, kind, T, E, dtype, pad):
+    """Rows that pass through shared memory: aligned ones of many tokens, the last columns partly past E."""
+    import torch
+    rng = np.random.default_rng(T * 13 + E)
+    shared = rng.standard_normal(T) if E in (261, 505) else None
+    valid = rng.random(T) < 0.7
+    b = Buffers(logits_of(kind, T, E, rng), dtype, pad=pad - (shared is not None), valid=valid, shared=shared)
+    assert b.stride * b.logits.element_size() % 16 == 0
+    l, sh = b.seen()
+    ref = Reference(l, valid, sh)
+    b.route(ctx)
+    assert ctx.status() == fb.OK
+    check_route(b, ref)
+    ids = b.expert.clone()
+    b.expert.fill_(-1)
+    b.gate.fill_(float("nan"))
+    b.route(ctx, balance=True)
+    assert ctx.status() == fb.OK
+    check_route(b, ref)
+    check_stats(b, ref)
+    assert bool(torch.equal(ids, b.expert))
+    b.count.fill_(-1)
+    b.prob.fill_(-1)
+    b.stats(ctx, ids)
+    assert ctx.status() == fb.OK
+    check_stats(b, ref)
+
+
 @pytest.mark.parametrize("E", [512, 100])
 def test_many_rows(ctx, E):
     """More rows than the GPU's warps; statistics summed over all of them."""
