@@ -10,10 +10,11 @@
 // expert), prob_e = mean p_e, loss = E sum_e count_e / (10 N) prob_e.
 //
 // A warp takes a row, 16 logits a lane; the logits' bytes bound it.  Measured
-// on one B200, graph replays, 512 experts fp32: statistics of 65,536 rows 28.9
-// us (4.7 TB/s), selection and statistics of 16,384 rows 20.8 us (480
-// instructions a row bound it), both gradients of 16,384 rows 15.8 us (17.8
-// with rows that are not 16-byte aligned), one row's selection 2.4 us.
+// on one B200, graph replays, 512 experts fp32: statistics of 65,536 rows 27.0
+// us (5.0 TB/s), selection and statistics of 16,384 rows 17.5 us and of 65,536
+// rows 44.5 (440 instructions a row bound it), both gradients of 16,384 rows
+// 14.7 us (16.7 with rows that are not 16-byte aligned), one row's selection
+// 2.4 us.
 #pragma once
 #include <cuda_bf16.h>
 
@@ -271,7 +272,8 @@ __device__ __forceinline__ unsigned col_at(unsigned i, unsigned lane) {
 // gets the r-th one's column and value.
 //
 // The tenth largest of the lanes' maxima bounds the tenth largest logit from
-// below, so only the logits at or above it (a dozen as a rule) are collected
+// below (a lane's rank is counted among all lanes' distances from the largest
+// rounded to bf16: any rounding leaves ten maxima at or above the bound), so only the logits at or above it (a dozen as a rule) are collected
 // and ranked against one another by {order of the value, lower column first}
 // as one integer.  Where a lane has more than four of them or the warp more
 // than 32 (ties), or the bound is -inf (few logits left), ten searches over
@@ -428,7 +430,9 @@ struct RouteShape {
 
 // One warp a row; SELECT: choose experts and gates; STATS: sums of p and
 // counts of the chosen (or given) experts over the CTA's rows.  The next
-// row's logits are on their way while one is worked on.
+// row's logits are on their way while one is worked on.  Neighbouring rows go
+// to different CTAs: runs of padding rows leave none idle (a ragged batch of
+// 16,384 rows 19.0 us, with 24 neighbours a CTA 19.9).
 template <typename L, unsigned V, bool FULL, bool SELECT, int STATS, bool MANY>
 __global__ void __launch_bounds__(32 * RouteShape<V, SELECT, STATS, MANY>::kWarps, 1) route_kernel(const RouteParams a, const RouteFinish f) {
   using Shape = RouteShape<V, SELECT, STATS, MANY>;
@@ -452,7 +456,7 @@ __global__ void __launch_bounds__(32 * RouteShape<V, SELECT, STATS, MANY>::kWarp
     __syncthreads();
   }
   const unsigned step = gridDim.x * warps;
-  unsigned t = warp * gridDim.x + blockIdx.x;  // runs of padding are dealt over the CTAs
+  unsigned t = warp * gridDim.x + blockIdx.x;
   RowLoad<L, V, FULL> next;
   bool next_valid = false;
   unsigned next_id = 0;
