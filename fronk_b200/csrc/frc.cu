@@ -1915,7 +1915,7 @@ static int route(frc_context* c, unsigned tokens, unsigned experts, const void* 
   RouteFinish f{};
   if (b) f = RouteFinish{a.part, a.pvalid, parts, experts, b->loss, b->count, b->prob};
   CK(launch_route(a, f, type, expert_in == nullptr, b != nullptr, sms, c->device, s));
-  c->launches += b && tokens > kRouteOneCluster ? 2 : 1;
+  c->launches += b && !route_one_cluster(tokens, expert_in == nullptr) ? 2 : 1;
   return FRC_OK;
 }
 

@@ -823,10 +823,12 @@ __global__ void __launch_bounds__(256, BALANCE ? 3 : 6) route_backward_kernel(co
 
 // ------------------------------------------------------------ host side
 
-// Up to this many rows one cluster makes the statistics in one launch
-// (measured at 512 experts: 20 rows 4.0 us, 333 rows 5.9, 1,000 rows 9.5; a
-// CTA an SM and the launch that joins them take 7.1 at 1,500 rows).
-constexpr unsigned kRouteOneCluster = 512;
+// Whether one cluster makes the statistics in one launch.  Measured at 512
+// experts fp32, one cluster against CTAs of eight rows and the launch that
+// joins them: statistics of 250 rows 5.3 and 5.2 us, of 512 rows 6.7 and 5.5,
+// of 700 rows 8.0 and 6.0; with the selection 100 rows 5.8 and 6.1, 160 rows
+// 7.4 and 6.2, 250 rows 8.1 and 6.5.  The second launch costs the host 1.2 us.
+inline bool route_one_cluster(unsigned tokens, bool select) { return tokens <= (select ? 160 : 512); }
 
 // CTAs that make statistics of `tokens` rows: one part of the sums each.
 inline unsigned route_parts(unsigned tokens, unsigned sms) {
@@ -872,7 +874,7 @@ inline cudaError_t launch_many(const RouteParams& a, const RouteFinish& f, unsig
 
 template <typename L, unsigned V, bool FULL, bool SELECT>
 inline cudaError_t launch_stats(const RouteParams& a, const RouteFinish& f, int device, cudaStream_t s) {
-  if (a.tokens <= kRouteOneCluster) {
+  if (route_one_cluster(a.tokens, SELECT)) {
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
     at.val.clusterDim.x = kRouteCluster;

@@ -319,6 +319,29 @@ def test_large_calls(ctx, kind, T, E, dtype, pad):
     check_stats(b, ref)
 
 
+@pytest.mark.parametrize("T", [160, 161, 168, 169, 512, 513, 520])
+@pytest.mark.parametrize("E,dtype", [(512, fb.F32), (37, fb.F32), (300, fb.BF16)])
+def test_calls_of_hundreds(ctx, T, E, dtype):
+    """Around the sizes where statistics change from one cluster to a CTA for eight rows and a launch behind them."""
+    rng = np.random.default_rng(T * 7 + E)
+    valid = rng.random(T) < 0.8
+    b = Buffers(rng.standard_normal((T, E)) * 2, dtype, valid=valid)
+    ref = Reference(b.seen()[0], valid)
+    b.route(ctx, balance=True)
+    assert ctx.status() == fb.OK
+    check_route(b, ref)
+    check_stats(b, ref)
+    first = (b.loss.clone(), b.prob.clone())
+    b.loss.fill_(-1)
+    b.count.fill_(-1)
+    b.prob.fill_(-1)
+    b.stats(ctx, b.expert)
+    assert ctx.status() == fb.OK
+    check_stats(b, ref)
+    b.route(ctx, balance=True)
+    assert ctx.status() == fb.OK and float(b.loss) == float(first[0]) and bool((b.prob == first[1]).all())
+
+
 @pytest.mark.parametrize("E", [512, 100])
 def test_many_rows(ctx, E):
     """More rows than the GPU's warps; statistics summed over all of them."""
