@@ -11,8 +11,8 @@
 //
 // A warp takes a row, 16 logits a lane; the logits' bytes bound it.  Measured
 // on one B200, graph replays, 512 experts fp32: statistics of 65,536 rows 27.0
-// us (5.0 TB/s), selection and statistics of 16,384 rows 17.5 us and of 65,536
-// rows 44.5 (440 instructions a row bound it), both gradients of 16,384 rows
+// us (5.0 TB/s), selection and statistics of 16,384 rows 17.2 us and of 65,536
+// rows 43.1 (430 instructions a row bound it), both gradients of 16,384 rows
 // 14.7 us (16.7 with rows that are not 16-byte aligned), one row's selection
 // 2.4 us.
 #pragma once
@@ -99,6 +99,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ float warp_max_nan(float v) {
   float d;
   asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
@@ -129,14 +134,11 @@ __device__ __forceinline__ float exp_below(float v, float m) {
 
 // The largest of a lane's slots (NaN when one is), as a tree.
 __device__ __forceinline__ float row_max(const float (&v)[kRouteSlots]) {
-  float m[kRouteSlots / 2];
+  static_assert(kRouteSlots == 16, "5 threes and one, then 2 threes");
+  float m[5];
 #pragma unroll
-  for (unsigned i = 0; i < kRouteSlots / 2; ++i) m[i] = max_nan(v[2 * i], v[2 * i + 1]);
-#pragma unroll
-  for (unsigned k = kRouteSlots / 4; k; k /= 2)
-#pragma unroll
-    for (unsigned i = 0; i < k; ++i) m[i] = max_nan(m[i], m[i + k]);
-  return m[0];
+  for (unsigned i = 0; i < 5; ++i) m[i] = max_nan(v[3 * i], v[3 * i + 1], v[3 * i + 2]);
+  return max_nan(max_nan(m[0], m[1], m[2]), max_nan(m[3], m[4], v[15]));
 }
 
 // Two fp32 operations an instruction: a row's arithmetic is 16 values a lane.
@@ -302,8 +304,17 @@ __device__ __forceinline__ void choose(const float (&v)[kRouteSlots], const L* r
   bool done = false;
   if (bound > -INFINITY) {
     unsigned mine = 0, total = 0;  // the lane's slots at or above the bound
+    // the signs of v - bound; 0 - bound is +0 for either zero, so that a zero less a zero is +0
+    const float less = 0.0f - bound;
+    const F2 below = pack2(less, less);
 #pragma unroll
-    for (unsigned i = 0; i < kRouteSlots; ++i) mine |= v[i] >= bound ? 1u << i : 0u;
+    for (unsigned i = kRouteSlots / 2; i-- > 0;) {
+      float x, y;
+      unpack2(add2(pack2(v[2 * i], v[2 * i + 1]), below), x, y);
+      mine = __funnelshift_l(__float_as_uint(y), mine, 1);
+      mine = __funnelshift_l(__float_as_uint(x), mine, 1);
+    }
+    mine ^= (1u << kRouteSlots) - 1u;
     done = !__any_sync(0xffffffffu, __popc(mine) > kLaneCand);
     if (done) {
       const unsigned before = (1u << lane) - 1u;
@@ -421,7 +432,8 @@ enum : int { kStatsNone = 0, kStatsParts = 1, kStatsCluster = 2 };
 // Warps of a CTA, and whether its rows come through shared memory: many
 // aligned rows, two buffers a warp.  Without the next row in registers there is
 // room for 32 warps, or 28 where experts are chosen and sums kept (65,536 rows
-// of 512, all of it: 44.7 us; with 24 warps 46.5, with 32, which spill, 45.7).
+// of 512, all of it, when this was chosen: 44.7 us; with 24 warps 46.5, with
+// 32, which spill, 45.7).
 template <unsigned V, bool SELECT, int STATS, bool MANY>
 struct RouteShape {
   static constexpr bool kStaged = MANY && V > 1;

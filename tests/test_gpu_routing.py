@@ -182,10 +182,15 @@ def logits_of(kind, T, E, rng):
         l = np.sort(l, 1) if rng.random() < 0.5 else -np.sort(-l, 1)
     elif kind == "large":
         l = l * 1e37
+    elif kind == "largest zeros":  # a dozen of +0 and -0 above the rest
+        l = -np.abs(l) - 0.1
+        for t in range(T):
+            l[t, rng.permutation(E)[:13]] = 0.0
+        l = np.where((l == 0) & (rng.random((T, E)) < 0.5), -0.0, l)
     return l
 
 
-KINDS = ["normal", "ties", "equal", "zeros", "masked", "few", "lowest", "wide", "sorted", "large"]
+KINDS = ["normal", "ties", "equal", "zeros", "masked", "few", "lowest", "wide", "sorted", "large", "largest zeros"]
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -288,7 +293,7 @@ def test_gradient_against_differences(ctx):
             assert abs((value(up) - value(down)) / (2 * h) - float(out[t, e])) < 1e-6 * (1 + abs(c[t]).max())
 
 
-@pytest.mark.parametrize("kind", ["normal", "ties", "zeros", "masked", "few", "lowest"])
+@pytest.mark.parametrize("kind", ["normal", "ties", "zeros", "masked", "few", "lowest", "largest zeros"])
 @pytest.mark.parametrize("T,E,dtype,pad", [(1301, 300, fb.F32, 0), (1400, 130, fb.F32, 2), (4999, 512, fb.F32, 4),
                                            (5000, 512, fb.BF16, 0), (1300, 261, fb.BF16, 3), (1299, 505, fb.BF16, 7)])
 def test_large_calls(ctx, kind, T, E, dtype, pad):
