@@ -584,3 +584,44 @@ def test_decode_step(gpu):
                 assert np.array_equal(y.cpu().numpy().view(np.uint32), host.view(np.uint32))
             del graph
             m.close()
+
+
+def gradient(ctx, b, d_gate, d_loss=None, expert=None):
+    """The gradient's columns [T][E (+ 1)] as float64, for d_gate [T][11] (numpy or None)."""
+    import torch
+    out = torch.full((b.T, b.cols), 5.0, dtype=b.logits.dtype, device="cuda")
+    dg = None if d_gate is None else torch.from_numpy(np.ascontiguousarray(d_gate, np.float32)).cuda()
+    dl = None if d_loss is None else torch.full((1,), d_loss, device="cuda")
+    b.backward(ctx, out, b.expert if expert is None else expert, dg, dl)
+    torch.cuda.synchronize()
+    return out.float().cpu().numpy().astype(np.float64)
+
+
+BOTH_TYPES_AND_LOSSES = pytest.mark.parametrize("dtype,d_loss", [(fb.F32, None), (fb.F32, -0.5), (fb.BF16, None), (fb.BF16, -0.5)])
+NOT_NUMBERS = [float("nan"), float("inf"), -float("inf")]
+
+
+@pytest.mark.parametrize("T,E", [(1, 10), (37, 512), (300, 97)])
+@BOTH_TYPES_AND_LOSSES
+def test_shared_gradient_stays_in_its_column(ctx, T, E, dtype, d_loss):
+    """What d_gate[t][10] holds reaches no expert's column: without the shared column it is not looked at, with it a
+    value that is not finite stays there."""
+    rng = np.random.default_rng(T + E)
+    dg = rng.standard_normal((T, 11))
+    for value in NOT_NUMBERS:
+        b = Buffers(rng.standard_normal((T, E)), dtype)
+        b.route(ctx, balance=True)
+        dg[:, 10] = 0
+        want = gradient(ctx, b, dg, d_loss)
+        dg[:, 10] = value
+        assert np.array_equal(gradient(ctx, b, dg, d_loss), want)
+        b = Buffers(rng.standard_normal((T, E)), dtype, shared=rng.standard_normal(T))
+        b.route(ctx, balance=True)
+        dg[:, 10] = rng.standard_normal(T)
+        want = gradient(ctx, b, dg, d_loss)
+        dg[T // 2, 10] = value
+        got = gradient(ctx, b, dg, d_loss)
+        assert np.array_equal(got[:, :E], want[:, :E])
+        assert np.array_equal(np.delete(got[:, E], T // 2), np.delete(want[:, E], T // 2))
+        assert not np.isfinite(got[T // 2, E])
+        assert ctx.status() == fb.OK
