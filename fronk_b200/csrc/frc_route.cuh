@@ -829,7 +829,7 @@ __global__ void __launch_bounds__(256, BALANCE ? 3 : 6) route_backward_kernel(co
     }
     if (a.shared && lane == kTopK) {
       const float sg = a.d_gate && valid ? sigmoid(val) : 0.0f;
-      store_grad(out + E, sg * (1.0f - sg) * cdg);
+      store_grad(out + E, valid ? sg * (1.0f - sg) * cdg : 0.0f);  // padding may hold any d_gate
     }
   }
 }

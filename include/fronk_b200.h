@@ -333,7 +333,8 @@ int frc_balance_device(frc_context *c, unsigned tokens, unsigned experts, const 
                        unsigned type, const uint8_t *valid, const uint16_t *expert, const frc_balance *balance,
                        void *stream);
 /* d_logits[t][experts (+ 1)] (`type`, d_stride) of both outputs; padding rows
- * get zeros, elements behind a row's columns are left alone.
+ * get zeros (their ids and d_gate are not looked at), elements behind a row's
+ * columns are left alone.
  *   gates (d_gate [tokens][11] not NULL; expert as chosen):
  *     g_i (d_i - sum_j g_j d_j) at the chosen, s (1 - s) d_10 at the shared column
  *     (without FRC_ROUTE_SHARED d_10 is not looked at)

@@ -625,3 +625,27 @@ def test_shared_gradient_stays_in_its_column(ctx, T, E, dtype, d_loss):
         assert np.array_equal(np.delete(got[:, E], T // 2), np.delete(want[:, E], T // 2))
         assert not np.isfinite(got[T // 2, E])
         assert ctx.status() == fb.OK
+
+
+@pytest.mark.parametrize("T,E", [(3, 10), (37, 512), (300, 97)])
+@BOTH_TYPES_AND_LOSSES
+def test_gradient_of_padding(ctx, T, E, dtype, d_loss):
+    """Padding rows get zeros in every column whatever their d_gate, ids and logits hold."""
+    import torch
+    rng = np.random.default_rng(T * 3 + E)
+    valid = rng.random(T) < 0.6
+    valid[1] = False
+    for value in NOT_NUMBERS:
+        l, sh = rng.standard_normal((T, E)), rng.standard_normal(T)
+        l[~valid], sh[~valid] = value, value
+        b = Buffers(l, dtype, valid=valid, shared=sh)
+        b.route(ctx, balance=True)
+        dg = rng.standard_normal((T, 11))
+        want = gradient(ctx, b, np.where(valid[:, None], dg, 0), d_loss)
+        dg[~valid] = value
+        ids = b.expert.clone()
+        ids[torch.from_numpy(~valid).cuda()] = -1
+        got = gradient(ctx, b, dg, d_loss, ids)
+        assert ctx.status() == fb.OK
+        assert not got[~valid].any()
+        assert np.array_equal(got, want) and np.isfinite(got).all()
