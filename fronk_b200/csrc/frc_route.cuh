@@ -828,8 +828,11 @@ __global__ void __launch_bounds__(256, BALANCE ? 3 : 6) route_backward_kernel(co
       if (valid && lane < kTopK && cid < E) store_grad(out + cid, term);
     }
     if (a.shared && lane == kTopK) {
-      const float sg = a.d_gate && valid ? sigmoid(val) : 0.0f;
-      store_grad(out + E, valid ? sg * (1.0f - sg) * cdg : 0.0f);  // padding may hold any d_gate
+      // an infinite logit's gate is constant, and a NaN one's, which is reported; padding may hold any d_gate
+      const bool moves = a.d_gate && valid && fabsf(val) < INFINITY;
+      if (a.d_gate && valid && val != val) atomicOr(a.status, kStNumeric);
+      const float sg = moves ? sigmoid(val) : 0.0f;
+      store_grad(out + E, moves ? sg * (1.0f - sg) * cdg : 0.0f);
     }
   }
 }

@@ -649,3 +649,33 @@ def test_gradient_of_padding(ctx, T, E, dtype, d_loss):
         assert ctx.status() == fb.OK
         assert not got[~valid].any()
         assert np.array_equal(got, want) and np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("T,E", [(3, 10), (37, 512), (300, 97)])
+@BOTH_TYPES_AND_LOSSES
+def test_gradient_of_a_shared_logit_that_is_nan(ctx, T, E, dtype, d_loss):
+    """A NaN shared logit is reported, as in the selection, and its gate is the constant 0; infinite ones are gates of
+    0 and 1; where no gate gradient is asked for, it is not looked at."""
+    rng = np.random.default_rng(T * 5 + E)
+    l, sh = rng.standard_normal((T, E)), rng.standard_normal(T)
+    dg = rng.standard_normal((T, 11))
+    clean = Buffers(l, dtype, shared=sh)
+    clean.route(ctx, balance=True)
+    want = gradient(ctx, clean, dg, d_loss)
+    assert ctx.status() == fb.OK
+    want[1, E] = 0
+    for value, status in [(float("nan"), fb.NUMERIC), (float("inf"), fb.OK), (-float("inf"), fb.OK)]:
+        sh[1] = value
+        b = Buffers(l, dtype, shared=sh)
+        b.route(ctx, balance=True)
+        assert ctx.status() == status
+        got = gradient(ctx, b, dg, d_loss)
+        assert ctx.status() == status
+        assert np.array_equal(got, want)
+        dg[1, 10] = float("nan")
+        got = gradient(ctx, b, dg, d_loss)
+        assert ctx.status() == status
+        assert np.array_equal(got, want)
+        dg[1, 10] = 1
+        gradient(ctx, b, None, 1.0)
+        assert ctx.status() == fb.OK
