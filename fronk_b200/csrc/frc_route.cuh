@@ -810,9 +810,11 @@ __global__ void __launch_bounds__(256, BALANCE ? 3 : 6) route_backward_kernel(co
       }
       const float chosen = lane < kTopK && valid ? val : -INFINITY, mk = warp_max(chosen);
       float g = mk > -INFINITY ? exp2f((chosen - mk) * 1.4426950408889634f) : 0.0f;  // subnormal gates count
-      // lane 10 holds the shared gate's gradient: its g is 0, but 0 times what is not finite is NaN
-      const float s = warp_sum(g), gd0 = warp_sum(lane < kTopK ? g * cdg : 0.0f), si = s > 0.0f ? rcp(s) : 0.0f;
-      const float own = g * si * (cdg - gd0 * si);
+      // gates that are 0 by a mask (or an id that is none) are constants: their gradient, which may be anything,
+      // does not count.  In lane 10 it is the shared gate's.
+      const float dgi = chosen > -INFINITY ? cdg : 0.0f;
+      const float s = warp_sum(g), gd0 = warp_sum(g * dgi), si = s > 0.0f ? rcp(s) : 0.0f;
+      const float own = g * si * (dgi - gd0 * si);
       float term = own;
       const unsigned same = __match_any_sync(0xffffffffu, cid) & 0x3ffu;
       const bool twice = lane < kTopK && same != 1u << lane;

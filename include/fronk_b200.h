@@ -337,8 +337,10 @@ int frc_balance_device(frc_context *c, unsigned tokens, unsigned experts, const 
  * columns are left alone.
  *   gates (d_gate [tokens][11] not NULL; expert as chosen):
  *     g_i (d_i - sum_j g_j d_j) at the chosen, s (1 - s) d_10 at the shared column
- *     (without FRC_ROUTE_SHARED d_10 is not looked at; a NaN shared logit sets
- *     FRC_NUMERIC, its gate and an infinite one's are constants)
+ *     (the gate of a masked expert, or of an id outside 0..experts-1, which
+ *     sets FRC_INVALID, is the constant 0 and its d_i is not looked at; nor is
+ *     d_10 without FRC_ROUTE_SHARED; a NaN shared logit sets FRC_NUMERIC, its
+ *     gate and an infinite one's are constants)
  *   loss (count as frc_balance wrote it and the scalar d_loss, not NULL):
  *     d_loss * experts / (10 N^2) * p_e (count_e - sum_j p_j count_j);
  *     the counts are constants, as usual

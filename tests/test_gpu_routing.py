@@ -679,3 +679,36 @@ def test_gradient_of_a_shared_logit_that_is_nan(ctx, T, E, dtype, d_loss):
         dg[1, 10] = 1
         gradient(ctx, b, None, 1.0)
         assert ctx.status() == fb.OK
+
+
+@pytest.mark.parametrize("T,E", [(9, 10), (40, 512), (300, 97)])
+@BOTH_TYPES_AND_LOSSES
+def test_gradient_of_masked_gates(ctx, T, E, dtype, d_loss):
+    """The gate of a masked expert (or of an id that is none) is the constant 0: its d_gate is not looked at."""
+    import torch
+    rng = np.random.default_rng(T * 7 + E)
+    for value in NOT_NUMBERS:
+        b = Buffers(logits_of("few", T, E, rng), dtype)
+        b.route(ctx, balance=True)
+        chosen = np.take_along_axis(b.seen()[0], b.expert.cpu().numpy().astype(np.int64), 1)
+        masked = np.isneginf(chosen)
+        assert masked.any(1).all()
+        dg = rng.standard_normal((T, 11))
+        dg[:, :10][masked] = 0
+        want = gradient(ctx, b, dg, d_loss)
+        dg[:, :10][masked] = value
+        got = gradient(ctx, b, dg, d_loss)
+        assert ctx.status() == fb.OK
+        assert np.array_equal(got, want) and np.isfinite(got).all()
+    b = Buffers(rng.standard_normal((T, E)), dtype)
+    b.route(ctx, balance=True)
+    dg = rng.standard_normal((T, 11))
+    ids = b.expert.clone()
+    ids[T // 2, 3] = E
+    dg[T // 2, 3] = 0
+    want = gradient(ctx, b, dg, d_loss, ids)
+    assert ctx.status() == fb.INVALID
+    dg[T // 2, 3] = float("nan")
+    got = gradient(ctx, b, dg, d_loss, ids)
+    assert ctx.status() == fb.INVALID
+    assert np.array_equal(got, want) and np.isfinite(got).all()
