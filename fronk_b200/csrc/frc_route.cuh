@@ -833,8 +833,9 @@ __global__ void __launch_bounds__(256, BALANCE ? 3 : 6) route_backward_kernel(co
       // an infinite logit's gate is constant, and a NaN one's, which is reported; padding may hold any d_gate
       const bool moves = a.d_gate && valid && fabsf(val) < INFINITY;
       if (a.d_gate && valid && val != val) atomicOr(a.status, kStNumeric);
-      const float sg = moves ? sigmoid(val) : 0.0f;
-      store_grad(out + E, moves ? sg * (1.0f - sg) * cdg : 0.0f);
+      // s (1 - s) as e / (1 + e)^2 with e = exp(-|val|): 1 - s would lose what s has rounded away, all of it from 17 on
+      const float e = expf(-fabsf(val)), r = 1.0f / (1.0f + e);
+      store_grad(out + E, moves ? e * r * r * cdg : 0.0f);
     }
   }
 }

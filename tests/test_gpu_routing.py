@@ -712,3 +712,22 @@ def test_gradient_of_masked_gates(ctx, T, E, dtype, d_loss):
     got = gradient(ctx, b, dg, d_loss, ids)
     assert ctx.status() == fb.INVALID
     assert np.array_equal(got, want) and np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("dtype", [fb.F32, fb.BF16])
+def test_gradient_of_saturated_shared_gates(ctx, dtype):
+    """s (1 - s) to a relative bound at every size of the shared logit l.  As e / (1 + e)^2, e = exp(-|l|): e is off by
+    2 steps (4 u), 1 + e by u and at most the 4 u of e, a reciprocal by 2 u, twice, and three products: at most
+    4 + 2 (1 + 4 + 2) + 3 = 21 u."""
+    sh = np.concatenate([np.linspace(-104, 104, 417), [-17.0, 17.0, 1e-3, -1e-3, 0.0, -3e38, 3e38]])
+    T, E = sh.size, 10
+    rng = np.random.default_rng(2)
+    b = Buffers(rng.standard_normal((T, E)), dtype, shared=sh)
+    b.route(ctx)
+    dg = rng.standard_normal((T, 11)).astype(np.float32).astype(np.float64)
+    got = gradient(ctx, b, dg)[:, E]
+    assert ctx.status() == fb.OK
+    e = np.exp(-np.abs(b.seen()[1]))
+    want = e / (1 + e) ** 2 * dg[:, 10]
+    tol = 21 * U * np.abs(want) + TINY * (1 + np.abs(dg[:, 10])) + (2.0 ** -8 * np.abs(want) if dtype == fb.BF16 else 0)
+    assert np.all(np.abs(got - want) <= tol), (np.abs(got - want) / tol).max()
