@@ -731,3 +731,71 @@ def test_gradient_of_saturated_shared_gates(ctx, dtype):
     want = e / (1 + e) ** 2 * dg[:, 10]
     tol = 21 * U * np.abs(want) + TINY * (1 + np.abs(dg[:, 10])) + (2.0 ** -8 * np.abs(want) if dtype == fb.BF16 else 0)
     assert np.all(np.abs(got - want) <= tol), (np.abs(got - want) / tol).max()
+
+
+# rows of each call, more of them than the gradient's launch has warps (3,552 with the balance term on 148 SMs, 7,104
+# without): some warps take one row more than others
+MANY = [(5000, 512, False, fb.F32, 0), (16391, 512, True, fb.F32, 0), (16391, 512, False, fb.BF16, 0),
+        (5003, 512, True, fb.BF16, 0), (9001, 511, True, fb.F32, 0), (5003, 300, False, fb.F32, 0),
+        (7200, 301, True, fb.BF16, 2), (15001, 37, False, fb.F32, 1), (11111, 64, True, fb.BF16, 0),
+        (6001, 264, False, fb.BF16, 0)]
+
+
+@pytest.mark.parametrize("T,E,shared,dtype,pad", MANY)
+def test_gradient_of_many_rows(ctx, T, E, shared, dtype, pad):
+    """Each gradient alone and both, with d_gate, ids, logits and validity of every row its own, out of place and in
+    place, rows 16-byte aligned and not."""
+    import torch
+    rng = np.random.default_rng(T + E)
+    valid = rng.random(T) < 0.8
+    l = logits_of("normal", T, E, rng)
+    l[rng.random((T, E)) < 0.05] = -np.inf
+    b = Buffers(l, dtype, pad=pad, valid=valid, shared=rng.standard_normal(T) * 3 if shared else None)
+    ref = Reference(b.seen()[0], valid, b.seen()[1])
+    b.route(ctx, balance=True)
+    dg = rng.standard_normal((T, 11)).astype(np.float32)
+    dg[~valid] = np.nan
+    d_gate, d_loss = torch.from_numpy(dg).cuda(), torch.full((1,), 0.5 * T, device="cuda")
+    dg[~valid] = 0
+    for use_gate, use_loss in [(True, True), (True, False), (False, True)]:
+        args = (b.expert if use_gate else None, d_gate if use_gate else None, d_loss if use_loss else None)
+        out = torch.full((T, b.stride), 5.0, dtype=b.logits.dtype, device="cuda")
+        b.backward(ctx, out, *args)
+        assert ctx.status() == fb.OK
+        d, tol = ref.backward(dg.astype(np.float64) if use_gate else None, 0.5 * T if use_loss else None, shared)
+        got = out.float().cpu().numpy().astype(np.float64)
+        tol = tol + (2.0 ** -8 * np.abs(d) + 2.0 ** -133 if dtype == fb.BF16 else 0)
+        assert np.all(np.abs(got[:, :b.cols] - d) <= tol), (np.abs(got[:, :b.cols] - d) / tol).max()
+        assert not got[~valid, :b.cols].any() and np.all(got[:, b.cols:] == 5)
+        keep = b.logits.clone()
+        b.backward(ctx, b.logits, *args)
+        assert ctx.status() == fb.OK
+        assert torch.equal(b.logits[:, :b.cols], out[:, :b.cols])
+        b.logits.copy_(keep)
+
+
+@pytest.mark.parametrize("kind", ["normal", "ties", "few"])
+@pytest.mark.parametrize("T,E,shared,dtype,pad", MANY)
+def test_selection_of_many_rows(ctx, kind, T, E, shared, dtype, pad):
+    """Selection and statistics where each warp takes several rows: rows with a shared column behind 512 experts
+    (their neighbours lie 513 elements apart) and other rows that are not 16-byte aligned, beside aligned ones."""
+    rng = np.random.default_rng(T * 3 + E)
+    valid = rng.random(T) < 0.8
+    b = Buffers(logits_of(kind, T, E, rng), dtype, pad=pad, valid=valid, shared=rng.standard_normal(T) * 3 if shared else None)
+    l, sh = b.seen()
+    ref = Reference(l, valid, sh)
+    b.route(ctx)
+    assert ctx.status() == fb.OK
+    check_route(b, ref)
+    ids = b.expert.clone()
+    b.expert.fill_(-1)
+    b.gate.fill_(float("nan"))
+    b.route(ctx, balance=True)
+    assert ctx.status() == fb.OK
+    check_route(b, ref)
+    check_stats(b, ref)
+    b.count.fill_(-1)
+    b.prob.fill_(-1)
+    b.stats(ctx, ids)
+    assert ctx.status() == fb.OK
+    check_stats(b, ref)
