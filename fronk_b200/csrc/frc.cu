@@ -1839,7 +1839,9 @@ int frc_matrix_open(frc_context* c, unsigned type, unsigned rows, unsigned n, co
   if (e != cudaSuccess || bad) {
     cudaGetLastError();  // reported here, not by a later call
     frc_matrix_close(m);
-    return bad ? fail(c, FRC_NUMERIC, "matrix: a scale is not finite") : fail(c, FRC_IO, "matrix: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) return fail(c, FRC_IO, "matrix: %s", cudaGetErrorString(e));
+    return bad & kMvNotFinite ? fail(c, FRC_NUMERIC, "matrix: a scale is not finite")
+                              : fail(c, FRC_UNSUPPORTED, "matrix: block scales of a row more than 2^%u apart", kMvField - 1);
   }
   *out = m;
   return FRC_OK;

@@ -17,7 +17,7 @@
 //     nibbles are made 1024 + q and one half2 operation takes the 1024 off
 //     (and multiplies by sc where that saves work on the results).
 //   MXFP4: in fp16, by the hardware's E2M1 conversion, and per 32 weights one
-//     fma with 2^(e - base), base the row's largest exponent.
+//     fma with the block's scale.
 //   In fp16 a bf16 x fits one value (P = 1); an fp32 x is the sum of two, hi
 //     and lo, a column each (P = 2): 22 of its 24 bits, or 2^-34 of the span's
 //     largest value where that is more.
@@ -52,12 +52,19 @@ constexpr unsigned kMvTile = 16;           // rows of one step
 // (Q4_K: 0..3 in the low nibbles of its bytes, 4..7 in the high ones).
 // The last span stops at the last piece that holds weights.
 //   Q4_K scales: the 16 header bytes of each row (d, dmin, packed 6 bits).
-//   MXFP4 scales: 8 exponents a row, relative to the row's largest (127 is
-//   that one, 0 stands for nothing); the largest are 16 bytes a tile at `base`.
+//   MXFP4 scales: 8 bytes a row, e + 1 - shift for a block of exponent e, so
+//   that each is the exponent field of an fp32 number (twice the scale; the
+//   spans' powers of two are halved), and 0 for a block whose weights are all
+//   zero.  The shift is 0 but in rows with scales over 2^102: it keeps the
+//   byte at or under kMvField, where a span's sum (at most 256 x 6 x 2^14
+//   times the scale) stays under 2^128.  127 + shift of the rows are 16 bytes
+//   a tile at `shift`.
 struct MvLayout {
   unsigned tiles, spans, pieces_last, span_bytes, scale_bytes;
-  size_t tile_bytes, base_at, total;
+  size_t tile_bytes, shift_at, total;
 };
+constexpr unsigned kMvField = 230;  // largest scale byte of MXFP4
+enum : unsigned { kMvNotFinite = 1, kMvTooFarApart = 2 };  // what matrix_layout_kernel finds
 inline MvLayout mv_layout(unsigned type, unsigned rows, unsigned n) {
   MvLayout l;
   l.tiles = (rows + kMvTile - 1) / kMvTile;
@@ -66,33 +73,48 @@ inline MvLayout mv_layout(unsigned type, unsigned rows, unsigned n) {
   l.scale_bytes = type == FRC_Q4_K ? 256 : 128;
   l.span_bytes = l.scale_bytes + 2048;
   l.tile_bytes = static_cast<size_t>(l.spans - 1) * l.span_bytes + l.scale_bytes + 512 * l.pieces_last;
-  l.base_at = l.tile_bytes * l.tiles;
-  l.total = l.base_at + static_cast<size_t>(l.tiles) * kMvTile;
+  l.shift_at = l.tile_bytes * l.tiles;
+  l.total = l.shift_at + static_cast<size_t>(l.tiles) * kMvTile;
   return l;
 }
 
-// Reference rows -> the layout above, one CTA a tile; scales that are not
-// finite (Q4_K super scales, MXFP4 exponent 255) raise the numeric bit.
+// Whether an MXFP4 block has a weight other than zero.
+__device__ __forceinline__ bool mv_block_counts(const uint8_t* b) {
+  unsigned any = 0;
+#pragma unroll
+  for (unsigned j = 1; j < 17; ++j) any |= b[j];
+  return any & 0x77u;
+}
+
+// Reference rows -> the layout above, one CTA a tile.  Flags scales that are
+// not finite (Q4_K super scales, MXFP4 exponent 255) and MXFP4 rows whose
+// smallest scale would not fit the byte.
 template <unsigned TYPE>
 __global__ void __launch_bounds__(256) matrix_layout_kernel(const uint8_t* __restrict__ src, uint8_t* dst, MvLayout l,
                                                             unsigned rows, unsigned n, unsigned row_bytes,
                                                             unsigned* flag) {
-  __shared__ unsigned s_base[kMvTile];
+  __shared__ unsigned s_high[kMvTile];  // a row's largest exponent, then its shift
   const unsigned tile = blockIdx.x, tid = threadIdx.x;
   const uint8_t* in = src + static_cast<size_t>(tile) * kMvTile * row_bytes;
   uint8_t* out = dst + tile * l.tile_bytes;
   const unsigned left = rows - tile * kMvTile < kMvTile ? rows - tile * kMvTile : kMvTile;
-  bool bad = false;
+  bool bad = false, apart = false;
   if (TYPE == kMXFP4) {
-    if (tid < kMvTile) s_base[tid] = 0;
+    if (tid < kMvTile) s_high[tid] = 0;
     __syncthreads();
     for (unsigned i = tid; i < left * (n / 32); i += 256) {
-      const unsigned r = i / (n / 32), b = i % (n / 32), e = in[static_cast<size_t>(r) * row_bytes + 17 * b];
-      bad |= e == 255;
-      atomicMax(&s_base[r], e);
+      const unsigned r = i / (n / 32), b = i % (n / 32);
+      const uint8_t* block = in + static_cast<size_t>(r) * row_bytes + 17 * b;
+      bad |= block[0] == 255;
+      if (mv_block_counts(block)) atomicMax(&s_high[r], static_cast<unsigned>(block[0]));
     }
     __syncthreads();
-    if (tid < kMvTile) dst[l.base_at + static_cast<size_t>(tile) * kMvTile + tid] = static_cast<uint8_t>(s_base[tid]);
+    if (tid < kMvTile) {
+      const unsigned shift = s_high[tid] < kMvField ? 0 : s_high[tid] + 1 - kMvField;
+      s_high[tid] = shift;
+      dst[l.shift_at + static_cast<size_t>(tile) * kMvTile + tid] = static_cast<uint8_t>(127 + shift);
+    }
+    __syncthreads();
   }
   for (unsigned s = 0; s < l.spans; ++s) {
     uint8_t* o = out + static_cast<size_t>(s) * l.span_bytes;
@@ -108,8 +130,11 @@ __global__ void __launch_bounds__(256) matrix_layout_kernel(const uint8_t* __res
       const unsigned r = tid / 8, b = 8 * s + tid % 8;
       unsigned e = 0;
       if (r < left && b < n / 32) {
-        const unsigned v = in[static_cast<size_t>(r) * row_bytes + 17 * b], base = s_base[r];
-        e = base - v < 127u ? v + 127u - base : 0u;
+        const uint8_t* block = in + static_cast<size_t>(r) * row_bytes + 17 * b;
+        if (mv_block_counts(block)) {
+          apart |= block[0] < s_high[r];
+          e = block[0] + 1 - s_high[r];
+        }
       }
       o[tid] = static_cast<uint8_t>(e);
     }
@@ -133,7 +158,8 @@ __global__ void __launch_bounds__(256) matrix_layout_kernel(const uint8_t* __res
       reinterpret_cast<unsigned*>(o + l.scale_bytes)[i] = v;
     }
   }
-  if (bad) atomicOr(flag, kStNumeric);
+  if (bad) atomicOr(flag, kMvNotFinite);
+  if (apart) atomicOr(flag, kMvTooFarApart);
 }
 
 struct MatvecParams {
@@ -141,7 +167,7 @@ struct MatvecParams {
   const void* x;
   void* y;
   size_t x_stride, y_stride;  // elements between tokens
-  size_t tile_bytes, base_at;
+  size_t tile_bytes, shift_at;
   unsigned rows, n, tokens, tiles, spans, pieces_last;
   unsigned slice;             // spans of K a CTA works on (all, or a share where a cluster splits K)
   unsigned chunk;             // spans of x in shared memory at a time, at most the slice
@@ -317,10 +343,10 @@ __device__ __forceinline__ void mv_prepare(const MatvecParams& a, const MvShared
       for (unsigned j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
       top = __reduce_max_sync(0xffffffffu, top);
       // x = v 2^ex, the largest |v| in [2^13, 2^14), or [2^29, 2^30) as digits; a span that is not finite has the
-      // scale NaN and so its results
-      constexpr int TOP = P == 4 ? 29 : 13;
+      // scale NaN and so its results.  The scales of MXFP4's blocks are doubled, so the span's is halved.
+      constexpr int TOP = P == 4 ? 29 : 13, HALVED = TYPE == kMXFP4 ? 1 : 0;
       int ex = static_cast<int>(top >> 23) - 127 - TOP;
-      if (ex < -126) ex = -126;
+      if (ex < HALVED - 126) ex = HALVED - 126;
       const bool finite = top < 0x7f800000u;
       const float inv = finite ? __uint_as_float(static_cast<uint32_t>(127 - ex) << 23) : 0.0f;
 #pragma unroll
@@ -358,7 +384,7 @@ __device__ __forceinline__ void mv_prepare(const MatvecParams& a, const MvShared
         *reinterpret_cast<uint4*>(c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         if (P == 2) *reinterpret_cast<uint4*>(c + 64) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
-      if (lane == 0) sh.scale[t * a.chunk + s] = finite ? __uint_as_float(static_cast<uint32_t>(127 + ex) << 23) : NAN;
+      if (lane == 0) sh.scale[t * a.chunk + s] = finite ? __uint_as_float(static_cast<uint32_t>(127 - HALVED + ex) << 23) : NAN;
       if (TYPE == kQ4K) {
         float sum = sum8;
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
@@ -422,8 +448,8 @@ __device__ __forceinline__ void mv_weights(uint32_t w, uint32_t (&av)[4]) {
     e2m1_f16(w, av);
   }
 }
-// Byte `at` of the eight in {lo, hi} as a float: a 6-bit scale, or 2^(e - 127)
-// (e at most 127).
+// Byte `at` of the eight in {lo, hi} as a float: a 6-bit scale, or the number
+// of that exponent field (0 for 0).
 template <unsigned TYPE>
 __device__ __forceinline__ float mv_scale(uint32_t lo, uint32_t hi, unsigned at) {
   const uint32_t v = prmt(lo, hi, at);
@@ -617,11 +643,7 @@ __device__ __forceinline__ bool mv_store(const MatvecParams& a, const MvLane<P, 
   for (unsigned h = 0; h < 2; ++h) {
     const unsigned row = tile * kMvTile + g + 8 * h;
     if (row >= a.rows) continue;
-    float f = 1.0f;
-    if (TYPE == kMXFP4) {
-      const unsigned e = a.w[a.base_at + row];
-      f = __uint_as_float(e ? e << 23 : 0x00400000u);
-    }
+    const float f = TYPE == kMXFP4 ? __uint_as_float(static_cast<unsigned>(a.w[a.shift_at + row]) << 23) : 1.0f;
 #pragma unroll
     for (unsigned i = 0; i < V / 2; ++i) {
       const unsigned t = i / A, k = i % A, tok = ln.token(t, k, q);
@@ -939,7 +961,7 @@ template <unsigned TYPE>
 inline cudaError_t launch_matvec(MatvecParams& a, const MvLayout& l, const MvPlan& p, unsigned x_type, int device,
                                  cudaStream_t s) {
   const unsigned P = mv_parts(TYPE, a.tokens, x_type), cols = a.tokens * P, nt = mv_groups(cols);
-  a.tile_bytes = l.tile_bytes; a.base_at = l.base_at; a.tiles = l.tiles; a.spans = l.spans; a.pieces_last = l.pieces_last;
+  a.tile_bytes = l.tile_bytes; a.shift_at = l.shift_at; a.tiles = l.tiles; a.spans = l.spans; a.pieces_last = l.pieces_last;
   a.slice = p.slice; a.chunk = p.chunk; a.cluster = p.cluster;
   if constexpr (TYPE == kQ4K) {
     if (P == 4) return nt == 1 ? mv_launch_w<TYPE, 4, 1, 8>(a, p, device, s) : mv_launch_w<TYPE, 4, 2, 8>(a, p, device, s);

@@ -265,7 +265,9 @@ int frc_matrix_check(unsigned type, unsigned rows, unsigned n);
 /* Copies rows x frc_row_bytes(type, n) bytes (the reference's row layout, row
  * after row; host or device memory, ready when the call is made) into HBM and
  * checks every scale: FRC_NUMERIC when one is not finite (MXFP4 exponent 255
- * too).  Synchronous.  The matrix belongs to the context's device, works with
+ * too), FRC_UNSUPPORTED when scales of one MXFP4 row lie more than 2^229 apart
+ * (those of blocks without a weight other than zero do not count).
+ * Synchronous.  The matrix belongs to the context's device, works with
  * any context of that device and may outlive the one that opened it. */
 int frc_matrix_open(frc_context *c, unsigned type, unsigned rows, unsigned n, const void *bytes, size_t len,
                     frc_matrix **out);

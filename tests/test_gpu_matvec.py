@@ -349,3 +349,93 @@ def test_device_rows_graph_and_streams(ctx):
     assert all(torch.equal(v, y) for v in ys)
     assert ctx.status() == fb.OK
     m.close()
+
+
+def far_apart(n, rng, pairs):
+    """Eight MXFP4 rows for each pair (small, large) of exponents: blocks of either kind mixed, and the columns of the
+    small ones."""
+    small = rng.random(n // 32) < 0.6
+    small[0] = True
+    raw = np.concatenate([quant.random_rows(fb.MXFP4, 8, n, rng, (lo, lo + 1)) for lo, _ in pairs])
+    b = raw.reshape(len(pairs), 8, n // 32, 17)
+    for k, (_, hi) in enumerate(pairs):
+        b[k, :, ~small, 0] = hi
+    return raw, np.repeat(small, 32)
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 3, 5, 16])
+@pytest.mark.parametrize("x_type", [fb.F32, fb.BF16])
+def test_block_scales_far_apart(ctx, tokens, x_type):
+    """MXFP4 rows whose block scales lie 100 to 229 binades apart, x zero where they are large: what the small ones
+    give counts in full.  A zero of x adds nothing and is exact, so the bound's terms are those of the small blocks."""
+    rng = np.random.default_rng(31)
+    for n in (544, 2560):
+        for pairs in ([(20, 120), (20, 146), (20, 147), (20, 148), (20, 220), (20, 229), (21, 248), (25, 254)],
+                      [(0, 229), (0, 127), (0, 128), (1, 230), (1, 128), (2, 200)]):
+            raw, small = far_apart(n, rng, pairs)
+            w, a = quant.weights(fb.MXFP4, raw, n)
+            x = np.where(small, rng.standard_normal((tokens, n)), 0) * 2.0 ** 105
+            xd = to_device(x, x_type)
+            y = host(run(ctx, fb.MXFP4, raw, n, xd, x_type, fb.F32))
+            xr = host(xd)
+            ref = xr @ w.T
+            tol = bound(a * small, xr, n) + 2.0 ** -126
+            assert np.all(np.abs(y - ref) <= tol), (np.abs(y - ref) / tol).max()
+            assert np.abs(ref).min() > 2.0 ** -60
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 3, 5, 16])
+def test_blocks_without_weights(ctx, tokens):
+    """The exponent of a block whose weights are all +-0 means nothing, to 254."""
+    rng = np.random.default_rng(32)
+    n = 1056
+    raw = quant.random_rows(fb.MXFP4, 40, n, rng)
+    b = raw.reshape(40, n // 32, 17)
+    zero = rng.random((40, n // 32)) < 0.3
+    b[zero, 1:] = rng.choice(np.array([0, 0x80, 0x08, 0x88], np.uint8), (int(zero.sum()), 16))
+    b[zero, 0] = rng.choice(np.array([0, 1, 200, 254], np.uint8), int(zero.sum()))
+    b[5, :, 1:] = 0
+    b[5, :, 0] = 254
+    w, a = quant.weights(fb.MXFP4, raw, n)
+    assert not w.reshape(40, -1, 32)[zero].any()
+    xd = to_device(rng.standard_normal((tokens, n)), fb.F32)
+    y = host(run(ctx, fb.MXFP4, raw, n, xd, fb.F32, fb.F32))
+    check(y, host(xd), w, a, n, fb.F32)
+    assert not y[:, 5].any()
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 3, 5, 16])
+@pytest.mark.parametrize("exponents,size", [((60, 90), 2.0 ** 125), ((0, 1), 2.0 ** 125), ((0, 40), 2.0 ** 110), ((224, 255), 2.0 ** -120),
+                                            ((254, 255), 2.0 ** -122), ((100, 130), 2.0 ** 100)])
+def test_products_of_extremes(ctx, exponents, size, tokens):
+    """MXFP4 scales and vectors at opposite ends of their ranges: results that are finite come out finite and right."""
+    rng = np.random.default_rng(33)
+    for n in (288, 4096):
+        raw = quant.random_rows(fb.MXFP4, 33, n, rng, exponents)
+        w, a = quant.weights(fb.MXFP4, raw, n)
+        x = rng.uniform(0.5, 1.0, (tokens, n)) * rng.choice((-1, 1), (tokens, n)) * size
+        xd = to_device(x, fb.F32)
+        xr = host(xd)
+        assert np.all(np.abs(xr) @ a.T < 2.0 ** 126)
+        y = host(run(ctx, fb.MXFP4, raw, n, xd, fb.F32, fb.F32))
+        tol = bound(a, xr, n) + 2.0 ** -126
+        assert np.all(np.abs(y - xr @ w.T) <= tol)
+
+
+def test_block_scales_too_far_apart(ctx):
+    """Scales of one row more than 229 binades apart are refused, at any place of the matrix; zero weights do not count."""
+    rng = np.random.default_rng(34)
+    n, rows = 320, 50
+    for row, refused, taken in [(0, (0, 230), (1, 230)), (17, (24, 254), (25, 254)), (49, (0, 254), (0, 229))]:
+        raw = quant.random_rows(fb.MXFP4, rows, n, rng)
+        b = raw.reshape(rows, n // 32, 17)
+        b[row, 0, 1] = b[row, 9, 16] = 0x10  # one weight of 0.5
+        b[row, 0, 0], b[row, 9, 0] = refused
+        with pytest.raises(fb.FrcError) as e:
+            ctx.matrix(fb.MXFP4, rows, n, raw)
+        assert e.value.code == fb.UNSUPPORTED
+        b[row, 0, 0], b[row, 9, 0] = taken
+        ctx.matrix(fb.MXFP4, rows, n, raw).close()
+        b[row, 0, 0], b[row, 9, 0] = refused
+        b[row, 0, 1:] = 0x80
+        ctx.matrix(fb.MXFP4, rows, n, raw).close()
