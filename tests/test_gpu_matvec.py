@@ -439,3 +439,23 @@ def test_block_scales_too_far_apart(ctx):
         b[row, 0, 0], b[row, 9, 0] = refused
         b[row, 0, 1:] = 0x80
         ctx.matrix(fb.MXFP4, rows, n, raw).close()
+
+
+@pytest.mark.parametrize("type_", [fb.Q4_K, fb.MXFP4])
+@pytest.mark.parametrize("tokens", [1, 3, 4, 5, 16])
+@pytest.mark.parametrize("exponent", [-97, -104, -112, -122, -130, -147])
+def test_tiny_vectors(ctx, type_, tokens, exponent):
+    """Vectors near the bottom of fp32's range, subnormal ones too, times large weights: they are carried as exactly
+    as others."""
+    rng = np.random.default_rng(35)
+    n = 256
+    raw = quant.random_rows(type_, 40, n, rng, exponents=(180, 190))
+    if type_ == fb.Q4_K:
+        raw.reshape(40, 1, 144)[..., :4] = (rng.choice((-1, 1), (40, 1, 2)) * rng.uniform(20000, 60000, (40, 1, 2))).astype(np.float16).view(np.uint8)
+    w, a = quant.weights(type_, raw, n)
+    xd = to_device(rng.standard_normal((tokens, n)) * 2.0 ** exponent, fb.F32)
+    x = host(xd)
+    assert x.any(1).all()
+    y = host(run(ctx, type_, raw, n, xd, fb.F32, fb.F32))
+    tol = bound(a, x, n) + 2.0 ** -126
+    assert np.all(np.abs(y - x @ w.T) <= tol), (np.abs(y - x @ w.T) / tol).max()
