@@ -459,3 +459,55 @@ def test_tiny_vectors(ctx, type_, tokens, exponent):
     y = host(run(ctx, type_, raw, n, xd, fb.F32, fb.F32))
     tol = bound(a, x, n) + 2.0 ** -126
     assert np.all(np.abs(y - x @ w.T) <= tol), (np.abs(y - x @ w.T) / tol).max()
+
+
+@pytest.mark.parametrize("type_,rows,n", [(fb.Q4_K, 513, 2048), (fb.Q4_K, 300, 8192), (fb.Q4_K, 200, 65536),
+                                          (fb.MXFP4, 513, 2048), (fb.MXFP4, 300, 16384), (fb.MXFP4, 200, 65440)])
+def test_size_of_the_error(ctx, type_, rows, n):
+    """The error's L2 norm over the rows, which a worst-case bound leaves room for a hundred times over.  With S = the
+    root of the sum of (a_j x_j)^2, the size of a sum of n terms of either sign, and roundings that are independent of
+    one another: 26 in a span of 256 (8 groups of 2 steps and a scale, 2 for the span's own), each up to 2^-23 of the
+    span's S, make sqrt(26) = 5.1; one an added span, up to 2^-24 of all of S, sqrt(spans) / 2; truncation moves a
+    group's sum by up to 2 steps the same way, 2; the vector's 22 bits 1; joining 16 parts 4.  Together
+    (sqrt(spans) / 2 + 13) 2^-23 S."""
+    rng = np.random.default_rng(rows + n)
+    raw = quant.random_rows(type_, rows, n, rng)
+    w, a = quant.weights(type_, raw, n)
+    for tokens in (1, 2, 4, 5, 9, 16):
+        for x_type in (fb.F32, fb.BF16):
+            xd = to_device(rng.standard_normal((tokens, n)), x_type)
+            x = host(xd)
+            y = host(run(ctx, type_, raw, n, xd, x_type, fb.F32))
+            size = np.sqrt((x ** 2 @ (a ** 2).T).sum(1))
+            err = np.sqrt(((y - x @ w.T) ** 2).sum(1))
+            limit = (np.sqrt(n / 256) / 2 + 13) * 2.0 ** -23
+            assert np.all(err <= limit * size), (tokens, x_type, (err / size).max() / limit)
+
+
+@pytest.mark.parametrize("type_", [fb.Q4_K, fb.MXFP4])
+@pytest.mark.parametrize("n,tokens,x_type", [(65536, 16, fb.F32), (65536, 16, fb.BF16), (65536, 3, fb.F32), (8192, 1, fb.F32),
+                                             (8192, 8, fb.BF16)])
+def test_one_span_at_a_time(ctx, type_, n, tokens, x_type):
+    """Vectors that are zero but for one span of 256 columns, each span in turn: a span that is lost, taken twice or
+    taken from another place shows.  The zeros are exact, so the bound is that of a single span."""
+    rng = np.random.default_rng(n + tokens)
+    n -= 0 if type_ == fb.Q4_K else 96
+    spans, rows = -(-n // 256), 70
+    raw = quant.random_rows(type_, rows, n, rng)
+    w, a = quant.weights(type_, raw, n)
+    with ctx.matrix(type_, rows, n, raw) as m:
+        for first in range(0, spans, tokens):
+            x = np.zeros((tokens, n))
+            for t in range(tokens):
+                s = (first + t) % spans
+                x[t, 256 * s:256 * s + 256] = rng.standard_normal(min(256, n - 256 * s))
+            xd = to_device(x, x_type)
+            yd = to_device(np.full((tokens, rows), np.nan), fb.F32)
+            m.matvec_device(tokens, xd.data_ptr(), yd.data_ptr(), x_type)
+            assert ctx.status() == fb.OK
+            for t in range(tokens):
+                s = (first + t) % spans
+                cols = slice(256 * s, 256 * s + 256)
+                xs, ys = host(xd[t:t + 1, cols]), host(yd[t:t + 1])
+                ref, tol = xs @ w[:, cols].T, bound(a[:, cols], xs, xs.shape[1])
+                assert np.all(np.abs(ys - ref) <= tol), (s, (np.abs(ys - ref) / tol).max())
