@@ -812,9 +812,10 @@ __global__ void __launch_bounds__(256, BALANCE ? 3 : 6) route_backward_kernel(co
       float g = mk > -INFINITY ? exp2f((chosen - mk) * 1.4426950408889634f) : 0.0f;  // subnormal gates count
       // gates that are 0 by a mask (or an id that is none) are constants: their gradient, which may be anything,
       // does not count.  In lane 10 it is the shared gate's.
-      const float dgi = chosen > -INFINITY ? cdg : 0.0f;
-      const float s = warp_sum(g), gd0 = warp_sum(g * dgi), si = s > 0.0f ? rcp(s) : 0.0f;
-      const float own = g * si * (dgi - gd0 * si);
+      // Taken as sixteenths: the ten products with gates that are not divided by their sum yet stay in range.
+      const float d16 = chosen > -INFINITY ? cdg * 0.0625f : 0.0f;
+      const float s = warp_sum(g), gd16 = warp_sum(g * d16), si = s > 0.0f ? rcp(s) : 0.0f;
+      const float own = g * si * (d16 - gd16 * si) * 16.0f;
       float term = own;
       const unsigned same = __match_any_sync(0xffffffffu, cid) & 0x3ffu;
       const bool twice = lane < kTopK && same != 1u << lane;

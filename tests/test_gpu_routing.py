@@ -799,3 +799,19 @@ def test_selection_of_many_rows(ctx, kind, T, E, shared, dtype, pad):
     b.stats(ctx, ids)
     assert ctx.status() == fb.OK
     check_stats(b, ref)
+
+
+@pytest.mark.parametrize("T,E", [(9, 10), (40, 512)])
+def test_gradient_of_large_gate_gradients(ctx, T, E):
+    """d_gate near the largest fp32 number: g (d - sum g d) is below twice a half of it, and comes out finite."""
+    rng = np.random.default_rng(T + E)
+    b = Buffers(rng.standard_normal((T, E)) * 0.1)
+    ref = Reference(b.seen()[0])
+    b.route(ctx)
+    dg = (rng.choice((-1, 1), (T, 11)) * rng.uniform(2e38, 3.4e38, (T, 11))).astype(np.float32)
+    dg[0] = 3.4e38
+    dg[1] = -3.4e38
+    got = gradient(ctx, b, dg)
+    assert ctx.status() == fb.OK
+    want, tol = ref.backward(dg.astype(np.float64))
+    assert np.all(np.abs(got - want) <= tol), (np.abs(got - want) / tol).max()
