@@ -10,9 +10,12 @@
 // columns ("a span of a tile") on the tensor cores by mma.sync, with the
 // vectors as the eight columns.  x is scaled by a power of two per span.
 //   Q4_K, up to four tokens: in integers.  The nibbles are the bytes of a u8
-//     operand after one mask each; x is held as four signed base-256 digits
-//     (32 bits under the span's largest value), a column each; the 6-bit
-//     scales multiply the int32 sums of each 32, so a span is exact.
+//     operand after one mask each; x is held as four signed base-256 digits,
+//     a column each: rounded to 2^-30 of the span's largest value, so that the
+//     parts of a span's sum that come from digits stay whole numbers (a value
+//     2^-7 of the largest loses its last bits, 2^-30 of the sum's size at
+//     most, where fp32 sums round 2^-24 at every step); the 6-bit scales
+//     multiply the int32 sums of each 32, so a span is exact.
 //   Q4_K, more tokens: in fp16, which holds q sc exactly (10 bits): masked
 //     nibbles are made 1024 + q and one half2 operation takes the 1024 off
 //     (and multiplies by sc where that saves work on the results).
@@ -20,18 +23,19 @@
 //     fma with the block's scale.
 //   In fp16 a bf16 x fits one value (P = 1); an fp32 x is the sum of two, hi
 //     and lo, a column each (P = 2): 22 of its 24 bits, or 2^-34 of the span's
-//     largest value where that is more.
+//     largest value where that is more.  A third part would cost half as many
+//     products again for 2^-23 of each x, which the sums' rounding hides.
 //   The minima of Q4_K are one more fp16 product, of mi with the sums of x
-//     over each 32 (hi and lo parts along K).
+//     over each 32 (hi and lo parts along K, 22 bits like x itself).
 // (fp16 subnormals as operands would save the half2 operations, but mma.sync
 // aligns its sums by the operands' exponents: measured, q 2^-24 costs 20 times
 // the rounding error.)
 //
-// Measured on one B200, graph replays: 131072 x 2048, one token: Q4_K 27.9 us
+// Measured on one B200, graph replays: 131072 x 2048, one token: Q4_K 27.8 us
 // (5.4 TB/s, 84 % of the copy rate), MXFP4 26.7 us; 65536 x 2048, Q4_K, 4, 8
-// and 16 fp32 tokens 19.6, 27.7 and 38.3 us (with more columns the products
+// and 16 fp32 tokens 20.6, 28.2 and 39.2 us (with more columns the products
 // and their operands' reads bound it, not the weights); 50021 x 2560, MXFP4,
-// 16 bf16 tokens 24.7 us.
+// 16 tokens: bf16 25.1 us, fp32 39.1 us (its 32 columns spill registers).
 #pragma once
 #include <atomic>
 #include <cuda_bf16.h>
@@ -282,8 +286,8 @@ struct MvFrag {
 // one accumulator keeps the groups' sums apart, each lane has the sums of its
 // own group, and a lane applies one scale where it would apply 8 / COLS.  The
 // zeros have to be written first: it pays from six spans a warp on (MXFP4,
-// bf16 x, one token: 131072 x 2048 29.5 against 32.2 us; 513 x 2048, one span
-// a warp, 3.7 against 3.4).
+// bf16 x, one token: 131072 x 2048 26.7 against 27.4 us; 513 x 2048, one span
+// a warp, 4.1 against 4.0).
 struct MvShared {
   uint8_t* col;     // [chunk][8 groups][NT][8 columns][64 or 32]
   uint8_t* sums;    // Q4_K: [chunk][NT][8 columns][32]: sums over each 32 (x 2^-5, so they fit fp16), eight hi, eight
@@ -347,8 +351,7 @@ __device__ __forceinline__ void mv_prepare(const MatvecParams& a, const MvShared
       constexpr int TOP = P == 4 ? 29 : 13, HALVED = TYPE == kMXFP4 ? 1 : 0;
       int ex = static_cast<int>(top >> 23) - 127 - TOP;
       // Near the smallest numbers, where 2^-ex is too large for fp32, v is made in two steps and the span's scale is
-      // subnormal (131072 x 2048, one token: the same time; 65536 x 2048, four tokens 20.8 us, 20.6 without; 50021 x
-      // 2560, 16 tokens 25.1 and 24.8).  At 2^-149, the last bit of any x, v is a whole number.
+      // subnormal (131072 x 2048, one token: the same time with and without; 50021 x 2560, 16 tokens 25.1 and 24.8 us).  At 2^-149, the last bit of any x, v is a whole number.
       constexpr int LOW = HALVED - 126;
       const int less = min(max(LOW - ex, 0), 23);
       ex = max(ex, LOW);
@@ -869,7 +872,7 @@ struct MvPlan {
   unsigned warps, slice, chunk, cluster, grid, smem, share;
 };
 
-// Spans a warp has on their way (131072 x 2048, one token: four are no faster, 32.0 against 31.1 us).
+// Spans a warp has on their way (131072 x 2048, one token: four are no faster, 28.0 against 27.8 us).
 constexpr unsigned kMvDepth = 2;
 constexpr unsigned kMvSmemSm = 228 * 1024, kMvSmemCta = 227 * 1024;
 
@@ -887,9 +890,10 @@ inline unsigned mv_ceil(unsigned a, unsigned b) { return (a + b - 1) / b; }
 // time in us, fitted to sweeps over both: a span takes a warp 0.06 us (times
 // `heavy`, for the columns) for each warp of its SM, at least 0.4; preparing
 // x 0.35 a span and warp, a cluster's exchange 0.1 a CTA and 0.02 a tile.
-// Measured both ways: 5120 x 2560 and 8 tokens 9.0 us with clusters of 4, 10.1
-// without; 4096 x 8192 and one token 8.6 and 9.0; 513 x 2048 and one token 3.8
-// and 3.4; 50021 x 2560 and 16 tokens 26.2 with clusters of 2, 24.9 without.
+// Measured both ways: 5120 x 2560 and 8 tokens 9.8 us with clusters of 4, 10.4
+// without; 513 x 2048 and one token 3.9 and 3.5; 50021 x 2560 and 16 tokens
+// 25.8 with clusters of 2, 25.1 without; 4096 x 8192 and one token 8.9 either
+// way.
 inline MvPlan mv_plan(unsigned type, unsigned P, unsigned nt, unsigned tokens, const MvLayout& l, unsigned sms) {
   const unsigned values = nt * (P >= 2 ? 2 : 4);
   const double heavy = nt == 1 ? 1.0 : nt == 2 ? 1.5 : 2.3;
@@ -957,8 +961,8 @@ inline cudaError_t mv_launch_w(const MatvecParams& a, const MvPlan& p, int devic
 }
 
 // Parts of x and groups of eight columns of a call.  The digits' four columns
-// a token pay up to four tokens (65536 x 2048, Q4_K: 4 tokens 19.6 us against
-// 23.3 in fp16, 8 tokens 28.7 against 27.7).
+// a token pay up to four tokens (65536 x 2048, Q4_K: 4 tokens 20.6 us against
+// 23.1 in fp16, 8 tokens 28.8 against 28.2).
 inline unsigned mv_parts(unsigned type, unsigned tokens, unsigned x_type) {
   return type == FRC_Q4_K && tokens <= 4 ? 4 : x_type == FRC_F32 ? 2 : 1;
 }

@@ -12,9 +12,10 @@
 // A warp takes a row, 16 logits a lane; the logits' bytes bound it.  Measured
 // on one B200, graph replays, 512 experts fp32: statistics of 65,536 rows 27.0
 // us (5.0 TB/s), selection and statistics of 16,384 rows 17.2 us and of 65,536
-// rows 43.1 (430 instructions a row bound it), both gradients of 16,384 rows
-// 14.7 us (16.7 with rows that are not 16-byte aligned), one row's selection
-// 2.4 us.
+// rows 43.5 (430 instructions a row bound it), both gradients of 16,384 rows
+// 14.9 us, one row's selection 2.4 us.  Rows that a shared column puts 513
+// elements apart are not 16-byte aligned: selection and statistics of 16,384
+// rows 20.8 us, both gradients 16.9.
 #pragma once
 #include <cuda_bf16.h>
 
@@ -25,7 +26,7 @@ namespace frc {
 
 constexpr unsigned kTopK = 10, kGates = 11, kMaxExperts = 512;
 constexpr unsigned kRouteSlots = kMaxExperts / 32;  // logits a lane holds
-constexpr unsigned kRouteWarps = 24;                // warps a CTA, at most
+constexpr unsigned kRouteWarps = 24;                // warps a CTA whose rows pass through registers alone, at most
 constexpr unsigned kRouteSums = 16;                 // arrays of sums a CTA folds its warps into; warps of a cluster's CTA
 constexpr unsigned kRouteRows = 8;                  // rows a CTA that makes statistics, at least, while SMs are free
 constexpr unsigned kRouteCtas = 160;                // CTAs that make statistics (one an SM), at most
@@ -444,7 +445,7 @@ struct RouteShape {
 // counts of the chosen (or given) experts over the CTA's rows.  The next
 // row's logits are on their way while one is worked on.  Neighbouring rows go
 // to different CTAs: runs of padding rows leave none idle (a ragged batch of
-// 16,384 rows 19.0 us, with 24 neighbours a CTA 19.9).
+// 16,384 rows 17.1 us, with neighbours in one CTA 18.1).
 template <typename L, unsigned V, bool FULL, bool SELECT, int STATS, bool MANY>
 __global__ void __launch_bounds__(32 * RouteShape<V, SELECT, STATS, MANY>::kWarps, 1) route_kernel(const RouteParams a, const RouteFinish f) {
   using Shape = RouteShape<V, SELECT, STATS, MANY>;
@@ -845,9 +846,11 @@ __global__ void __launch_bounds__(256, BALANCE ? 3 : 6) route_backward_kernel(co
 
 // Whether one cluster makes the statistics in one launch.  Measured at 512
 // experts fp32, one cluster against CTAs of eight rows and the launch that
-// joins them: statistics of 250 rows 5.3 and 5.2 us, of 512 rows 6.7 and 5.5,
-// of 700 rows 8.0 and 6.0; with the selection 100 rows 5.8 and 6.1, 160 rows
-// 7.4 and 6.2, 250 rows 8.1 and 6.5.  The second launch costs the host 1.2 us.
+// joins them: statistics of 250 rows 5.0 and 5.1 us, of 512 rows 6.3 and 5.3,
+// of 700 rows 7.7 and 5.8; with the selection 100 rows 5.8 and 5.9, 160 rows
+// 7.3 and 6.1, 250 rows 7.9 and 6.2.  The second launch costs the host 1.2 us,
+// which is what a call that is not replayed from a graph waits for: the rule
+// takes the cluster until the device time outweighs that.
 inline bool route_one_cluster(unsigned tokens, bool select) { return tokens <= (select ? 160 : 512); }
 
 // CTAs that make statistics of `tokens` rows: one part of the sums each.

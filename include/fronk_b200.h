@@ -266,7 +266,9 @@ int frc_matrix_check(unsigned type, unsigned rows, unsigned n);
  * after row; host or device memory, ready when the call is made) into HBM and
  * checks every scale: FRC_NUMERIC when one is not finite (MXFP4 exponent 255
  * too), FRC_UNSUPPORTED when scales of one MXFP4 row lie more than 2^229 apart
- * (those of blocks without a weight other than zero do not count).
+ * (those of blocks without a weight other than zero do not count).  The
+ * matrix holds the rows in a layout of its own: the caller's copy is not
+ * needed after the call, and until it is freed both are in memory.
  * Synchronous.  The matrix belongs to the context's device, works with
  * any context of that device and may outlive the one that opened it. */
 int frc_matrix_open(frc_context *c, unsigned type, unsigned rows, unsigned n, const void *bytes, size_t len,
@@ -280,10 +282,12 @@ int frc_matrix_close(frc_matrix *m);
  * for one token.  x and y must not overlap.  A result that is not finite
  * (or whose x is not) sets FRC_NUMERIC in the context's device status
  * (frc_status).  Concurrent calls on several streams are independent.  The
- * same call repeats its bits; the last bits of a row may depend on where it
- * lies in the matrix.  x is carried to 2^-30 (Q4_K, up to 4 tokens) or to 22
- * bits and 2^-34 of the largest value among its 256 neighbours that share a
- * block of columns. */
+ * same call repeats its bits; the last bits of a result may depend on the
+ * row's place in the matrix and on the number and type of the tokens, so that
+ * a token's router logits in a burst need not equal those of a call of its
+ * own, and near ties may choose other experts.  x is carried to 2^-30 (Q4_K,
+ * up to 4 tokens) or to 22 bits and 2^-34 of the largest value among its 256
+ * neighbours that share a block of columns. */
 int frc_matvec_device(frc_context *c, const frc_matrix *m, unsigned tokens, const void *x, size_t x_stride,
                       unsigned x_type, void *y, size_t y_stride, unsigned y_type, void *stream);
 
