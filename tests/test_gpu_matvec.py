@@ -511,3 +511,20 @@ def test_one_span_at_a_time(ctx, type_, n, tokens, x_type):
                 xs, ys = host(xd[t:t + 1, cols]), host(yd[t:t + 1])
                 ref, tol = xs @ w[:, cols].T, bound(a[:, cols], xs, xs.shape[1])
                 assert np.all(np.abs(ys - ref) <= tol), (s, (np.abs(ys - ref) / tol).max())
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 3, 5, 16])
+@pytest.mark.parametrize("x_type", [fb.F32, fb.BF16])
+@pytest.mark.parametrize("exponent", [0, 228, 229, 230, 254])
+def test_largest_sums(ctx, exponent, x_type, tokens):
+    """Every weight 6, every x just under a power of two: the largest sum a span can have, at the scales around which
+    rows take a common shift."""
+    n, rows = 1024, 20
+    rng = np.random.default_rng(36)
+    raw = quant.random_rows(fb.MXFP4, rows, n, rng, (exponent, exponent + 1))
+    raw.reshape(rows, n // 32, 17)[..., 1:] = 0x77
+    w, a = quant.weights(fb.MXFP4, raw, n)
+    xd = to_device(np.full((tokens, n), (2.0 - 2.0 ** -7) * 2.0 ** (80 if exponent == 0 else -60)), x_type)
+    x = host(xd)
+    y = host(run(ctx, fb.MXFP4, raw, n, xd, x_type, fb.F32))
+    assert np.all(np.abs(y - x @ w.T) <= bound(a, x, n) + 2.0 ** -126)
